@@ -11,6 +11,7 @@ tensor-core kernel covers the shape; the 32-bit path always uses the engine's ow
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -25,6 +26,8 @@ DELTA_RULE_SOURCES = ["delta_rule.cu"]             # likewise for the gated delt
 DIFF_ATTENTION_SOURCES = ["attention_diff.cu"]     # likewise for differential attention
 MOE_SOURCES = ["moe.cu", "moe_grouped.cu", "moe_grouped_tc.cu"]   # likewise for a feed-forward of routed experts
 SEQUENCE_SOURCES = ["sequence_filters.cu"]         # likewise for an embedding that reads the token before, a convolution in front of a sublayer
+SHARED_PREFIX_SOURCES = ["attention_shared_prefix.cu"]   # likewise for attention over a prefix that a batch shares
+SAMPLE_FILTERED_SOURCES = ["sample_filtered.cu"]   # likewise for a choice of tokens with top-k or min-p
 _F32, _BF16 = 0, 1
 launch_count = 0  # kernels of this engine launched by this process (a claim the bench reports)
 
@@ -43,7 +46,8 @@ def build_all() -> list:
     return [build_library("tlie_core", CORE_SOURCES), build_library("tlie_recurrent", RECURRENT_SOURCES),
             build_library("tlie_attention_mixed", MIXED_ATTENTION_SOURCES), build_library(f"tlie_delta_rule_l{DELTA_LANES}", DELTA_RULE_SOURCES, {"TLIE_DELTA_LANES": DELTA_LANES}),
             build_library("tlie_attention_diff", DIFF_ATTENTION_SOURCES), build_library("tlie_moe", MOE_SOURCES),
-            build_library("tlie_sequence", SEQUENCE_SOURCES)] + fast.build_all()
+            build_library("tlie_sequence", SEQUENCE_SOURCES), build_library("tlie_shared_prefix", SHARED_PREFIX_SOURCES),
+            build_library("tlie_sample_filtered", SAMPLE_FILTERED_SOURCES)] + fast.build_all()
 
 
 def _code(tensor: torch.Tensor) -> int:
@@ -98,7 +102,8 @@ def _i32(tensor: torch.Tensor | None, what: str) -> c_void_p:
 _error_flags: dict[torch.device, torch.Tensor] = {}
 DEVICE_ERRORS = {1: "a bounded wait inside a tensor-core kernel gave up; the step's results are not valid",
                  2: "a token id outside the vocabulary reached the embedding kernel (non-finite logits upstream?)",
-                 4: "a position beyond the table of learned position vectors reached the embedding kernel"}
+                 4: "a position beyond the table of learned position vectors reached the embedding kernel",
+                 8: "a position beyond the block table, or a page outside the pool, reached the attention over a shared prefix (page 0 was read instead)"}
 
 
 def error_flag(device: torch.device) -> torch.Tensor:
@@ -659,6 +664,77 @@ def attention_step(qkv, positions, token_seq, block_table, inv_freq, rotary_dim:
             return
     rope_store(qkv, positions, token_seq, block_table, inv_freq, rotary_dim, pages, q_heads, kv_heads, head_dim, page_size, write_cache)
     paged_attention(qkv, pages, positions, token_seq, block_table, out, q_heads, kv_heads, head_dim, page_size, window, scale, batch)
+
+
+def shared_prefix():
+    return load_library("tlie_shared_prefix", SHARED_PREFIX_SOURCES)
+
+
+def _one_device(what: str, **tensors) -> torch.device:
+    """The CUDA device that all of these tensors lie on; anything else raises."""
+    devices = {tensor.device for tensor in tensors.values()}
+    if any(device.type != "cuda" for device in devices):
+        raise KernelError(f"this engine has no CPU path: {what} was given a tensor that is not on a CUDA device")
+    if len(devices) != 1:
+        raise KernelError(f"{what}: all tensors must lie on one device, got " + ", ".join(f"{name} on {tensor.device}" for name, tensor in tensors.items()), code="invalid_argument")
+    return devices.pop()
+
+
+def _on(device: torch.device):
+    """Launches inside go to this device, whichever is the current one."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared: int, out, q_heads: int, kv_heads: int, head_dim: int, page_size: int,
+                            scale: float | None = None) -> None:
+    """``paged_attention`` for a batch whose requests share their first ``shared`` cached keys: answers to one prompt, questions behind one system prompt.
+
+    Row t of ``qkv`` (its first ``q_heads * head_dim`` columns: the rotated query heads; rows may be a run of columns of wider ones) belongs to the entry b
+    with ``seq_starts[b] <= t < seq_starts[b + 1]`` and attends to that request's cached keys up to ``positions[t]``.  Keys below ``shared`` are read through row 0 of
+    ``block_table`` once for the whole batch, whose rows must name the same pages (or copies of them) there; ``shared`` need not end a page, and a request's own
+    keys may lie in the rest of that page or of its copy.  An entry brings any number of rows, none included.  Rows in front of ``seq_starts[0]`` and behind ``seq_starts[-1]`` are left as they
+    were; a row that sees no key (a negative position) becomes zero.  Positions that the block table does not reach and pages outside the pool are reported in
+    the device's error word.  ``scale``: positive, ``head_dim ** -0.5`` by default.  32-bit or bfloat16, head sizes that are multiples of 16 up to 256.
+
+    Called inside the capture of a CUDA graph, the graph keeps ``shared`` and the tensors' addresses; what the tensors hold may change from replay to replay."""
+    if head_dim % 16 != 0 or not 0 < head_dim <= 256:
+        raise KernelError(f"attention kernels take head sizes that are multiples of 16 up to 256, got {head_dim}", code="invalid_shape")
+    if kv_heads < 1 or q_heads < 1 or q_heads % kv_heads != 0:
+        raise KernelError("attention: query heads must be a multiple of key/value heads", code="invalid_shape")
+    if qkv.dim() != 2 or qkv.shape[1] < q_heads * head_dim or (qkv.shape[0] > 0 and qkv.stride(1) != 1):
+        raise KernelError("shared_prefix_attention: qkv must be [rows, at least q_heads * head_dim] with contiguous rows", code="invalid_shape")
+    rows, entries = qkv.shape[0], block_table.shape[0]
+    if out.shape != (rows, q_heads * head_dim) or out.dtype != qkv.dtype:
+        raise KernelError("shared_prefix_attention: out must be [rows, q_heads * head_dim] of qkv's dtype", code="invalid_shape")
+    if pages.dim() != 5 or tuple(pages.shape[1:]) != (2, kv_heads, page_size, head_dim) or pages.dtype != qkv.dtype or pages.shape[0] < 1:
+        raise KernelError("shared_prefix_attention: pages must be [pages, 2, kv heads, page size, head size] of qkv's dtype", code="invalid_shape")
+    if block_table.dim() != 2 or tuple(seq_starts.shape) != (entries + 1,) or tuple(positions.shape) != (rows,):
+        raise KernelError("shared_prefix_attention: a block table [entries, pages], seq_starts [entries + 1] and positions [rows]", code="invalid_shape")
+    if isinstance(shared, bool) or not isinstance(shared, int) or not 0 <= shared <= block_table.shape[1] * page_size:
+        raise KernelError(f"shared_prefix_attention: shared must be a whole number from 0 to the {block_table.shape[1] * page_size} keys that a block-table row reaches, got {shared!r}",
+                          code="invalid_argument")
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise KernelError(f"shared_prefix_attention: scale must be positive and finite, got {scale}", code="invalid_argument")
+    _code(qkv)
+    if any(t.dtype != torch.int32 for t in (positions, seq_starts, block_table)):
+        raise KernelError("shared_prefix_attention: positions, seq_starts and the block table are int32", code="invalid_dtype")
+    device = _one_device("shared_prefix_attention", qkv=qkv, pages=pages, positions=positions, seq_starts=seq_starts, block_table=block_table, out=out)
+    if rows == 0 or entries == 0:
+        return
+    with _on(device):
+        tiles = -(-rows * (q_heads // kv_heads) // 32) * kv_heads
+        prefix_parts = 0 if shared == 0 else max(1, min(-(-4 * fast.sm_count() // tiles), -(-shared // 128), 64))
+        own_parts = max(1, min(2 * fast.sm_count() // (tiles + entries * kv_heads), -(-(block_table.shape[1] * page_size - shared) // 256), 16))
+        buffer = torch.empty(rows * q_heads * (prefix_parts + own_parts) * (head_dim + 2), dtype=torch.float32, device=device)
+        _check(
+            shared_prefix().tlie_shared_prefix_generic(
+                _code(qkv), c_void_p(qkv.data_ptr()), c_longlong(qkv.stride(0)), _ptr(pages), c_int(pages.shape[0]), _i32(positions, "positions"), _i32(seq_starts, "seq_starts"),
+                _i32(block_table, "block_table"), c_int(block_table.shape[1]), _ptr(out), _ptr(buffer), c_int(rows), c_int(entries), c_int(q_heads), c_int(kv_heads),
+                c_int(head_dim), c_int(page_size), c_int(shared), c_float(scale), c_int(prefix_parts), c_int(own_parts), _ptr(error_flag(device)), _stream(),
+            ),
+            "shared_prefix_attention",
+        )
 
 
 # --- recurrences ---------------------------------------------------------------------------
@@ -1319,6 +1395,62 @@ def sample(logits, temperature, top_p, seeds, counters, out) -> None:
         core().tlie_sample(_ptr(logits), c_int(logits.shape[0]), c_int(logits.shape[1]), _ptr(temperature), _ptr(top_p), _ptr(seeds), _ptr(counters), _i32(out, "out"), _stream()),
         "sample",
     )
+
+
+def filtered_sampling():
+    return load_library("tlie_sample_filtered", SAMPLE_FILTERED_SOURCES)
+
+
+SAMPLE_FILTERED_MAX_VOCAB = 1 << 19    # sums of that many weights of 2^44 and less fit 64 bits (csrc/sample_filtered.cu)
+
+
+def sample_filtered(logits, temperature, top_k, top_p, min_p, uniforms, out, rows=None) -> None:
+    """One token per row of 32-bit ``logits`` [R, vocab] (rows may be a run of columns of wider ones), drawn with the number ``uniforms[r]`` in [0, 1).
+
+    A row's tokens are ordered by logit, the lower id first among equals; token i weighs w_i = exp((l_i - max) / temperature).  Kept is the shortest of three prefixes
+    of that order, and the first token always: ``top_k`` tokens (0 or less: all); the fewest whose weights reach ``top_p`` of the weight that top-k leaves (1 or more: all); those with
+    w_i >= ``min_p``.  ``out[r]`` is the first kept token, in order of ids, at which the running sum of kept weights exceeds ``uniforms[r]`` times their sum.  Rows
+    with a temperature that is not above 0 take the first token of the order, rows of NaN token 0.  Sums are exact, so a row's token
+    depends on nothing but its own logits and options.
+
+    temperature, top_p, min_p and uniforms are 32-bit floats, top_k int32, one per row.  ``rows`` (int32): the r-th options are for row ``rows[r]`` of
+    the logits and of ``out``, each named once; numbers outside the logits (-1, say) are passed over, and rows that nobody names keep what ``out`` holds."""
+    count = logits.shape[0] if rows is None else rows.shape[0]
+    given = {"logits": logits, "temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p, "uniforms": uniforms, "out": out}
+    if rows is not None:
+        given["rows"] = rows
+    vocab = logits.shape[1] if logits.dim() == 2 else 0
+    if logits.dtype != torch.float32 or any(t.dtype != torch.float32 for t in (temperature, top_p, min_p, uniforms)):
+        raise KernelError("sampling takes 32-bit logits, temperatures, top_p, min_p and uniform numbers", code="invalid_dtype")
+    if any(t.dtype != torch.int32 for t in (top_k, out, top_k if rows is None else rows)):
+        raise KernelError("sample_filtered: top_k, out and rows are int32", code="invalid_dtype")
+    if not 0 < vocab <= SAMPLE_FILTERED_MAX_VOCAB or (vocab > 1 and logits.stride(1) != 1):
+        raise KernelError(f"sample_filtered: logits must be [rows, 1 to {SAMPLE_FILTERED_MAX_VOCAB} tokens] with contiguous rows", code="invalid_shape")
+    if any(tuple(t.shape) != (count,) for t in (temperature, top_k, top_p, min_p, uniforms)) or tuple(out.shape) != (logits.shape[0],) or (rows is not None and rows.dim() != 1):
+        raise KernelError("sample_filtered: one temperature, top_k, top_p, min_p and uniform number per row, and out [rows of the logits]", code="invalid_shape")
+    device = _one_device("sample_filtered", **given)
+    if count == 0 or logits.shape[0] == 0:
+        return
+    with _on(device):
+        _check(
+            filtered_sampling().tlie_sample_filtered(
+                c_void_p(logits.data_ptr()), c_longlong(logits.stride(0)), c_int(logits.shape[0]), c_int(vocab), _i32(rows, "rows"), c_int(count), _ptr(temperature),
+                _i32(top_k, "top_k"), _ptr(top_p), _ptr(min_p), _ptr(uniforms), _i32(out, "out"), _stream(),
+            ),
+            "sample_filtered",
+        )
+
+
+def uniforms(seeds, counters, out) -> None:
+    """out[r] = ``uniform_from(seeds[r], counters[r])``: the numbers that ``sample`` draws with, for ``sample_filtered``."""
+    if seeds.dtype != torch.int64 or counters.dtype != torch.int64 or out.dtype != torch.float32:
+        raise KernelError("uniforms takes int64 seeds and counters and gives 32-bit numbers", code="invalid_dtype")
+    if seeds.shape != counters.shape or out.shape != seeds.shape:
+        raise KernelError("uniforms: one number per seed and counter", code="invalid_shape")
+    device = _one_device("uniforms", seeds=seeds, counters=counters, out=out)
+    if out.numel() > 0:
+        with _on(device):
+            _check(filtered_sampling().tlie_uniforms(_ptr(seeds), _ptr(counters), _ptr(out), c_int(out.numel()), _stream()), "uniforms")
 
 
 def decode_advance(token_ids, sampled, positions, seq_lens, first_positions, counters, mailbox=None, steps_done=None) -> None:
