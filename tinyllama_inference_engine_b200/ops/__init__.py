@@ -26,7 +26,7 @@ DELTA_RULE_SOURCES = ["delta_rule.cu"]             # likewise for the gated delt
 DIFF_ATTENTION_SOURCES = ["attention_diff.cu"]     # likewise for differential attention
 MOE_SOURCES = ["moe.cu", "moe_grouped.cu", "moe_grouped_tc.cu"]   # likewise for a feed-forward of routed experts
 SEQUENCE_SOURCES = ["sequence_filters.cu"]         # likewise for an embedding that reads the token before, a convolution in front of a sublayer
-SHARED_PREFIX_SOURCES = ["attention_shared_prefix.cu"]   # likewise for attention over a prefix that a batch shares
+SHARED_PREFIX_SOURCES = ["attention_shared_prefix.cu", "attention_prefix_rows.cu"]   # likewise for attention over a prefix that a batch shares
 SAMPLE_FILTERED_SOURCES = ["sample_filtered.cu"]   # likewise for a choice of tokens with top-k or min-p
 _F32, _BF16 = 0, 1
 launch_count = 0  # kernels of this engine launched by this process (a claim the bench reports)
@@ -719,10 +719,14 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     _code(qkv)
     if any(t.dtype != torch.int32 for t in (positions, seq_starts, block_table)):
         raise KernelError("shared_prefix_attention: positions, seq_starts and the block table are int32", code="invalid_dtype")
+    if not all(t.is_contiguous() for t in (pages, positions, seq_starts, block_table, out)):
+        raise KernelError("kernels take contiguous tensors")
     device = _one_device("shared_prefix_attention", qkv=qkv, pages=pages, positions=positions, seq_starts=seq_starts, block_table=block_table, out=out)
     if rows == 0 or entries == 0:
         return
     with _on(device):
+        if fast.shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale):
+            return
         tiles = -(-rows * (q_heads // kv_heads) // 32) * kv_heads
         prefix_parts = 0 if shared == 0 else max(1, min(-(-4 * fast.sm_count() // tiles), -(-shared // 128), 64))
         own_parts = max(1, min(2 * fast.sm_count() // (tiles + entries * kv_heads), -(-(block_table.shape[1] * page_size - shared) // 256), 16))

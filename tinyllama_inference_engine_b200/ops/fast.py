@@ -1192,3 +1192,47 @@ def moe_grouped(x, gate_up, down, ids, weights, shared, out, kind: int, weight_i
                                                   ops._ptr(meta), ops._ptr(act), ops._ptr(y), ops._ptr(out), c_int(tokens), c_int(width), c_int(ff), c_int(experts), c_int(top),
                                                   c_int(kind), c_int(1 if weight_input else 0), *clamp, ops._stream()), "moe_grouped")
     ops.launch_count += 3   # four kernels: the sort, two products per expert, the sum
+
+
+# --- attention over a prefix that a batch shares ------------------------------------------------
+SHARED_PREFIX_HEAD_DIMS = (64, 128)
+PREFIX_ROWS_MAX_CTAS = 8      # CTAs of a cluster that share a row's keys
+
+
+def shared_prefix_library():
+    """The kernels of attention over a shared prefix; their launchers take plain Python numbers."""
+    lib = _ops().shared_prefix()
+    if not getattr(lib, "_tlie_typed", False):
+        pointer, i32, i64 = c_void_p, c_int, c_longlong
+        lib.tlie_prefix_rows.argtypes = [pointer, i64, pointer, i32, pointer, pointer, pointer, i32, pointer, pointer, pointer, i32, i32, i32, i32, i32, i32, i32, i32, c_float, i32, pointer, pointer]
+        lib._tlie_typed = True
+    return lib
+
+
+def shared_prefix_takes(qkv, pages, out, page_size: int, head_dim: int) -> bool:
+    """Whether the bfloat16 kernels for head sizes 64 and 128 can read these tensors: 16 bytes at a time, pages of a multiple of 16 keys."""
+    return (qkv.dtype == torch.bfloat16 and head_dim in SHARED_PREFIX_HEAD_DIMS and page_size % 16 == 0 and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0
+            and pages.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
+
+
+def prefix_rows_ctas(rows: int, kv_heads: int, group: int, keys: int) -> int:
+    """CTAs per (row, key/value head): as many as keep two on every SM, each with at least 128 keys to read."""
+    pairs = rows * kv_heads * -(-group // 16)
+    ctas = 1
+    while ctas < PREFIX_ROWS_MAX_CTAS and pairs * ctas * 2 <= 2 * sm_count() and keys > 128 * ctas:
+        ctas *= 2
+    return ctas
+
+
+def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared: int, out, q_heads: int, kv_heads: int, head_dim: int, page_size: int, scale: float) -> bool:
+    """bfloat16 attention over a shared prefix on the kernels made for it; False if they do not take the call."""
+    rows, entries, width = qkv.shape[0], block_table.shape[0], block_table.shape[1]
+    if rows > entries or not shared_prefix_takes(qkv, pages, out, page_size, head_dim):
+        return False
+    ops = _ops()
+    lib = shared_prefix_library()
+    ctas = prefix_rows_ctas(rows, kv_heads, q_heads // kv_heads, width * page_size)
+    ops._check(lib.tlie_prefix_rows(qkv.data_ptr(), qkv.stride(0), pages.data_ptr(), pages.shape[0], positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), width,
+                                    out.data_ptr(), 0, 0, 0, rows, entries, q_heads, kv_heads, head_dim, page_size, 0, scale, ctas, ops.error_flag(qkv.device).data_ptr(),
+                                    ops._stream()), "prefix_rows")
+    return True
