@@ -26,7 +26,7 @@ DELTA_RULE_SOURCES = ["delta_rule.cu"]             # likewise for the gated delt
 DIFF_ATTENTION_SOURCES = ["attention_diff.cu"]     # likewise for differential attention
 MOE_SOURCES = ["moe.cu", "moe_grouped.cu", "moe_grouped_tc.cu"]   # likewise for a feed-forward of routed experts
 SEQUENCE_SOURCES = ["sequence_filters.cu"]         # likewise for an embedding that reads the token before, a convolution in front of a sublayer
-SHARED_PREFIX_SOURCES = ["attention_shared_prefix.cu", "attention_prefix_rows.cu"]   # likewise for attention over a prefix that a batch shares
+SHARED_PREFIX_SOURCES = ["attention_shared_prefix.cu", "attention_prefix_rows.cu", "attention_prefix_tc.cu"]   # likewise for attention over a prefix that a batch shares
 SAMPLE_FILTERED_SOURCES = ["sample_filtered.cu"]   # likewise for a choice of tokens with top-k or min-p
 _F32, _BF16 = 0, 1
 launch_count = 0  # kernels of this engine launched by this process (a claim the bench reports)

@@ -1205,6 +1205,7 @@ def shared_prefix_library():
     if not getattr(lib, "_tlie_typed", False):
         pointer, i32, i64 = c_void_p, c_int, c_longlong
         lib.tlie_prefix_rows.argtypes = [pointer, i64, pointer, i32, pointer, pointer, pointer, i32, pointer, pointer, pointer, i32, i32, i32, i32, i32, i32, i32, i32, c_float, i32, pointer, pointer]
+        lib.tlie_prefix_tc.argtypes = [i32, pointer, i64, pointer, i32, pointer, pointer, pointer, i32, pointer, pointer, pointer, i32, i32, i32, i32, i32, i32, i32, i32, i32, c_float, pointer, pointer]
         lib._tlie_typed = True
     return lib
 
@@ -1224,15 +1225,46 @@ def prefix_rows_ctas(rows: int, kv_heads: int, group: int, keys: int) -> int:
     return ctas
 
 
+PREFIX_TC_PAIRS = 128         # (row, head) pairs of a row tile of the tensor-core kernel, of which a CTA has two (csrc/attention_prefix_tc.cu)
+PREFIX_TC_KEYS = 128          # keys of one of its key tiles
+
+
+def prefix_tc_parts(rows: int, kv_heads: int, group: int, shared: int) -> int:
+    """Runs that the prefix's key tiles are cut into: what makes the longest SM's share of them least, an item's own start and end counted as two key tiles."""
+    tiles = -(-shared // PREFIX_TC_KEYS)
+    items = -(-rows // (2 * (PREFIX_TC_PAIRS // group))) * kv_heads
+    best, cost = 1, None
+    for parts in range(1, min(tiles, 32) + 1):
+        here = -(-items * parts // sm_count()) * (-(-tiles // parts) + 2)
+        if cost is None or here < cost:
+            best, cost = parts, here
+    return best
+
+
 def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared: int, out, q_heads: int, kv_heads: int, head_dim: int, page_size: int, scale: float) -> bool:
     """bfloat16 attention over a shared prefix on the kernels made for it; False if they do not take the call."""
-    rows, entries, width = qkv.shape[0], block_table.shape[0], block_table.shape[1]
-    if rows > entries or not shared_prefix_takes(qkv, pages, out, page_size, head_dim):
+    rows, entries, width, group = qkv.shape[0], block_table.shape[0], block_table.shape[1], q_heads // kv_heads
+    if group > PREFIX_TC_PAIRS or not shared_prefix_takes(qkv, pages, out, page_size, head_dim):
         return False
     ops = _ops()
     lib = shared_prefix_library()
-    ctas = prefix_rows_ctas(rows, kv_heads, q_heads // kv_heads, width * page_size)
-    ops._check(lib.tlie_prefix_rows(qkv.data_ptr(), qkv.stride(0), pages.data_ptr(), pages.shape[0], positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), width,
-                                    out.data_ptr(), 0, 0, 0, rows, entries, q_heads, kv_heads, head_dim, page_size, 0, scale, ctas, ops.error_flag(qkv.device).data_ptr(),
-                                    ops._stream()), "prefix_rows")
+    common = (qkv.data_ptr(), qkv.stride(0), pages.data_ptr(), pages.shape[0], positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), width, out.data_ptr())
+    sizes = (rows, entries, q_heads, kv_heads, head_dim, page_size)
+    flag, stream = ops.error_flag(qkv.device).data_ptr(), ops._stream()
+    parts, part_ml, part_o, first_key = 0, 0, 0, 0
+    if PREFIX_MODE and shared > 0:
+        parts = prefix_tc_parts(rows, kv_heads, group, shared)
+        buffer = torch.empty(rows * q_heads * parts * (head_dim + 2), dtype=torch.float32, device=qkv.device)
+        part_o = buffer.data_ptr()
+        part_ml = part_o + 4 * rows * q_heads * parts * head_dim
+        ops._check(lib.tlie_prefix_tc(0, *common, part_ml, part_o, parts, *sizes, shared, 0, scale, flag, stream), "prefix_tc")
+        first_key = shared
+    if rows > entries:
+        ops._check(lib.tlie_prefix_tc(1, *common, part_ml, part_o, parts, *sizes, shared, first_key, scale, flag, stream), "prefix_tc")
+    else:
+        ctas = prefix_rows_ctas(rows, kv_heads, group, width * page_size - first_key)
+        ops._check(lib.tlie_prefix_rows(*common, part_ml, part_o, parts, *sizes, first_key, scale, ctas, flag, stream), "prefix_rows")
     return True
+
+
+PREFIX_MODE = True
