@@ -6,29 +6,31 @@
 //     to the finished output.  With first_key = 0 it is the whole attention of portions of many rows.
 //
 // The query heads of a group meet the same keys: a row tile is 128 (row, head of the group) pairs, 128 / group rows of the step.  A CTA has two such tiles and a
-// ring of key and value tiles (128 keys) for both, so that keys and values come from L2 once per 256 pairs, and so that one tile's products run
-// under the other's softmax: with 512 columns of tensor memory there is one score buffer and one output per tile (128 columns each), and what is in turn for a tile (scores, softmax,
-// weighted values) alternates between the two.  One CTA fills an SM.
+// ring of key and value tiles for both, so that keys and values come from L2 once per 256 pairs.  One CTA fills an SM.
 //   * TMA brings Q once (a box of 64 dims x the group's heads x 128 / group rows per half), and every key tile as boxes that lie inside a page.  The lanes of
 //     the producing warp each look up one box's page and copy it;
-//   * S = Q . K^T (128 x 128 x head size) and O += P . V (128 x head size x 128) are issued by one thread per row tile.  P lies in tensor memory, over the
-//     first half of its scores, and is handed over in halves: the product of the first 64 keys runs under the exponentials of the others;
+//   * S = Q . K^T (a warp per row tile) and O += P . V are issued by warps of their own.  P has a place of its own in tensor memory: scores may be written again as soon as the softmax threads
+//     have them in registers, so the next scores are computed under this tile's softmax, and a softmax thread finds its next scores waiting.  With the weights over
+//     the scores (128 keys at both head sizes), scores, softmax and weighted values of a row tile were a chain that the other tile's could only half
+//     fill: 3,900 cycles per 128 keys and two row tiles at head size 128, where the tensor core has 2,050 and the exponential unit 2,050 to do.  512 columns of tensor
+//     memory hold, twice, output, scores and weights of 64 dims and 128 keys, or of 128 dims and 80 keys;
 //   * thread = (row, head) pair = lane of tensor memory: maxima and sums need no other thread.  The output is taken against a reference maximum that
 //     moves only when a tile's maximum is more than 2^8 above it;
 //   * what a tile's rows do not all see is masked; a value that some of them see and that is not finite would spread through a weight of zero, so in such tiles values are looked
 //     through, what is not finite is taken out and noted, and the rows that do see it show it in the end.
 // Every wait is bounded; a CTA that gives up raises the device's error word, lets its copies land and returns.
+#include <type_traits>
+
 #include "shared_memory_limit.cuh"
 #include "tcgen05_utils.cuh"
 
 namespace tlie {
 
 constexpr int kPairsTC = 128;       // (row, head) pairs of a row tile
-constexpr int kKeysTC = 128;        // keys of a key tile
 constexpr int kBoxDims = 64;        // dims of one box: 128 bytes, the swizzle span
-constexpr int kThreadsTC = 384;     // warps 0 copies, 1 and 2 products, 3 none, 4 to 7 and 8 to 11 softmax of the two row tiles
-constexpr int kFirstSoftmaxWarp = 4;
-constexpr int kControlRegs = 56, kSoftmaxRegs = 224, kLaunchRegs = 168;   // 128 * 56 + 256 * 224 = 384 * 168
+constexpr int kThreadsTC = 512;     // warps 0 copies keys, 1 values, 2 and 3 scores of the two row tiles, 4 weighted values, 5 to 7 none, 8 to 11 and 12 to 15 softmax of the row tiles
+constexpr int kFirstSoftmaxWarp = 8;
+constexpr int kControlRegs = 56, kSoftmaxRegs = 200, kLaunchRegs = 128;   // 256 * 56 + 256 * 200 = 512 * 128
 constexpr float kToLog2 = 1.4426950408889634f;
 constexpr float kLazyRescale = 8.0f;
 constexpr int kBadPage = 8;         // the bit of the device's error word
@@ -37,24 +39,23 @@ constexpr int kNoKey = 0x7fffffff;
 // bf16 x bf16 -> f32, A K-major, B MN-major (V stays [key][dim], as the cache stores it), tile m x n.
 __host__ __device__ constexpr uint32_t instr_desc_b_mn(int m, int n) { return umma_instr_desc(m, n) | (1u << 16); }
 
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
-  uint32_t r[32], s[32];
-  tmem_load_32(taddr, r);
-  tmem_load_32(taddr + 32, s);
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]), v[32 + i] = __uint_as_float(s[i]);
+// Columns of this thread's lane written from registers (not waited for).
+__device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+               "r"(r[6]), "r"(r[7])
+               : "memory");
 }
-__device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
-      "%23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-      "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+__device__ __forceinline__ void tmem_store_4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
+// ... and read into them (not waited for).
+__device__ __forceinline__ void tmem_load_8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+// The four softmax warps of row tile u meet.
+__device__ __forceinline__ void tile_barrier(int u) { asm volatile("bar.sync %0, 128;\n" ::"r"(1 + u) : "memory"); }
 // The product with its A operand in tensor memory (lane = row, 16 k = 8 columns of two bfloat16) and B by its descriptor's lower word.
 __device__ __forceinline__ void umma_bf16_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -99,9 +100,39 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   return r;
 }
 
+// One lane of the (converged) warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(elected));
+  return elected != 0;
+}
+
 // A whole warp waits: what follows is warp-wide, so the lanes go on or give up together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+}
+
+// Non-zero where one of two bfloat16 numbers is infinite or NaN (an exponent of ones carries into the sign's place).
+__device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+// Of eight values of a key those that are not finite become zero, and the first such key is noted per dim: at bad[dim] for +infinity, `dims` further for -infinity, as much
+// again for NaN.
+__device__ __forceinline__ void take_out(uint16_t* eight, int* bad, int dims, int key, int* any_bad) {
+#pragma unroll 1
+  for (int w = 0; w < 8; ++w) {
+    const uint32_t bits = eight[w];
+    if ((bits & 0x7f80u) != 0x7f80u) continue;
+    atomicMin(bad + ((bits & 0x7fu) != 0u ? 2 : bits >> 15) * dims + w, key);
+    *(volatile int*)any_bad = 1;
+    __threadfence_block();
+    eight[w] = 0;
+  }
 }
 
 struct PrefixTCParams {
@@ -119,19 +150,22 @@ struct PrefixTCParams {
 };
 
 template <int D>
+constexpr int kKeysOf = D <= 64 ? 128 : 80;   // keys of a key tile
+
+template <int D>
 struct SmemPrefix {
-  static constexpr int kStages = D <= 64 ? 3 : 2;
+  static constexpr int kKeys = kKeysOf<D>, kStages = D <= 64 ? 4 : 3;
   // 1024-byte aligned, each a run of sub-tiles [rows][64] of 64 dims in the 128-byte swizzle
   __nv_bfloat16 q[2][kPairsTC * D];
-  __nv_bfloat16 k[kStages][kKeysTC * D];
-  __nv_bfloat16 v[kStages][kKeysTC * D];
+  __nv_bfloat16 k[kStages][kKeys * D];
+  __nv_bfloat16 v[kStages][kKeys * D];
   int bad[3][D];                 // per dim the first key whose value is +infinity, -infinity, NaN and was taken out
   int lowest[2], last[2];        // the fewest and the most keys that a row of each row tile sees
   int entry, token0, tokens;     // OWN: whose rows, the first one of this CTA, how many
   int any_bad;
-  // k_full, v_full: a tile has landed.  k_empty, v_empty: both row tiles' products have read it.  s_full: a row tile's scores are there.  p_full: a half of its weights is.  pv_done:
-  // its weighted values are added.
-  uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2][2], pv_done[2];
+  // k_full, v_full: a tile has landed.  k_empty, v_empty: both row tiles' products have read it.  s_full: a row tile's scores are there; s_read: its threads have
+  // them.  p_full: its weights are there; pv_done: its weighted values are added.
+  uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], s_read[2], p_full[2], pv_done[2], exps_done[2][4];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -141,27 +175,30 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const PrefixTCParams p) {
   extern __shared__ uint8_t smem_raw[];
   using Smem = SmemPrefix<D>;
-  constexpr int kStages = Smem::kStages, kHalves = D / kBoxDims;
+  constexpr int kStages = Smem::kStages, kKeys = Smem::kKeys, kHalves = D / kBoxDims;
   Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   volatile int* abort_flag = &sm.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = OWN ? blockIdx.x : blockIdx.y;
   const int group = p.q_heads / p.kv_heads, tile_tokens = kPairsTC / group;
-  constexpr int kTmemCols = 512, kOutCol0 = 256;   // S of the two row tiles at 0 and 128, their outputs at 256 and 384
+  // tensor memory: the two row tiles' outputs, scores and weights (two keys a column)
+  constexpr int kTmemCols = 512, kScoreCol0 = 2 * D, kWeightCol0 = kScoreCol0 + 2 * kKeys, kWeightCols = (kKeys / 2 + 15) / 16 * 16;
+  static_assert(kWeightCol0 + 2 * kWeightCols <= kTmemCols && kKeys % 16 == 0, "tensor memory holds 512 columns");
 
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sm.k_full[s], 1);
       mbar_init(&sm.v_full[s], 1);
-      mbar_init(&sm.k_empty[s], 2);
-      mbar_init(&sm.v_empty[s], 2);
+      mbar_init(&sm.k_empty[s], 2);   // a commit per row tile
+      mbar_init(&sm.v_empty[s], 1);
     }
     for (int u = 0; u < 2; ++u) {
+      for (int w = 0; w < 4; ++w) mbar_init(&sm.exps_done[u][w], 1);
       mbar_init(&sm.s_full[u], 1);
       mbar_init(&sm.pv_done[u], 1);
-      mbar_init(&sm.p_full[u][0], 4);   // one arrival per softmax warp
-      mbar_init(&sm.p_full[u][1], 4);
+      mbar_init(&sm.s_read[u], 4);   // one arrival per softmax warp
+      mbar_init(&sm.p_full[u], 4);
       sm.lowest[u] = kNoKey;
       sm.last[u] = 0;
     }
@@ -235,26 +272,32 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     }
     return (int)max(0ll, OWN ? seen : min(seen, (long long)p.shared));
   };
-  for (int i = threadIdx.x; i < tokens; i += kThreadsTC) {
-    const int limit = limit_of(token0 + i), u = i >= tile_tokens;
-    atomicMin(&sm.lowest[u], limit);
-    atomicMax(&sm.last[u], limit);
-  }
-  __syncthreads();
-  // key tiles: of the prefix a run of them per CTA
-  const int last = max(sm.last[0], sm.last[1]);
-  int kt_begin = OWN ? p.first_key / kKeysTC : 0, kt_end = (last + kKeysTC - 1) / kKeysTC;
-  if (!OWN) {
-    const int all = (p.shared + kKeysTC - 1) / kKeysTC;
+  // Key tiles.  Of the prefix a run of them per CTA, whichever rows see them: nothing has to wait for the rows' positions then.  Of an entry's own keys those that some row sees.
+  int kt_begin, n0, n1, last;
+  if (OWN) {
+    for (int i = threadIdx.x; i < tokens; i += kThreadsTC) {
+      const int limit = limit_of(token0 + i), u = i >= tile_tokens;
+      atomicMin(&sm.lowest[u], limit);
+      atomicMax(&sm.last[u], limit);
+    }
+    __syncthreads();
+    last = max(sm.last[0], sm.last[1]);
+    kt_begin = p.first_key / kKeys;
+    n0 = max(0, (sm.last[0] + kKeys - 1) / kKeys - kt_begin);
+    n1 = max(0, (sm.last[1] + kKeys - 1) / kKeys - kt_begin);
+  } else {
+    const int all = (p.shared + kKeys - 1) / kKeys;
+    last = p.shared;
     kt_begin = (int)((long long)all * blockIdx.x / gridDim.x);
-    kt_end = min(kt_end, (int)((long long)all * (blockIdx.x + 1) / gridDim.x));
+    const int mine = (int)((long long)all * (blockIdx.x + 1) / gridDim.x) - kt_begin;
+    n0 = tokens > 0 ? mine : 0;
+    n1 = tokens > tile_tokens ? mine : 0;
   }
-  auto tiles_of = [&](int u) { return max(0, min(kt_end, (sm.last[u] + kKeysTC - 1) / kKeysTC) - kt_begin); };
-  const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+  const int n = max(n0, n1);
 
   if (warp < kFirstSoftmaxWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kControlRegs));
-  if (warp == 0) {
-    if (n > 0 && lane == 0) {   // Q: per row tile and 64 dims one box of the group's heads of tile_tokens rows
+  if (warp < 2) {
+    if (warp == 0 && n > 0 && lane == 0) {   // Q: per row tile and 64 dims one box of the group's heads of tile_tokens rows
       const uint32_t bytes = (uint32_t)tile_tokens * group * kBoxDims * 2 * kHalves;
       const int row_tiles = tokens > tile_tokens ? 2 : 1;
       mbar_expect_tx(smem_u32(&sm.q_full), bytes * row_tiles);
@@ -263,193 +306,235 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
         for (int c = 0; c < kHalves; ++c)
           tma_load_3d(smem_u32(sm.q[u]) + c * (kPairsTC * kBoxDims * 2), &map_q, c * kBoxDims, kvh * group, token0 + u * tile_tokens, smem_u32(&sm.q_full));
     }
-    // A key tile is `boxes` boxes of box_keys keys in each half of the dims; lane i copies box i % boxes of half i / boxes.
-    const int boxes = kKeysTC / p.box_keys, box = lane % boxes, half = lane / boxes;
-    const bool copies = half < kHalves;
+    // A warp for keys and one for values: a copy costs the warp that issues it some 85 cycles, and a tile of 80 keys is five boxes in each half of the dims.  Lane i looks up where
+    // box i lies in the pool, a tile ahead; one lane copies them all.
+    constexpr int kMostBoxes = kKeys % 128 == 0 ? 8 : kKeys / 16;
+    const int boxes = kKeys / p.box_keys, box_bytes = p.box_keys * kBoxDims * 2, further = warp * p.kv_heads * p.page_size;   // values lie behind a page's keys
     const int rows_of_pool = p.num_pages * 2 * p.kv_heads * p.page_size;   // (the host has seen that this fits)
+    const uint32_t tiles = smem_u32(warp == 0 ? sm.k[0] : sm.v[0]);
+    uint64_t* const full = warp == 0 ? sm.k_full : sm.v_full;
+    uint64_t* const empty = warp == 0 ? sm.k_empty : sm.v_empty;
+    const bool leader = elect_one();
+    auto look_up = [&](int j) {
+      const int key = (kt_begin + j) * kKeys + lane * p.box_keys;
+      if (lane >= boxes || key >= last) return rows_of_pool;   // past the last key nothing is read: zeros arrive
+      const int index = key / p.page_size;
+      int page = table[index];
+      if ((unsigned)page >= (unsigned)p.num_pages) {   // reported, and page 0 read in its place
+        atomicOr(p.error_flag, kBadPage);
+        page = 0;
+      }
+      return (page * 2 * p.kv_heads + kvh) * p.page_size + (key - index * p.page_size) + further;
+    };
+    RingPosition<kStages> ring;
+    bool ok = true;
+    int rows = n > 0 ? look_up(0) : 0;
+    for (int j = 0; j < n && ok; ++j, ring.advance()) {
+      ok = warp_wait(&empty[ring.stage], ring.phase ^ 1, abort_flag);
+      if (!ok) break;
+      const uint32_t to = tiles + ring.stage * (kKeys * D * 2), bar = smem_u32(&full[ring.stage]);
+      if (leader) mbar_expect_tx(bar, kKeys * D * 2);
+#pragma unroll
+      for (int b = 0; b < kMostBoxes; ++b) {
+        const int row = __shfl_sync(0xffffffffu, rows, b);
+        if (leader && b < boxes) {
+#pragma unroll
+          for (int c = 0; c < kHalves; ++c) tma_load_2d(to + b * box_bytes + c * (kKeys * kBoxDims * 2), &map_kv, c * kBoxDims, row, bar);
+        }
+      }
+      rows = j + 1 < n ? look_up(j + 1) : 0;
+    }
+  } else if (warp < 4) {
+    // S(u, j) = Q(u) . K(j)^T, as soon as the threads of row tile u have the scores before in registers; a warp per row tile.  The whole warp goes through the
+    // loop and one lane issues, so that what the instructions take stays in uniform registers.
+    constexpr uint32_t idesc = umma_instr_desc(kPairsTC, kKeys);
+    constexpr uint32_t kQSub = (kPairsTC * kBoxDims * 2) >> 4, kKSub = (kKeys * kBoxDims * 2) >> 4;   // one sub-tile of 64 dims further, in descriptor units
+    const int u = warp - 2, mine = u == 0 ? n0 : n1;
+    const uint32_t q_low = umma_desc_low(smem_u32(sm.q[u])), k_low = umma_desc_low(smem_u32(sm.k)), to = tmem + kScoreCol0 + u * kKeys;
+    const bool leader = elect_one();
+    RingPosition<kStages> ring;
+    bool ok = mine == 0 || warp_wait(&sm.q_full, 0, abort_flag);
+    for (int j = 0; j < mine && ok; ++j, ring.advance()) {
+      ok = warp_wait(&sm.k_full[ring.stage], ring.phase, abort_flag);
+      if (ok && j > 0) ok = warp_wait(&sm.s_read[u], (j - 1) & 1, abort_flag);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      const uint32_t k_tile = k_low + ring.stage * ((kKeys * D * 2) >> 4);
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)   // 16 dims further: 32 bytes inside a sub-tile's rows, then the next sub-tile
+          umma_bf16(to, q_low + (kk >> 2) * kQSub + (kk & 3) * 2, k_tile + (kk >> 2) * kKSub + (kk & 3) * 2, idesc, kk > 0 ? 1u : 0u);
+        umma_commit(&sm.s_full[u]);
+        umma_commit(&sm.k_empty[ring.stage]);
+      }
+    }
+    for (int j = mine; j < n && ok; ++j, ring.advance()) {   // none of this tile's rows sees these keys
+      ok = warp_wait(&sm.k_full[ring.stage], ring.phase, abort_flag);
+      if (ok && leader) mbar_arrive(&sm.k_empty[ring.stage]);
+    }
+  } else if (warp == 4) {
+    // O(u) += P(u, j) . V(j) as soon as the weights are there
+    constexpr uint32_t idesc = instr_desc_b_mn(kPairsTC, D);
+    // V is the MN-major operand: beyond 64 dims the next sub-tile lies this far on, which the leading-dimension offset says; one sub-tile needs none
+    constexpr uint32_t kVLeading = kHalves > 1 ? (kKeys * kBoxDims * 2) >> 4 : 1u;
+    const uint32_t v_low = ((smem_u32(sm.v) >> 4) & 0x3FFF) | (kVLeading << 16);
+    const bool leader = elect_one();
     RingPosition<kStages> ring;
     bool ok = true;
     for (int j = 0; j < n && ok; ++j, ring.advance()) {
-      const int key = (kt_begin + j) * kKeysTC + box * p.box_keys;
-      int row = rows_of_pool, value_row = rows_of_pool;   // past the last key nothing is read: zeros arrive
-      if (copies && key < last) {
-        int page = table[key / p.page_size];
-        if ((unsigned)page >= (unsigned)p.num_pages) {   // reported, and page 0 read in its place
-          atomicOr(p.error_flag, kBadPage);
-          page = 0;
-        }
-        row = (page * 2 * p.kv_heads + kvh) * p.page_size + key % p.page_size;
-        value_row = row + p.kv_heads * p.page_size;
-      }
-      const uint32_t offset = ring.stage * (kKeysTC * D * 2) + half * (kKeysTC * kBoxDims * 2) + box * p.box_keys * (kBoxDims * 2);
-      ok = warp_wait(&sm.k_empty[ring.stage], ring.phase ^ 1, abort_flag);
-      if (lane == 0 && ok) mbar_expect_tx(&sm.k_full[ring.stage], kKeysTC * D * 2);
-      __syncwarp();
-      if (ok && copies) tma_load_2d(smem_u32(sm.k) + offset, &map_kv, half * kBoxDims, row, smem_u32(&sm.k_full[ring.stage]));
-      if (ok) ok = warp_wait(&sm.v_empty[ring.stage], ring.phase ^ 1, abort_flag);
-      if (lane == 0 && ok) mbar_expect_tx(&sm.v_full[ring.stage], kKeysTC * D * 2);
-      __syncwarp();
-      if (ok && copies) tma_load_2d(smem_u32(sm.v) + offset, &map_kv, half * kBoxDims, value_row, smem_u32(&sm.v_full[ring.stage]));
-    }
-  } else if (warp < 3) {
-    if (lane == 0) {   // the products of row tile u
-      const int u = warp - 1, mine = u == 0 ? n0 : n1;
-      constexpr uint32_t idesc_s = umma_instr_desc(kPairsTC, kKeysTC), idesc_pv = instr_desc_b_mn(kPairsTC, D);
-      constexpr uint32_t kSub = (kKeysTC * kBoxDims * 2) >> 4;   // one sub-tile of 64 dims further, in descriptor units (Q's and K's alike)
-      // V is the MN-major operand: beyond 64 dims the next sub-tile lies kSub on, which the leading-dimension offset says; one sub-tile needs none
-      constexpr uint32_t kVLeading = kHalves > 1 ? kSub : 1u;
-      const uint32_t q_low = umma_desc_low(smem_u32(sm.q[u])), k_low = umma_desc_low(smem_u32(sm.k));
-      const uint32_t v_low = ((smem_u32(sm.v) >> 4) & 0x3FFF) | (kVLeading << 16);
-      const uint32_t tmem_s = tmem + u * kKeysTC, tmem_o = tmem + kOutCol0 + u * 128;
-      RingPosition<kStages> ring;
-      bool ok = mine == 0 || mbar_wait(&sm.q_full, 0, abort_flag);
-      for (int j = 0; j < n && ok; ++j, ring.advance()) {
-        ok = mbar_wait(&sm.k_full[ring.stage], ring.phase, abort_flag);
-        if (ok && j >= mine) {   // none of this tile's rows sees these keys
-          mbar_arrive(&sm.k_empty[ring.stage]);
-          ok = mbar_wait(&sm.v_full[ring.stage], ring.phase, abort_flag);
-          if (ok) mbar_arrive(&sm.v_empty[ring.stage]);
-          continue;
-        }
-        if (ok && j > 0) ok = mbar_wait(&sm.pv_done[u], (j - 1) & 1, abort_flag);   // the weights that lie over the scores have been read
-        if (!ok) break;
+      ok = warp_wait(&sm.v_full[ring.stage], ring.phase, abort_flag);
+      const uint32_t v_tile = v_low + ring.stage * ((kKeys * D * 2) >> 4);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (!ok || j >= (u == 0 ? n0 : n1)) continue;
+        ok = warp_wait(&sm.p_full[u], j & 1, abort_flag);
+        if (!ok) continue;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const uint32_t k_tile = k_low + ring.stage * ((kKeysTC * D * 2) >> 4), v_tile = v_low + ring.stage * ((kKeysTC * D * 2) >> 4);
+        if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)   // 16 dims further: 32 bytes inside a sub-tile's rows, then the next sub-tile
-          umma_bf16(tmem_s, q_low + (kk >> 2) * kSub + (kk & 3) * 2, k_tile + (kk >> 2) * kSub + (kk & 3) * 2, idesc_s, kk > 0 ? 1u : 0u);
-        umma_commit(&sm.s_full[u]);
-        umma_commit(&sm.k_empty[ring.stage]);
-        ok = mbar_wait(&sm.v_full[ring.stage], ring.phase, abort_flag);
-#pragma unroll
-        for (int h = 0; h < 2 && ok; ++h) {
-          ok = mbar_wait(&sm.p_full[u][h], j & 1, abort_flag);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-#pragma unroll
-          for (int kk = 4 * h; kk < 4 * h + 4; ++kk)   // 16 keys further: 8 columns of P, 16 rows (2048 bytes) down in a V sub-tile
-            umma_bf16_a_tmem(tmem_o, tmem_s + kk * 8, v_tile + kk * ((16 * kBoxDims * 2) >> 4), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < kKeys / 16; ++kk)   // 16 keys further: 8 columns of P, 16 rows (2048 bytes) down in a V sub-tile
+            umma_bf16_a_tmem(tmem + u * D, tmem + kWeightCol0 + u * kWeightCols + kk * 8, v_tile + kk * ((16 * kBoxDims * 2) >> 4), idesc, (j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&sm.pv_done[u]);
         }
-        if (!ok) break;
-        umma_commit(&sm.v_empty[ring.stage]);
-        umma_commit(&sm.pv_done[u]);
       }
+      if (ok && leader) umma_commit(&sm.v_empty[ring.stage]);
     }
   } else if (warp >= kFirstSoftmaxWarp) {
+    // (Two threads per pair, half of a tile's keys each and the maximum agreed on at a barrier, took 5 to 10 % longer.)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
-    const int u = (warp - kFirstSoftmaxWarp) >> 2, sub = warp & 3, pair = sub * 32 + lane, mine = u == 0 ? n0 : n1;
+    const int u = (warp - kFirstSoftmaxWarp) / 4, sub = warp & 3, pair = sub * 32 + lane, mine = u == 0 ? n0 : n1;
     const uint32_t lane_base = (uint32_t)(sub * 32) << 16;
-    const uint32_t tmem_s = tmem + lane_base + u * kKeysTC, tmem_o = tmem + lane_base + kOutCol0 + u * 128;
+    const uint32_t tmem_s = tmem + lane_base + kScoreCol0 + u * kKeys, tmem_p = tmem + lane_base + kWeightCol0 + u * kWeightCols, tmem_o = tmem + lane_base + u * D;
     const int tile_rows = max(0, min(tile_tokens, tokens - u * tile_tokens));
     const bool mine_valid = pair < tile_rows * group;
     const int token = token0 + u * tile_tokens + pair / group, head = kvh * group + pair % group;
     const int limit = mine_valid ? limit_of(token) : 0;
+    if (!OWN) {
+      const int fewest = __reduce_min_sync(0xffffffffu, mine_valid ? limit : kNoKey);
+      if (lane == 0) atomicMin(&sm.lowest[u], fewest);
+      tile_barrier(u);
+    }
     const int lowest = sm.lowest[u];
     const float sl2 = p.scale * kToLog2;
     float reference = -INFINITY, row_sum = 0.0f;
     RingPosition<kStages> at;
-    bool ok = true;
-    for (int j = 0; j < mine && ok; ++j, at.advance()) {
-      const int key0 = (kt_begin + j) * kKeysTC;
-      ok = warp_wait(&sm.s_full[u], j & 1, abort_flag);
-      if (!ok) break;
+    bool ok = true;   // (a warp that gives up goes on to the end without waiting: the others of its row tile meet it at their barriers)
+    // Turn -1 works on whatever tensor memory holds and hands nothing on: the loop's instructions are fetched while the first keys are on their way (fetched behind them, the first
+    // tile took 5,000 cycles where the others take 2,000).
+    auto take_tile = [&](int j, auto some_masked) {
+      constexpr bool masked = decltype(some_masked)::value;
+      const int key0 = (kt_begin + max(j, 0)) * kKeys;
+      if (j >= 0 && ok) ok = warp_wait(&sm.s_full[u], j & 1, abort_flag);
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      float sc[kKeysTC];
-      tmem_ld64(tmem_s, sc);
-      tmem_ld64(tmem_s + 64, sc + 64);
-      const bool masked = key0 + kKeysTC > lowest || (OWN && key0 < p.first_key);
+      float sc[kKeys];
+      {
+        uint32_t raw[kKeys];
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 8) tmem_load_8(tmem_s + c, raw + c);
+        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) sc[i] = __uint_as_float(raw[i]);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      if (lane == 0 && j >= 0) mbar_arrive(&sm.s_read[u]);   // (the load was warp-wide: every lane has its scores)
       if (masked) {
 #pragma unroll
-        for (int i = 0; i < kKeysTC; ++i) sc[i] = key0 + i < limit && (!OWN || key0 + i >= p.first_key) ? sc[i] : -INFINITY;
+        for (int i = 0; i < kKeys; ++i) sc[i] = key0 + i < limit && (!OWN || key0 + i >= p.first_key) ? sc[i] : -INFINITY;
       }
       float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kKeysTC; i += 8) {
+      for (int i = 0; i < kKeys; i += 8) {
         m0 = max3(m0, sc[i], sc[i + 1]);
         m1 = max3(m1, sc[i + 2], sc[i + 3]);
         m2 = max3(m2, sc[i + 4], sc[i + 5]);
         m3 = max3(m3, sc[i + 6], sc[i + 7]);
       }
       const float scaled_max = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * sl2;
-      if (j == 0) {
-        reference = scaled_max;
-      } else {
-        // The output and the sum are taken against `reference`.  (The product that last added to the output is done: the scores waited for were issued behind it.)
-        const bool grown = scaled_max > reference + kLazyRescale;
-        if (__any_sync(0xffffffffu, grown)) {
+      // The output and the sum are taken against a reference, which moves only where a tile's maximum is far above it (the first tile's always is).
+      const bool grown = scaled_max > reference + kLazyRescale;
+      if (__builtin_expect(__any_sync(0xffffffffu, grown), 0)) {
+        if (j > 0) {
+          if (ok) ok = warp_wait(&sm.pv_done[u], (j - 1) & 1, abort_flag);   // the product that last added to the output
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           const float alpha = grown ? exp2f(reference - scaled_max) : 1.0f;
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_load_32(tmem_o + c * 32, o);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {   // (loads and stores are warp-wide: rows that need nothing multiply by one)
+            uint32_t o[16];
+            tmem_load_16(tmem_o + c, o);
             asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_store_32(tmem_o + c * 32, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_store_8(tmem_o + c, o);
+            tmem_store_8(tmem_o + c + 8, o + 8);
           }
+          asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
           row_sum *= alpha;
-          if (grown) reference = scaled_max;
         }
+        if (grown) reference = scaled_max;
       }
       const float base = reference == -INFINITY ? 0.0f : reference;   // a row that has seen no key yet: every weight is 0
       if (masked) {
         // Values of keys that none of the CTA's rows sees (never written, perhaps) become zeros: 0 * (whatever is there) must stay 0.  Of keys that some rows see, what is
         // not finite is taken out and noted.
-        const bool some_see = lowest < min(key0 + kKeysTC, last);
-        const int none_from = max(0, min(kKeysTC, last - key0)), none_to = OWN ? max(0, min(kKeysTC, p.first_key - key0)) : 0;
-        if (none_from < kKeysTC || none_to > 0 || some_see) {
-          ok = warp_wait(&sm.v_full[at.stage], at.phase, abort_flag);
-          if (!ok) break;
+        const bool some_see = lowest < min(key0 + kKeys, last);
+        const int none_from = max(0, min(kKeys, last - key0)), none_to = OWN ? max(0, min(kKeys, p.first_key - key0)) : 0;
+        if (none_from < kKeys || none_to > 0 || some_see) {
+          if (ok) ok = warp_wait(&sm.v_full[at.stage], at.phase, abort_flag);
           uint8_t* v_tile = reinterpret_cast<uint8_t*>(sm.v[at.stage]);
-          for (int r = pair >> 3; r < kKeysTC; r += kPairsTC / 8) {   // 8 threads a row of 128 bytes, whatever the swizzle
+          for (int r = pair >> 3; r < kKeys; r += kPairsTC / 8) {   // 8 threads a row of 128 bytes, whatever the swizzle
             if (r < none_to || r >= none_from) {
 #pragma unroll
-              for (int c = 0; c < kHalves; ++c) *reinterpret_cast<uint4*>(v_tile + c * (kKeysTC * kBoxDims * 2) + r * 128 + (pair & 7) * 16) = make_uint4(0, 0, 0, 0);
+              for (int c = 0; c < kHalves; ++c) *reinterpret_cast<uint4*>(v_tile + c * (kKeys * kBoxDims * 2) + r * 128 + (pair & 7) * 16) = make_uint4(0, 0, 0, 0);
             } else if (some_see) {
 #pragma unroll
               for (int c = 0; c < kHalves; ++c) {
-                uint16_t* chunk = reinterpret_cast<uint16_t*>(v_tile + c * (kKeysTC * kBoxDims * 2) + r * 128 + (pair & 7) * 16);
+                uint8_t* chunk = v_tile + c * (kKeys * kBoxDims * 2) + r * 128 + (pair & 7) * 16;
                 const uint4 eight = *reinterpret_cast<const uint4*>(chunk);
-                const uint32_t words[4] = {eight.x, eight.y, eight.z, eight.w};
-#pragma unroll
-                for (int w = 0; w < 8; ++w) {
-                  const uint32_t bits = (words[w >> 1] >> (16 * (w & 1))) & 0xffffu;
-                  if ((bits & 0x7f80u) == 0x7f80u) {
-                    const int dim = c * kBoxDims + (((pair & 7) ^ (r & 7)) << 3) + w;   // the 128-byte swizzle: chunk i of row r lies at i ^ (r % 8)
-                    atomicMin(&sm.bad[(bits & 0x7fu) != 0u ? 2 : (bits >> 15)][dim], key0 + r);
-                    sm.any_bad = 1;
-                    __threadfence_block();
-                    chunk[w] = 0;
-                  }
-                }
+                if (__builtin_expect(not_finite(eight.x) | not_finite(eight.y) | not_finite(eight.z) | not_finite(eight.w), 0u) != 0u)
+                  take_out(reinterpret_cast<uint16_t*>(chunk), &sm.bad[0][c * kBoxDims + (((pair & 7) ^ (r & 7)) << 3)], D, key0 + r, &sm.any_bad);   // the 128-byte swizzle: chunk i of row r lies at i ^ (r % 8)
               }
             }
           }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");   // generic-proxy writes -> visible to the tensor core
         }
       }
+      // The warps of the two row tiles that share a scheduler take turns: one's exponentials, which the exponential unit sets the pace of, run under the other's loads, maxima and
+      // stores.  Left alone they fall into step and wait for the unit together, then leave it idle together (2,750 cycles a tile).
+      if (ok && (u == 0 ? j > 0 && j <= n1 : j >= 0 && j < n0)) ok = warp_wait(&sm.exps_done[u ^ 1][sub], (u == 0 ? j - 1 : j) & 1, abort_flag);
       const Pair scale2 = pair_of(sl2, sl2), minus_base2 = pair_of(-base, -base);
       Pair sums = pair_of(0.0f, 0.0f);
+      uint32_t packed[kKeys / 2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float x0, x1;
-          unpair(fma2(pair_of(sc[64 * h + 2 * i], sc[64 * h + 2 * i + 1]), scale2, minus_base2), x0, x1);
-          const float p0 = exp2_approx(x0), p1 = exp2_approx(x1);
-          sums = add2(sums, pair_of(p0, p1));
-          packed[i] = pack_bf16(p0, p1);   // a weight keeps 8 bits where it meets its value, as in the other bfloat16 attention kernels; the sum has all of it
-        }
-        tmem_store_32(tmem_s + 32 * h, packed);   // over scores that are in registers by now
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[u][h]);
+      for (int i = 0; i < kKeys / 2; ++i) {
+        float x0, x1;
+        unpair(fma2(pair_of(sc[2 * i], sc[2 * i + 1]), scale2, minus_base2), x0, x1);
+        const float p0 = exp2_approx(x0), p1 = exp2_approx(x1);
+        sums = add2(sums, pair_of(p0, p1));
+        packed[i] = pack_bf16(p0, p1);   // a weight keeps 8 bits where it meets its value, as in the other bfloat16 attention kernels; the sum has all of it
       }
+      if (lane == 0 && j >= 0) mbar_arrive(&sm.exps_done[u][sub]);
+      if (j > 0 && ok) ok = warp_wait(&sm.pv_done[u], (j - 1) & 1, abort_flag);   // the weights before have been read
+#pragma unroll
+      for (int c = 0; c < kKeys / 2; c += 4) tmem_store_4(tmem_p + c, packed + c);
+      asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && j >= 0) mbar_arrive(&sm.p_full[u]);
       float sum0, sum1;
       unpair(sums, sum0, sum1);
       row_sum += sum0 + sum1;
-    }
+      if (j >= 0) {
+        at.advance();
+      } else {
+        reference = -INFINITY;
+        row_sum = 0.0f;
+      }
+    };
+    // Tiles that every row sees all of, then the others: what the masks take stays out of the loop that counts (with it inside, every tile took a fifth longer).
+    const int all_seen = OWN && p.first_key % kKeys != 0 ? 0 : max(0, min(mine, lowest / kKeys - kt_begin));
+    int j = -1;
+    for (; mine > 0 && j < all_seen; ++j) take_tile(j, std::false_type{});
+    for (; mine > 0 && j < mine; ++j) take_tile(j, std::true_type{});
     if (ok && mine > 0) ok = warp_wait(&sm.pv_done[u], (mine - 1) & 1, abort_flag);
     if (waits_late) grid_dependency_wait();   // the prefix's parts
     if (ok) {
@@ -470,21 +555,22 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
         p.part_ml[at_pair * p.parts + blockIdx.x] = make_float2(reference, row_sum);
       }
       const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+      // A thread has its row, memory wants lines: 16 columns of the warp's 32 rows go through shared memory (Q's place: its products are done), piece i of row r at i ^ (r / 2 % 4).
+      float4* staged = reinterpret_cast<float4*>(sm.q[u]) + sub * 32 * 4;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {   // 32 columns at a time (the load is warp-wide: every lane takes part)
-        uint32_t raw[32];
+      for (int c = 0; c < D; c += 16) {   // (the load is warp-wide: every lane takes part)
+        uint32_t raw[16];
         if (mine > 0) {
-          tmem_load_32(tmem_o + c * 32, raw);
+          tmem_load_16(tmem_o + c, raw);
           asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
         }
-        if (!mine_valid) continue;
-        float o[32];
+        float o[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = mine > 0 ? __uint_as_float(raw[i]) : 0.0f;
-        if (any_bad) {
+        for (int i = 0; i < 16; ++i) o[i] = mine > 0 ? __uint_as_float(raw[i]) : 0.0f;
+        if (__builtin_expect(any_bad, 0)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const volatile int* first = &sm.bad[0][c * 32 + i];
+          for (int i = 0; i < 16; ++i) {
+            const volatile int* first = &sm.bad[0][c + i];
             const bool plus = first[0] < limit, minus = first[D] < limit, none = first[2 * D] < limit;
             if (none || (plus && minus)) o[i] = __int_as_float(0x7fffffff);
             else if (plus) o[i] += INFINITY;
@@ -492,28 +578,38 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
           }
         }
         if (OWN) {
+          if (!mine_valid) continue;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = factor == 0.0f ? 0.0f : o[i] * factor;
+          for (int i = 0; i < 16; ++i) o[i] = factor == 0.0f ? 0.0f : o[i] * factor;
           for (int s = 0; s < p.parts; ++s) {
             const float2 ml = __ldcg(&p.part_ml[at_pair * p.parts + s]);
             const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : exp2f(ml.x - top);
             if (f == 0.0f) continue;
-            const float4* part = reinterpret_cast<const float4*>(p.part_o + (at_pair * p.parts + s) * D + c * 32);
+            const float4* part = reinterpret_cast<const float4*>(p.part_o + (at_pair * p.parts + s) * D + c);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4; ++i) {
               const float4 v = __ldcg(part + i);
               o[4 * i] = fmaf(f, v.x, o[4 * i]), o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]), o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]), o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
             }
           }
-          uint4* to = reinterpret_cast<uint4*>(p.out + at_pair * D + c * 32);
+          uint4* to = reinterpret_cast<uint4*>(p.out + at_pair * D + c);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 2; ++i)
             to[i] = make_uint4(pack_bf16(o[8 * i] * inverse, o[8 * i + 1] * inverse), pack_bf16(o[8 * i + 2] * inverse, o[8 * i + 3] * inverse),
                                pack_bf16(o[8 * i + 4] * inverse, o[8 * i + 5] * inverse), pack_bf16(o[8 * i + 6] * inverse, o[8 * i + 7] * inverse));
         } else if (mine > 0) {
-          float4* to = reinterpret_cast<float4*>(p.part_o + (at_pair * p.parts + blockIdx.x) * D + c * 32);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 4; ++i) staged[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 2), other = sub * 32 + r;
+            if (other < tile_rows * group) {
+              const size_t other_pair = (size_t)(token0 + u * tile_tokens + other / group) * p.q_heads + kvh * group + other % group;
+              reinterpret_cast<float4*>(p.part_o + (other_pair * p.parts + blockIdx.x) * D + c)[lane & 3] = staged[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
+            }
+          }
+          __syncwarp();
         }
       }
     }
@@ -540,6 +636,7 @@ static int launch_tc(const CUtensorMap& map_q, const CUtensorMap& map_kv, const 
   static std::atomic<unsigned long long> devices{0};
   static std::atomic<int> registers{0};
   const int smem = (int)sizeof(SmemPrefix<D>) + 1024;
+  static_assert(sizeof(SmemPrefix<D>) + 1024 <= 232448, "shared memory of a CTA");
   cudaError_t e = allow_shared_memory(prefix_tc_kernel<D, OWN>, smem, devices);
   if (e != cudaSuccess) return (int)e;
   if (registers.load(std::memory_order_relaxed) == 0) {   // the warps' shares are handed out of what the launch holds: less than that would wait for good
@@ -571,8 +668,9 @@ TLIE_EXPORT int tlie_prefix_tc(int own, const void* q, long long q_row_stride, c
   const int group = q_heads / kv_heads, tile_tokens = kPairsTC / group;
   const long long pool_rows = (long long)num_pages * 2 * kv_heads * page_size;
   if (pool_rows >= 0x7fffffffLL - 256) return (int)cudaErrorInvalidValue;   // a copy's row is a 32-bit coordinate
-  int box_keys = 16;
-  while (box_keys < kKeysTC && page_size % (2 * box_keys) == 0) box_keys *= 2;
+  const int keys = head_dim == 64 ? kKeysOf<64> : kKeysOf<128>;
+  int box_keys = 16;   // keys of a box: what divides a page and a key tile
+  while (page_size % (2 * box_keys) == 0 && keys % (2 * box_keys) == 0) box_keys *= 2;
   CUtensorMap map_q, map_kv;
   if (!make_q_map(&map_q, q, rows, q_heads, head_dim, q_row_stride, group, tile_tokens) || !make_map(&map_kv, pages, (int)pool_rows, head_dim, box_keys))
     return (int)cudaErrorInvalidValue;
