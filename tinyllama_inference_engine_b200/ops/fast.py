@@ -1218,7 +1218,7 @@ def shared_prefix_takes(qkv, pages, out, page_size: int, head_dim: int) -> bool:
 
 def prefix_rows_ctas(rows: int, kv_heads: int, group: int, keys: int) -> int:
     """CTAs per (row, key/value head): as many as keep two on every SM, each with at least 128 keys to read."""
-    pairs = rows * kv_heads * -(-group // 16)
+    pairs = rows * kv_heads * -(-group // 8)
     ctas = 1
     while ctas < PREFIX_ROWS_MAX_CTAS and pairs * ctas * 2 <= 2 * sm_count() and keys > 128 * ctas:
         ctas *= 2
@@ -1226,16 +1226,20 @@ def prefix_rows_ctas(rows: int, kv_heads: int, group: int, keys: int) -> int:
 
 
 PREFIX_TC_PAIRS = 128         # (row, head) pairs of a row tile of the tensor-core kernel, of which a CTA has two (csrc/attention_prefix_tc.cu)
-PREFIX_TC_KEYS = 128          # keys of one of its key tiles
+PREFIX_TC_KEYS = {64: 128, 128: 80}   # keys of one of its key tiles, by head size
+PREFIX_MOST_PARTS = 32        # runs of the prefix whose parts are brought together
 
 
-def prefix_tc_parts(rows: int, kv_heads: int, group: int, shared: int) -> int:
-    """Runs that the prefix's key tiles are cut into: what makes the longest SM's share of them least, an item's own start and end counted as two key tiles."""
-    tiles = -(-shared // PREFIX_TC_KEYS)
+def prefix_tc_parts(rows: int, kv_heads: int, group: int, head_dim: int, shared: int) -> int:
+    """Runs that the prefix's key tiles are cut into: what takes the longest SM's share of them and the parts' way through memory the least time.
+
+    In units of a key tile (1.1 us): an item's own start and end cost three, the parts are written and read again at some 4 TB/s."""
+    tiles = -(-shared // PREFIX_TC_KEYS[head_dim])
     items = -(-rows // (2 * (PREFIX_TC_PAIRS // group))) * kv_heads
+    part = rows * kv_heads * group * head_dim * 8 / 4e6 / 1.1
     best, cost = 1, None
-    for parts in range(1, min(tiles, 32) + 1):
-        here = -(-items * parts // sm_count()) * (-(-tiles // parts) + 2)
+    for parts in range(1, min(tiles, PREFIX_MOST_PARTS) + 1):
+        here = -(-items * parts // sm_count()) * (-(-tiles // parts) + 3) + parts * part
         if cost is None or here < cost:
             best, cost = parts, here
     return best
@@ -1253,7 +1257,7 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     flag, stream = ops.error_flag(qkv.device).data_ptr(), ops._stream()
     parts, part_ml, part_o, first_key = 0, 0, 0, 0
     if PREFIX_MODE and shared > 0:
-        parts = prefix_tc_parts(rows, kv_heads, group, shared)
+        parts = prefix_tc_parts(rows, kv_heads, group, head_dim, shared)
         buffer = torch.empty(rows * q_heads * parts * (head_dim + 2), dtype=torch.float32, device=qkv.device)
         part_o = buffer.data_ptr()
         part_ml = part_o + 4 * rows * q_heads * parts * head_dim
