@@ -21,7 +21,7 @@ constexpr int kRowWarps = 8;
 constexpr int kRowHeads = 8;       // query heads of a CTA: the columns of a product
 constexpr int kRowKeys = 16;       // keys of a tile: the rows of a product
 constexpr int kMostParts = 64;     // of the keys below first_key
-constexpr int kMostSources = 8 * kRowWarps + kMostParts;
+constexpr int kMostSources = 8 + kMostParts;   // (a CTA's warps, or a cluster's CTAs, and the parts)
 constexpr float kToLog2 = 1.4426950408889634f;
 constexpr int kBadPage = 8;        // the bit of the device's error word
 
@@ -205,33 +205,61 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) prefix_rows_kernel(PrefixRo
       *reinterpret_cast<float4*>(to + 4) = make_float4(o[b * 4 + 2][h], o[b * 4 + 2][h + 2], o[b * 4 + 3][h], o[b * 4 + 3][h + 2]);
     }
   }
-  if (ctas > 1) cluster.sync();
-  else __syncthreads();
-  if (waits_late) grid_dependency_wait();
-
-  // What every part counts for, head by head: a warp each, the parts over its lanes (those of the cluster's warps, then those of the keys below first_key).
-  const int own_sources = ctas * kRowWarps, sources = own_sources + p.parts;
-  if (warp < heads && entry >= 0) {
-    const size_t pair = (size_t)row * p.q_heads + head0 + warp;
-    constexpr int kPerLane = (kMostSources + 31) / 32;
-    float2 ml[kPerLane];
-    float m = -INFINITY;
+  __syncthreads();
+  // Parts are weighed head by head: a warp each, the parts over its lanes; (m, l) of them all, and what each counts for in units of the largest.
+  constexpr int kPerLane = (kMostSources + 31) / 32;
+  auto weigh = [&](float2 (&ml)[kPerLane]) {
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int source = lane + 32 * i;
-      ml[i] = make_float2(-INFINITY, 0.0f);
-      if (source < own_sources) ml[i] = *cluster.map_shared_rank(&merge_ml[source % kRowWarps][warp], source / kRowWarps);
-      else if (source < sources) ml[i] = __ldcg(&p.part_ml[pair * p.parts + source - own_sources]);
-      m = fmaxf(m, ml[i].x);
-    }
+    for (int i = 0; i < kPerLane; ++i) m = fmaxf(m, ml[i].x);
     m = warp_max(m);
-    float l = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       ml[i].x = ml[i].x == -INFINITY ? (ml[i].y == 0.0f ? 0.0f : 1.0f) : exp2f(ml[i].x - m);   // (a part of nothing but NaN keeps its NaN)
       if (ml[i].x != 0.0f) l = fmaf(ml[i].x, ml[i].y, l);
     }
-    l = warp_sum(l);
+    return make_float2(m, warp_sum(l));
+  };
+  if (ctas > 1) {   // this CTA's part into the place of its first warp's, for the cluster
+    if (warp < heads) {
+      float2 ml[kPerLane];
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) ml[i] = lane + 32 * i < kRowWarps ? merge_ml[lane + 32 * i][warp] : make_float2(-INFINITY, 0.0f);
+      const float2 together = weigh(ml);
+      if (lane < kRowWarps) factor_of[warp][lane] = ml[0].x;
+      __syncwarp();
+      if (lane == 0) merge_ml[0][warp] = together;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * (D / 4); i += kRowWarps * 32) {
+      const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kRowWarps; ++w) {
+        const float f = factor_of[h][w];
+        if (f == 0.0f) continue;
+        const float4 part = *reinterpret_cast<const float4*>(&merge_o[w][h][d]);
+        acc.x = fmaf(f, part.x, acc.x), acc.y = fmaf(f, part.y, acc.y), acc.z = fmaf(f, part.z, acc.z), acc.w = fmaf(f, part.w, acc.w);
+      }
+      *reinterpret_cast<float4*>(&merge_o[0][h][d]) = acc;
+    }
+    cluster.sync();
+  }
+  if (waits_late) grid_dependency_wait();
+
+  // the cluster's CTAs' parts (or this CTA's warps') and those of the keys below first_key
+  const int own_sources = ctas > 1 ? ctas : kRowWarps, sources = own_sources + p.parts;
+  if (warp < heads && entry >= 0) {
+    const size_t pair = (size_t)row * p.q_heads + head0 + warp;
+    float2 ml[kPerLane];
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int source = lane + 32 * i;
+      ml[i] = make_float2(-INFINITY, 0.0f);
+      if (source < own_sources) ml[i] = ctas > 1 ? *cluster.map_shared_rank(&merge_ml[0][warp], source) : merge_ml[source][warp];
+      else if (source < sources) ml[i] = __ldcg(&p.part_ml[pair * p.parts + source - own_sources]);
+    }
+    const float l = weigh(ml).y;
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i)
@@ -246,18 +274,17 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) prefix_rows_kernel(PrefixRo
       const float* factor = factor_of[h];
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       auto add = [&](float f, float4 part) { acc.x = fmaf(f, part.x, acc.x), acc.y = fmaf(f, part.y, acc.y), acc.z = fmaf(f, part.z, acc.z), acc.w = fmaf(f, part.w, acc.w); };
+      const float4 nothing = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
       for (int c = 0; c < p.parts; ++c) {
         const float f = factor[own_sources + c];
-        add(f, f != 0.0f ? __ldcg(reinterpret_cast<const float4*>(p.part_o + (pair * p.parts + c) * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        add(f, f != 0.0f ? __ldcg(reinterpret_cast<const float4*>(p.part_o + (pair * p.parts + c) * D + d)) : nothing);
       }
-      for (int c = 0; c < ctas; ++c) {
-        const float* from = cluster.map_shared_rank(&merge_o[0][h][d], c);
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) {
-          const float f = factor[c * kRowWarps + w];
-          if (f != 0.0f) add(f, *reinterpret_cast<const float4*>(from + w * kRowHeads * kOutRow));
-        }
+#pragma unroll 4
+      for (int c = 0; c < own_sources; ++c) {
+        const float f = factor[c];
+        const float* from = ctas > 1 ? cluster.map_shared_rank(&merge_o[0][h][d], c) : &merge_o[c][h][d];
+        add(f, f != 0.0f ? *reinterpret_cast<const float4*>(from) : nothing);
       }
       *reinterpret_cast<uint2*>(p.out + pair * D + d) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
     }

@@ -273,3 +273,33 @@ TLIE_EXPORT int tlie_shared_prefix_generic(int dtype, const void* q, long long q
                        rows, entries, q_heads, kv_heads, head_dim, page_size, shared, scale, prefix_parts, own_parts, error_flag};
   return dtype == TLIE_F32 ? launch_generic<float>(p, stream) : launch_generic<__nv_bfloat16>(p, stream);
 }
+
+extern "C" int tlie_prefix_tc(int, const void*, long long, const void*, int, const int*, const int*, const int*, int, void*, float*, float*, int, int, int, int, int, int, int, int, int, float,
+                              int*, cudaStream_t);
+extern "C" int tlie_prefix_rows(const void*, long long, const void*, int, const int*, const int*, const int*, int, void*, const float*, const float*, int, int, int, int, int, int, int, int,
+                                float, int, int*, cudaStream_t);
+
+// The bfloat16 kernels for head sizes 64 and 128 (each checks what it takes).  prefix: 0, every row reads the shared keys for itself; 1, the prefix's parts come
+// from the tensor cores, `parts` runs of them.  own: 0, a row at a time (`ctas` per row and head), 1, an entry's rows on the tensor cores.
+// scratch: rows * q_heads * parts * (head_dim + 2) floats, 16-byte aligned.
+TLIE_EXPORT int tlie_shared_prefix_bf16(int prefix, int own, int parts, int ctas, const void* q, long long q_row_stride, const void* pages, int num_pages, const int* positions,
+                                        const int* seq_starts, const int* block_table, int table_stride, void* out, float* scratch, int rows, int entries, int q_heads, int kv_heads,
+                                        int head_dim, int page_size, int shared, float scale, int* error_flag, cudaStream_t stream) {
+  float *part_o = nullptr, *part_ml = nullptr;
+  int first_key = 0, status = 0;
+  if (prefix != 0) {
+    if (scratch == nullptr) return (int)cudaErrorInvalidValue;
+    part_o = scratch;
+    part_ml = scratch + (size_t)rows * q_heads * parts * head_dim;
+    first_key = shared;
+    status = tlie_prefix_tc(0, q, q_row_stride, pages, num_pages, positions, seq_starts, block_table, table_stride, out, part_ml, part_o, parts, rows, entries, q_heads, kv_heads,
+                            head_dim, page_size, shared, 0, scale, error_flag, stream);
+    if (status != 0) return status;
+  } else {
+    parts = 0;
+  }
+  return own == 0 ? tlie_prefix_rows(q, q_row_stride, pages, num_pages, positions, seq_starts, block_table, table_stride, out, part_ml, part_o, parts, rows, entries, q_heads, kv_heads,
+                                     head_dim, page_size, first_key, scale, ctas, error_flag, stream)
+                  : tlie_prefix_tc(1, q, q_row_stride, pages, num_pages, positions, seq_starts, block_table, table_stride, out, part_ml, part_o, parts, rows, entries, q_heads, kv_heads,
+                                   head_dim, page_size, shared, first_key, scale, error_flag, stream);
+}

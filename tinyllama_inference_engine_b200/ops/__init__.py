@@ -685,18 +685,8 @@ def _on(device: torch.device):
     return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared: int, out, q_heads: int, kv_heads: int, head_dim: int, page_size: int,
-                            scale: float | None = None) -> None:
-    """``paged_attention`` for a batch whose requests share their first ``shared`` cached keys: answers to one prompt, questions behind one system prompt.
-
-    Row t of ``qkv`` (its first ``q_heads * head_dim`` columns: the rotated query heads; rows may be a run of columns of wider ones) belongs to the entry b
-    with ``seq_starts[b] <= t < seq_starts[b + 1]`` and attends to that request's cached keys up to ``positions[t]``.  Keys below ``shared`` are read through row 0 of
-    ``block_table`` once for the whole batch, whose rows must name the same pages (or copies of them) there; ``shared`` need not end a page, and a request's own
-    keys may lie in the rest of that page or of its copy.  An entry brings any number of rows, none included.  Rows in front of ``seq_starts[0]`` and behind ``seq_starts[-1]`` are left as they
-    were; a row that sees no key (a negative position) becomes zero.  Positions that the block table does not reach and pages outside the pool are reported in
-    the device's error word.  ``scale``: positive, ``head_dim ** -0.5`` by default.  32-bit or bfloat16, head sizes that are multiples of 16 up to 256.
-
-    Called inside the capture of a CUDA graph, the graph keeps ``shared`` and the tensors' addresses; what the tensors hold may change from replay to replay."""
+def _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale) -> None:
+    """What of a call of ``shared_prefix_attention`` is wrong."""
     if head_dim % 16 != 0 or not 0 < head_dim <= 256:
         raise KernelError(f"attention kernels take head sizes that are multiples of 16 up to 256, got {head_dim}", code="invalid_shape")
     if kv_heads < 1 or q_heads < 1 or q_heads % kv_heads != 0:
@@ -713,15 +703,44 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     if isinstance(shared, bool) or not isinstance(shared, int) or not 0 <= shared <= block_table.shape[1] * page_size:
         raise KernelError(f"shared_prefix_attention: shared must be a whole number from 0 to the {block_table.shape[1] * page_size} keys that a block-table row reaches, got {shared!r}",
                           code="invalid_argument")
-    scale = head_dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
+    if scale is not None and not 0.0 < scale < float("inf"):
         raise KernelError(f"shared_prefix_attention: scale must be positive and finite, got {scale}", code="invalid_argument")
     _code(qkv)
     if any(t.dtype != torch.int32 for t in (positions, seq_starts, block_table)):
         raise KernelError("shared_prefix_attention: positions, seq_starts and the block table are int32", code="invalid_dtype")
     if not all(t.is_contiguous() for t in (pages, positions, seq_starts, block_table, out)):
         raise KernelError("kernels take contiguous tensors")
-    device = _one_device("shared_prefix_attention", qkv=qkv, pages=pages, positions=positions, seq_starts=seq_starts, block_table=block_table, out=out)
+    _one_device("shared_prefix_attention", qkv=qkv, pages=pages, positions=positions, seq_starts=seq_starts, block_table=block_table, out=out)
+    raise KernelError("shared_prefix_attention: the arguments do not fit each other", code="invalid_argument")
+
+
+def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared: int, out, q_heads: int, kv_heads: int, head_dim: int, page_size: int,
+                            scale: float | None = None) -> None:
+    """``paged_attention`` for a batch whose requests share their first ``shared`` cached keys: answers to one prompt, questions behind one system prompt.
+
+    Row t of ``qkv`` (its first ``q_heads * head_dim`` columns: the rotated query heads; rows may be a run of columns of wider ones) belongs to the entry b
+    with ``seq_starts[b] <= t < seq_starts[b + 1]`` and attends to that request's cached keys up to ``positions[t]``.  Keys below ``shared`` are read through row 0 of
+    ``block_table`` once for the whole batch, whose rows must name the same pages (or copies of them) there; ``shared`` need not end a page, and a request's own
+    keys may lie in the rest of that page or of its copy.  An entry brings any number of rows, none included.  Rows in front of ``seq_starts[0]`` and behind ``seq_starts[-1]`` are left as they
+    were; a row that sees no key (a negative position) becomes zero.  Positions that the block table does not reach and pages outside the pool are reported in
+    the device's error word.  ``scale``: positive, ``head_dim ** -0.5`` by default.  32-bit or bfloat16, head sizes that are multiples of 16 up to 256.
+
+    Called inside the capture of a CUDA graph, the graph keeps ``shared`` and the tensors' addresses; what the tensors hold may change from replay to replay."""
+    if qkv.dim() != 2 or block_table.dim() != 2:
+        _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
+    rows, width = qkv.shape
+    entries, table_width = block_table.shape
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    device, dtype = qkv.device, qkv.dtype
+    if not (device.type == "cuda" and (dtype is torch.bfloat16 or dtype is torch.float32) and pages.dtype is dtype and out.dtype is dtype
+            and positions.dtype is torch.int32 and seq_starts.dtype is torch.int32 and block_table.dtype is torch.int32
+            and pages.device == device and out.device == device and positions.device == device and seq_starts.device == device and block_table.device == device
+            and 0 < head_dim <= 256 and head_dim % 16 == 0 and 0 < kv_heads <= q_heads and q_heads % kv_heads == 0 and width >= q_heads * head_dim
+            and out.shape == (rows, q_heads * head_dim) and pages.shape[1:] == (2, kv_heads, page_size, head_dim) and pages.shape[0] > 0
+            and positions.shape == (rows,) and seq_starts.shape == (entries + 1,) and type(shared) is int and 0 <= shared <= table_width * page_size
+            and 0.0 < scale < float("inf") and (qkv.stride(1) == 1 or rows == 0) and pages.is_contiguous() and out.is_contiguous()
+            and positions.is_contiguous() and seq_starts.is_contiguous() and block_table.is_contiguous()):
+        _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
     if rows == 0 or entries == 0:
         return
     with _on(device):

@@ -1197,23 +1197,27 @@ def moe_grouped(x, gate_up, down, ids, weights, shared, out, kind: int, weight_i
 # --- attention over a prefix that a batch shares ------------------------------------------------
 SHARED_PREFIX_HEAD_DIMS = (64, 128)
 PREFIX_ROWS_MAX_CTAS = 8      # CTAs of a cluster that share a row's keys
+PREFIX_TC_PAIRS = 128         # (row, head) pairs of a row tile of the tensor-core kernel, of which a CTA has two (csrc/attention_prefix_tc.cu)
+PREFIX_TC_KEYS = {64: 128, 128: 80}   # keys of one of its key tiles, by head size
+PREFIX_MOST_PARTS = 32        # runs of the prefix whose parts are brought together
+use_prefix = None             # None: by the rule below; 0, 1: every row reads the shared keys for itself, they are worked out once for all rows (for measurements)
+use_own = None                # likewise 0, 1: a row at a time, the tensor cores
 
 
 def shared_prefix_library():
-    """The kernels of attention over a shared prefix; their launchers take plain Python numbers."""
+    """The kernels of attention over a shared prefix; this launcher takes plain Python numbers."""
     lib = _ops().shared_prefix()
     if not getattr(lib, "_tlie_typed", False):
-        pointer, i32, i64 = c_void_p, c_int, c_longlong
-        lib.tlie_prefix_rows.argtypes = [pointer, i64, pointer, i32, pointer, pointer, pointer, i32, pointer, pointer, pointer, i32, i32, i32, i32, i32, i32, i32, i32, c_float, i32, pointer, pointer]
-        lib.tlie_prefix_tc.argtypes = [i32, pointer, i64, pointer, i32, pointer, pointer, pointer, i32, pointer, pointer, pointer, i32, i32, i32, i32, i32, i32, i32, i32, i32, c_float, pointer, pointer]
+        p, i, n = c_void_p, c_int, c_longlong
+        lib.tlie_shared_prefix_bf16.argtypes = [i, i, i, i, p, n, p, i, p, p, p, i, p, p, i, i, i, i, i, i, i, c_float, p, p]
         lib._tlie_typed = True
     return lib
 
 
-def shared_prefix_takes(qkv, pages, out, page_size: int, head_dim: int) -> bool:
-    """Whether the bfloat16 kernels for head sizes 64 and 128 can read these tensors: 16 bytes at a time, pages of a multiple of 16 keys."""
-    return (qkv.dtype == torch.bfloat16 and head_dim in SHARED_PREFIX_HEAD_DIMS and page_size % 16 == 0 and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0
-            and pages.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
+def shared_prefix_takes(qkv, pages, out, page_size: int, head_dim: int, group: int) -> bool:
+    """Whether the bfloat16 kernels for head sizes 64 and 128 can read these tensors: 16 bytes at a time, pages of a multiple of 16 keys, copies by 32-bit rows of the pool."""
+    return (qkv.dtype == torch.bfloat16 and head_dim in SHARED_PREFIX_HEAD_DIMS and page_size % 16 == 0 and group <= PREFIX_TC_PAIRS and qkv.stride(0) % 8 == 0
+            and (qkv.data_ptr() | pages.data_ptr() | out.data_ptr()) % 16 == 0 and pages.numel() // head_dim < 0x7FFFFF00)
 
 
 def prefix_rows_ctas(rows: int, kv_heads: int, group: int, keys: int) -> int:
@@ -1225,50 +1229,49 @@ def prefix_rows_ctas(rows: int, kv_heads: int, group: int, keys: int) -> int:
     return ctas
 
 
-PREFIX_TC_PAIRS = 128         # (row, head) pairs of a row tile of the tensor-core kernel, of which a CTA has two (csrc/attention_prefix_tc.cu)
-PREFIX_TC_KEYS = {64: 128, 128: 80}   # keys of one of its key tiles, by head size
-PREFIX_MOST_PARTS = 32        # runs of the prefix whose parts are brought together
+def prefix_tc_parts(rows: int, kv_heads: int, group: int, head_dim: int, shared: int) -> tuple[int, float]:
+    """Runs that the prefix's key tiles are cut into, and microseconds: what takes the longest SM's share of them and the parts' way through memory the least time.
 
-
-def prefix_tc_parts(rows: int, kv_heads: int, group: int, head_dim: int, shared: int) -> int:
-    """Runs that the prefix's key tiles are cut into: what takes the longest SM's share of them and the parts' way through memory the least time.
-
-    In units of a key tile (1.1 us): an item's own start and end cost three, the parts are written and read again at some 4 TB/s."""
+    A key tile takes 1.1 us, an item's own start and end some 8, the parts are written and read again at some 4 TB/s."""
     tiles = -(-shared // PREFIX_TC_KEYS[head_dim])
     items = -(-rows // (2 * (PREFIX_TC_PAIRS // group))) * kv_heads
-    part = rows * kv_heads * group * head_dim * 8 / 4e6 / 1.1
-    best, cost = 1, None
-    for parts in range(1, min(tiles, PREFIX_MOST_PARTS) + 1):
-        here = -(-items * parts // sm_count()) * (-(-tiles // parts) + 3) + parts * part
-        if cost is None or here < cost:
-            best, cost = parts, here
-    return best
+    part = rows * kv_heads * group * head_dim * 8 / 4e6
+    return min(((-(-items * parts // sm_count()) * (-(-tiles // parts) * 1.1 + 3) + parts * part + 5, parts) for parts in range(1, min(tiles, PREFIX_MOST_PARTS) + 1)))[::-1]
+
+
+@functools.lru_cache(maxsize=4096)
+def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_heads: int, head_dim: int, page_size: int, shared: int) -> tuple:
+    """Which kernels a call of these sizes runs: (prefix, own, parts, CTAs per row and head, floats of scratch memory)."""
+    group = q_heads // kv_heads
+    prefix, own = use_prefix, use_own
+    own_keys = width * page_size - shared
+    if own is None:
+        own = 1 if rows > 2 * entries else 0
+    parts = 0
+    if shared > 0 and prefix != 0:
+        tc_parts, once = prefix_tc_parts(rows, kv_heads, group, head_dim, shared)
+        if prefix is None:
+            if own:   # an entry's rows fill the row tiles that would share the prefix
+                prefix = 0 if rows * group >= 2 * PREFIX_TC_PAIRS * entries else 1
+            else:     # every row reads the prefix for itself, from L2 at some 7 TB/s
+                prefix = 0 if rows * kv_heads * -(-group // 8) * shared * head_dim * 4 / 7e6 < once else 1
+        parts = tc_parts if prefix else 0
+    else:
+        prefix = 0
+    ctas = prefix_rows_ctas(rows, kv_heads, group, own_keys if prefix else width * page_size)
+    return prefix, own, parts, ctas, rows * q_heads * parts * (head_dim + 2)
 
 
 def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared: int, out, q_heads: int, kv_heads: int, head_dim: int, page_size: int, scale: float) -> bool:
     """bfloat16 attention over a shared prefix on the kernels made for it; False if they do not take the call."""
-    rows, entries, width, group = qkv.shape[0], block_table.shape[0], block_table.shape[1], q_heads // kv_heads
-    if group > PREFIX_TC_PAIRS or not shared_prefix_takes(qkv, pages, out, page_size, head_dim):
+    if not shared_prefix_takes(qkv, pages, out, page_size, head_dim, q_heads // kv_heads):
         return False
     ops = _ops()
-    lib = shared_prefix_library()
-    common = (qkv.data_ptr(), qkv.stride(0), pages.data_ptr(), pages.shape[0], positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), width, out.data_ptr())
-    sizes = (rows, entries, q_heads, kv_heads, head_dim, page_size)
-    flag, stream = ops.error_flag(qkv.device).data_ptr(), ops._stream()
-    parts, part_ml, part_o, first_key = 0, 0, 0, 0
-    if PREFIX_MODE and shared > 0:
-        parts = prefix_tc_parts(rows, kv_heads, group, head_dim, shared)
-        buffer = torch.empty(rows * q_heads * parts * (head_dim + 2), dtype=torch.float32, device=qkv.device)
-        part_o = buffer.data_ptr()
-        part_ml = part_o + 4 * rows * q_heads * parts * head_dim
-        ops._check(lib.tlie_prefix_tc(0, *common, part_ml, part_o, parts, *sizes, shared, 0, scale, flag, stream), "prefix_tc")
-        first_key = shared
-    if rows > entries:
-        ops._check(lib.tlie_prefix_tc(1, *common, part_ml, part_o, parts, *sizes, shared, first_key, scale, flag, stream), "prefix_tc")
-    else:
-        ctas = prefix_rows_ctas(rows, kv_heads, group, width * page_size - first_key)
-        ops._check(lib.tlie_prefix_rows(*common, part_ml, part_o, parts, *sizes, first_key, scale, ctas, flag, stream), "prefix_rows")
+    rows, (entries, width), device = qkv.shape[0], block_table.shape, qkv.device
+    prefix, own, parts, ctas, floats = shared_prefix_plan(rows, entries, width, q_heads, kv_heads, head_dim, page_size, shared)
+    buffer = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+    ops._check(shared_prefix_library().tlie_shared_prefix_bf16(
+        prefix, own, parts, ctas, qkv.data_ptr(), qkv.stride(0), pages.data_ptr(), pages.shape[0], positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), width,
+        out.data_ptr(), buffer.data_ptr() if floats else None, rows, entries, q_heads, kv_heads, head_dim, page_size, shared, scale, ops.error_flag(device).data_ptr(),
+        ops._stream()), "shared_prefix_attention")
     return True
-
-
-PREFIX_MODE = True
