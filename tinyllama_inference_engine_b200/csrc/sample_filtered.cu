@@ -6,15 +6,21 @@
 // token always.  Drawn is the first kept token, in order of ids, at which the running sum of kept weights exceeds u times their sum.
 // Rows with T <= 0, and rows whose largest logit is not above -infinity, give the first token of the order.  A logit of +infinity leaves weight to such logits alone.
 //
-// Weights are whole numbers of 2^-44: their sums are exact in 64 bits (2^19 tokens at most), so that no sum depends on the order it is
+// Weights are whole numbers of 2^-44: their sums are exact in 64 bits, so that no sum depends on the order it is
 // taken in, on how a row is spread over threads and blocks, or on which atomic came first.  What is left of rounding is a weight's own error, a few 2^-25 of
 // it: with sums in 32-bit floats the border of top-p, and the token that a number falls on, would be off by a token in one draw of some hundred over a flat row.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+#include "shared_memory_limit.cuh"
 
 namespace tlie {
 
-constexpr int kFilterThreads = 1024;
-constexpr int kFilterMaxVocab = 1 << 19;
+constexpr int kFilterThreads = 512, kFilterWarps = kFilterThreads / 32;
+constexpr int kBinBits = 10, kBins = 1 << kBinBits;
+constexpr int kListed = 2048;                            // tokens that the first CTA of a cluster can sort
+constexpr int kMostSlice = 49152;                        // tokens of a CTA: 192 KB
+constexpr int kFilterMaxVocab = 8 * kMostSlice;          // (weights of 2^44 and less, fewer than 2^19 of them: sums fit 64 bits, a token's id and weight one number)
 constexpr int kWeightBits = 44;
 
 // Logits as unsigned numbers of the same order: equal floats are equal numbers (-0 counts as 0), NaN is below everything.
@@ -61,124 +67,503 @@ __device__ __forceinline__ unsigned long long token_weight(float l, float m, Sca
   return mantissa >> down;
 }
 
-__device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long* scratch /* >= 32 */) {
-#pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = threadIdx.x % 32 < blockDim.x / 32 ? scratch[threadIdx.x & 31] : 0ull;
-#pragma unroll
-  for (int offset = 16; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
-  return v;
-}
-
 // The last token of a prefix of the order: tokens with a larger key, and those of this key up to this id, belong to it.
 struct Border {
   unsigned key;
   int id;
   __device__ bool holds(unsigned k, int i) const { return k > key || (k == key && i <= id); }
-  __device__ bool before(const Border& o) const { return o.holds(key, id); }   // no longer than o's prefix
 };
 
-// One block per row.  A border is found by bisecting first on the key, then, among tokens of that key, on the id.
+// A row's tokens lie in the shared memory of a cluster of CTAs, consecutive ones in each.
+//
+// Bound by the reading of the logits where there are many rows, else by the chain of steps that each need the cluster's answer before.  So a step asks for much: a
+// border (of top_k by number of tokens, of top_p by weight) is found from a histogram over 1,024 runs of logits, 1/32 wide, below the largest, and the tokens of
+// the run that it falls in, which the first CTA sorts.  Where those are too many (equal logits, or very close ones) the run is cut by the bits of the logits, and equal ones by id.
+// top_k of up to some hundred needs less: as many threads' maxima as top_k asks for bound the last logit that counts from below, what is not
+// below that bound is a short list, and the rest is done on the list by the first CTA.
+struct FilterShared {
+  float* tokens;                  // this CTA's
+  unsigned *low, *high;           // a histogram's numbers, 64 bits in two words: an atomic of 64 bits on shared memory is a loop
+  unsigned long long* list;
+  unsigned long long scan[kFilterWarps];
+  unsigned long long gather[2][8];   // one number per CTA
+  unsigned long long weight_of_warp[kFilterWarps];
+  unsigned long long above;       // the first CTA's are the cluster's, as are:
+  unsigned long long total;
+  int bin, listed, chosen, found_id;
+  unsigned found_key;
+};
+
+__device__ __forceinline__ unsigned long long warp_sum_u64(unsigned long long v) {
+#pragma unroll
+  for (int offset = 16; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
+  return v;
+}
+__device__ __forceinline__ unsigned long long warp_prefix_u64(unsigned long long v, int lane) {   // the sum up to and with this lane
+#pragma unroll
+  for (int offset = 1; offset < 32; offset <<= 1) {
+    const unsigned long long other = __shfl_up_sync(0xffffffffu, v, offset);
+    if (lane >= offset) v += other;
+  }
+  return v;
+}
+
+// One row, by the threads of a cluster.
+class RowFilter {
+ public:
+  __device__ RowFilter(FilterShared& shared, const float* row, int vocab, int slice)
+      : sh(shared), cluster(cooperative_groups::this_cluster()), row(row), vocab(vocab), ctas(cluster.num_blocks()), rank(cluster.block_rank()),
+        lane(threadIdx.x & 31), warp(threadIdx.x >> 5), first_id(min(vocab, rank * slice)), count(min(vocab, (rank + 1) * slice) - first_id) {}
+
+  // Brings the tokens into shared memory; the first one of the order.
+  __device__ void load() {
+    float best = -INFINITY;
+    int id = 0x7fffffff;
+    auto take = [&](float l, int i) {
+      if (l > best || (l == best && i < id)) best = l, id = i;
+    };
+    const float* from = row + first_id;
+    if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+      const int quads = count >> 2;
+      constexpr int kFlight = 8;
+      for (int q0 = threadIdx.x; q0 < quads; q0 += kFlight * kFilterThreads) {
+        float4 v[kFlight];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u)
+          if (q0 + u * kFilterThreads < quads) v[u] = reinterpret_cast<const float4*>(from)[q0 + u * kFilterThreads];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+          const int q = q0 + u * kFilterThreads;
+          if (q >= quads) break;
+          reinterpret_cast<float4*>(sh.tokens)[q] = v[u];
+          take(v[u].x, 4 * q), take(v[u].y, 4 * q + 1), take(v[u].z, 4 * q + 2), take(v[u].w, 4 * q + 3);
+        }
+      }
+      for (int i = 4 * quads + threadIdx.x; i < count; i += kFilterThreads) {
+        sh.tokens[i] = from[i];
+        take(sh.tokens[i], i);
+      }
+    } else {
+      constexpr int kFlight = 8;
+      for (int i0 = threadIdx.x; i0 < count; i0 += kFlight * kFilterThreads) {
+        float v[kFlight];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u)
+          if (i0 + u * kFilterThreads < count) v[u] = from[i0 + u * kFilterThreads];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+          const int i = i0 + u * kFilterThreads;
+          if (i >= count) break;
+          sh.tokens[i] = v[u];
+          take(v[u], i);
+        }
+      }
+    }
+    thread_max = best;
+    unsigned long long mine = id == 0x7fffffff ? 0ull : ((unsigned long long)logit_key(best) << 32) | (unsigned)~(first_id + id);
+    mine = cluster_max(mine);
+    first = mine == 0ull ? 0 : (int)~(unsigned)mine;
+    m = mine == 0ull ? __int_as_float(0x7fffffff) : key_logit((unsigned)(mine >> 32));
+  }
+
+  // The token of the row.
+  __device__ int choose(float temperature, int top_k, float top_p, float min_p, float u) {
+    if (mine_is_nan()) return 0;
+    if (!(temperature > 0.0f) || !(m > -INFINITY) || top_k == 1 || !(min_p <= 1.0f || min_p != min_p) || top_p <= 0.0f) return first;
+    scale = weight_scale(temperature);
+    floor_weight = min_p > 0.0f ? (unsigned long long)ceil((double)min_p * (double)(1ull << kWeightBits)) : 0ull;
+    const bool by_number = top_k > 0 && top_k < vocab, by_weight = top_p < 1.0f;
+    if (by_number && top_k <= kFilterThreads * ctas && list_top(top_k)) return choose_from_list(top_k, top_p, u);
+    Border kept = {0u, vocab};
+    if (by_number) kept = find(kept, (unsigned long long)top_k, false, 0.0f);
+    if (by_weight) kept = find(kept, 0ull, true, top_p);
+    return draw(kept, u);
+  }
+
+ private:
+  FilterShared& sh;
+  cooperative_groups::cluster_group cluster;
+  const float* row;
+  const int vocab, ctas, rank, lane, warp, first_id, count;
+  float m, thread_max;
+  int first;
+  Scale scale;
+  unsigned long long floor_weight;
+  int gathers = 0;
+
+  __device__ bool mine_is_nan() const { return m != m; }
+  static __device__ float key_logit(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+  __device__ unsigned long long weight(float l) const { return token_weight(l, m, scale); }
+  __device__ void sync() {
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+  }
+  template <typename T>
+  __device__ T* at_first(T* mine) {   // the first CTA's
+    return ctas > 1 ? cluster.map_shared_rank(mine, 0) : mine;
+  }
+  // The run that a logit falls in: monotone, and the last one is for all that lies further below.
+  __device__ int bin_of(float l) const { return l == m ? 0 : (int)fminf((m - l) * 32.0f, (float)(kBins - 1)); }
+
+  // Every CTA's number, in every CTA (a CTA's threads bring the same).  Two places in turn: a CTA is past its reading of one when it brings the one after the next.
+  __device__ const unsigned long long* gather(unsigned long long mine) {
+    unsigned long long* place = sh.gather[gathers ^= 1];
+    if (threadIdx.x < ctas) *(ctas > 1 ? cluster.map_shared_rank(&place[rank], threadIdx.x) : &place[0]) = mine;
+    sync();
+    return place;
+  }
+  __device__ unsigned long long cluster_max(unsigned long long v) {
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, offset));
+    __syncthreads();
+    if (lane == 0) sh.scan[warp] = v;
+    __syncthreads();
+    v = sh.scan[lane % kFilterWarps];
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, offset));
+    const unsigned long long* all = gather(v);
+    for (int c = 0; c < ctas; ++c) v = max(v, all[c]);
+    return v;
+  }
+  // Sum over the threads before this one, and of all of this CTA.
+  __device__ unsigned long long block_prefix(unsigned long long v, unsigned long long& all) {
+    const unsigned long long upto = warp_prefix_u64(v, lane);
+    __syncthreads();
+    if (lane == 31) sh.scan[warp] = upto;
+    __syncthreads();
+    unsigned long long before = 0ull;
+    all = 0ull;
+#pragma unroll
+    for (int w = 0; w < kFilterWarps; ++w) {
+      const unsigned long long here = sh.scan[w];
+      if (w < warp) before += here;
+      all += here;
+    }
+    return before + upto - v;
+  }
+  __device__ void clear_bins() {
+    for (int i = threadIdx.x; i < kBins; i += kFilterThreads) sh.low[i] = sh.high[i] = 0u;
+    if (threadIdx.x == 0) sh.listed = 0;
+  }
+  __device__ void add_to_bin(int bin, unsigned long long v) {
+    if (v == 0ull) return;
+    const unsigned part = (unsigned)v, before = atomicAdd(&sh.low[bin], part);
+    const unsigned rest = (unsigned)(v >> 32) + (before + part < before ? 1u : 0u);
+    if (rest != 0u) atomicAdd(&sh.high[bin], rest);
+  }
+  // What lies in the cluster's bins up to each of this thread's, and of all; by the first CTA's threads.
+  __device__ void scan_bins(unsigned long long (&upto)[kBins / kFilterThreads], unsigned long long& all) {
+    unsigned long long mine[kBins / kFilterThreads], sum = 0ull;
+#pragma unroll
+    for (int i = 0; i < kBins / kFilterThreads; ++i) {
+      const int bin = threadIdx.x * (kBins / kFilterThreads) + i;
+      mine[i] = 0ull;
+      for (int c = 0; c < ctas; ++c) {
+        const unsigned* low = ctas > 1 ? cluster.map_shared_rank(sh.low, c) : sh.low;
+        const unsigned* high = ctas > 1 ? cluster.map_shared_rank(sh.high, c) : sh.high;
+        mine[i] += ((unsigned long long)high[bin] << 32) + low[bin];
+      }
+      sum += mine[i];
+    }
+    unsigned long long running = block_prefix(sum, all);
+#pragma unroll
+    for (int i = 0; i < kBins / kFilterThreads; ++i) upto[i] = running += mine[i];
+  }
+  // Puts a token on the first CTA's list if `wanted`; a warp's threads come together.  The list may be too short: its length says so.
+  __device__ void put(bool wanted, float l, int id) {
+    const unsigned who = __ballot_sync(0xffffffffu, wanted);
+    if (who == 0u) return;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(at_first(&sh.listed), __popc(who));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+    if (wanted && at < kListed) at_first(sh.list)[at] = ((unsigned long long)logit_key(l) << 32) | (unsigned)~id;
+  }
+  // Sorts n numbers of the list, falling (the order) or rising; by the first CTA's threads.
+  __device__ void sort(int n, bool falling) {
+    int size = 2;
+    while (size < n) size *= 2;
+    for (int i = n + threadIdx.x; i < size; i += kFilterThreads) sh.list[i] = falling ? 0ull : ~0ull;
+    __syncthreads();
+    for (int run = 2; run <= size; run *= 2)
+      for (int reach = run / 2; reach > 0; reach /= 2) {
+        for (int i = threadIdx.x; i < size / 2; i += kFilterThreads) {
+          const int a = 2 * i - (i & (reach - 1)), b = a + reach;
+          const unsigned long long x = sh.list[a], y = sh.list[b];
+          if ((x < y) == (((a & run) == 0) == falling)) sh.list[a] = y, sh.list[b] = x;
+        }
+        __syncthreads();
+      }
+  }
+
+  // Lists the tokens from the first of the order down to a bound with at least top_k of them above it; false if they are too many.
+  __device__ bool list_top(int top_k) {
+    clear_bins();
+    __syncthreads();
+    atomicAdd(&sh.low[thread_max == thread_max ? bin_of(thread_max) : kBins - 1], 1u);
+    sync();
+    if (rank == 0) {
+      unsigned long long upto[kBins / kFilterThreads], all;
+      scan_bins(upto, all);
+#pragma unroll
+      for (int i = 0; i < kBins / kFilterThreads; ++i) {
+        const unsigned long long before = i > 0 ? upto[i - 1] : upto[0] - bin_total(threadIdx.x * (kBins / kFilterThreads));
+        if (before < (unsigned long long)top_k && upto[i] >= (unsigned long long)top_k) sh.bin = threadIdx.x * (kBins / kFilterThreads) + i;
+      }
+    }
+    sync();
+    const int last = *at_first(&sh.bin);
+    if (last == kBins - 1) return false;   // (the same in all CTAs)
+    for (int i = threadIdx.x; i - (int)threadIdx.x < count; i += kFilterThreads) {
+      const float l = i < count ? sh.tokens[i] : __int_as_float(0x7fffffff);
+      put(i < count && bin_of(l) <= last, l, first_id + i);
+    }
+    sync();
+    const bool fits = *at_first(&sh.listed) <= kListed;
+    if (!fits) sync();   // (all have read it before the next search clears it)
+    return fits;
+  }
+  __device__ unsigned long long bin_total(int bin) {
+    unsigned long long sum = 0ull;
+    for (int c = 0; c < ctas; ++c) {
+      const unsigned* low = ctas > 1 ? cluster.map_shared_rank(sh.low, c) : sh.low;
+      const unsigned* high = ctas > 1 ? cluster.map_shared_rank(sh.high, c) : sh.high;
+      sum += ((unsigned long long)high[bin] << 32) + low[bin];
+    }
+    return sum;
+  }
+
+  // The rest of a row whose first top_k tokens are on the list; by the first CTA.
+  __device__ int choose_from_list(int top_k, float top_p, float u) {
+    if (rank != 0) return -1;
+    constexpr int kEach = kListed / kFilterThreads;
+    const int listed = sh.listed;
+    sort(listed, true);
+    const int number = min(top_k, listed);
+    // consecutive tokens of the order per thread
+    unsigned long long w[kEach], sum = 0ull, total;
+    int above_floor = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = threadIdx.x * kEach + i;
+      w[i] = at < number ? weight(key_logit((unsigned)(sh.list[at] >> 32))) : 0ull;
+      sum += w[i];
+      above_floor += at < number && w[i] >= floor_weight;
+    }
+    unsigned long long before = block_prefix(sum, total);
+    const unsigned long long wanted = top_p < 1.0f ? max(1ull, min(total, (unsigned long long)ceil((double)top_p * (double)total))) : ~0ull;
+    int kept_here = 0;   // of this thread's tokens: those in front of which top_p has not been reached, that are heavy enough (both stand in front of the others)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = threadIdx.x * kEach + i;
+      kept_here += at < number && before < wanted && w[i] >= floor_weight;
+      before += w[i];
+    }
+    unsigned long long kept;
+    block_prefix((unsigned long long)kept_here, kept);
+    const int many = max(1, (int)kept);
+    // in order of ids, the weight behind the id
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = threadIdx.x * kEach + i;
+      if (at < many) sh.list[at] = ((unsigned long long)~(unsigned)sh.list[at] << (kWeightBits + 1)) | w[i];
+    }
+    __syncthreads();
+    sort(many, false);
+    sum = 0ull;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = threadIdx.x * kEach + i;
+      w[i] = at < many ? sh.list[at] & ((2ull << kWeightBits) - 1ull) : 0ull;
+      sum += w[i];
+    }
+    before = block_prefix(sum, total);
+    const unsigned long long target = target_of(u, total);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (target >= before && target < before + w[i]) sh.chosen = (int)(sh.list[threadIdx.x * kEach + i] >> (kWeightBits + 1));
+      before += w[i];
+    }
+    __syncthreads();
+    return sh.chosen;
+  }
+  static __device__ unsigned long long target_of(float u, unsigned long long total) {
+    const unsigned long long target = u > 0.0f ? (unsigned long long)((double)fminf(u, 1.0f) * (double)total) : 0ull;
+    return target >= total ? total - 1ull : target;
+  }
+
+  // The shortest prefix of the order that brings `wanted`, or `share` of all that `within` holds, in number of tokens or in weight.
+  __device__ Border find(const Border& within, unsigned long long wanted, bool weights, float share) {
+    unsigned from = 0u, to = 0xffffffffu;   // keys among which the border lies (from level 1 on)
+    int shift = 0;
+    for (int level = 0;; ++level) {
+      auto bin = [&](float l, unsigned key) { return level == 0 ? bin_of(l) : (int)((to - key) >> shift); };
+      auto counts = [&](unsigned key, int id) { return within.holds(key, id) && (level == 0 || (key >= from && key <= to)); };
+      clear_bins();
+      __syncthreads();
+      for (int i = threadIdx.x; i < count; i += kFilterThreads) {
+        const float l = sh.tokens[i];
+        const unsigned key = logit_key(l);
+        if (counts(key, first_id + i)) add_to_bin(bin(l, key), weights ? weight(l) : 1ull);
+      }
+      sync();
+      if (rank == 0) {
+        unsigned long long upto[kBins / kFilterThreads], all;
+        scan_bins(upto, all);
+        const unsigned long long above = level == 0 ? 0ull : sh.above;
+        if (level == 0 && weights) wanted = max(1ull, min(all, (unsigned long long)ceil((double)share * (double)all)));
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kBins / kFilterThreads; ++i) {
+          const int here = threadIdx.x * (kBins / kFilterThreads) + i;
+          const unsigned long long before = i > 0 ? upto[i - 1] : upto[0] - bin_total(here);
+          if (above + before < wanted && above + upto[i] >= wanted) {
+            sh.bin = here;
+            sh.above = above + before;
+            sh.total = wanted;
+          }
+        }
+      }
+      sync();
+      const int border_bin = *at_first(&sh.bin);
+      wanted = *at_first(&sh.total);
+      unsigned lowest = 0xffffffffu, highest = 0u;
+      for (int i = threadIdx.x; i - (int)threadIdx.x < count; i += kFilterThreads) {
+        const float l = i < count ? sh.tokens[i] : 0.0f;
+        const unsigned key = logit_key(l);
+        const bool in_bin = i < count && counts(key, first_id + i) && bin(l, key) == border_bin;
+        if (in_bin) lowest = min(lowest, key), highest = max(highest, key);
+        put(in_bin, l, first_id + i);
+      }
+      sync();
+      if (*at_first(&sh.listed) <= kListed) {
+        if (rank == 0) border_of_list(wanted, weights);
+        sync();
+        return Border{*at_first(&sh.found_key), *at_first(&sh.found_id)};
+      }
+      to = (unsigned)cluster_max(highest);
+      from = ~(unsigned)cluster_max((unsigned)~lowest);
+      if (from == to) return border_of_equals(within, to, wanted, weights);
+      shift = max(0, 32 - __clz(to - from) - kBinBits);
+    }
+  }
+  // Where on the first CTA's list (the border's run) the border lies.
+  __device__ void border_of_list(unsigned long long wanted, bool weights) {
+    constexpr int kEach = kListed / kFilterThreads;
+    const int listed = sh.listed;
+    sort(listed, true);
+    unsigned long long w[kEach], sum = 0ull, all;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = threadIdx.x * kEach + i;
+      w[i] = at >= listed ? 0ull : weights ? weight(key_logit((unsigned)(sh.list[at] >> 32))) : 1ull;
+      sum += w[i];
+    }
+    unsigned long long before = sh.above + block_prefix(sum, all);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (before < wanted && before + w[i] >= wanted) {
+        const unsigned long long token = sh.list[threadIdx.x * kEach + i];
+        sh.found_key = (unsigned)(token >> 32);
+        sh.found_id = (int)~(unsigned)token;
+      }
+      before += w[i];
+    }
+  }
+  // The border among more tokens of one key than the list holds: so many of them, in order of ids, as are still wanted.
+  __device__ Border border_of_equals(const Border& within, unsigned key, unsigned long long wanted, bool weights) {
+    const unsigned long long each = weights ? weight(key_logit(key)) : 1ull, above = *at_first(&sh.above);
+    const unsigned long long number = (wanted - above + each - 1ull) / each;   // (a border in weight lies where there is some)
+    const int segment = (count + kFilterWarps - 1) / kFilterWarps, begin = min(count, warp * segment), end = min(count, begin + segment);
+    unsigned mine = 0u;
+    for (int i0 = begin; i0 < end; i0 += 32) {
+      const int i = i0 + lane;
+      const bool equal = i < end && logit_key(sh.tokens[i]) == key && within.holds(key, first_id + i);
+      mine += __popc(__ballot_sync(0xffffffffu, equal));
+    }
+    unsigned long long before, all;
+    before = block_prefix(lane == 0 ? (unsigned long long)mine : 0ull, all);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    const unsigned long long* of_cta = gather(all);
+    for (int c = 0; c < rank; ++c) before += of_cta[c];
+    if (before < number && before + mine >= number) {
+      unsigned left = (unsigned)(number - before);
+      for (int i0 = begin; i0 < end; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned who = __ballot_sync(0xffffffffu, i < end && logit_key(sh.tokens[i]) == key && within.holds(key, first_id + i));
+        const unsigned here = __popc(who);
+        if (left <= here) {
+          if ((who >> lane & 1u) && __popc(who & ((1u << lane) - 1u)) == (int)left - 1) *at_first(&sh.found_id) = first_id + i;
+          break;
+        }
+        left -= here;
+      }
+    }
+    sync();
+    return Border{key, *at_first(&sh.found_id)};
+  }
+
+  // The token that the number falls on among the kept ones, in order of ids; in the first CTA.
+  __device__ int draw(const Border& kept, float u) {
+    const int segment = (count + kFilterWarps - 1) / kFilterWarps, begin = min(count, warp * segment), end = min(count, begin + segment);
+    auto kept_weight = [&](int i) {
+      const float l = sh.tokens[i];
+      if (!kept.holds(logit_key(l), first_id + i)) return 0ull;
+      const unsigned long long w = weight(l);
+      return w >= floor_weight ? w : 0ull;
+    };
+    unsigned long long mine = 0ull;
+    for (int i = begin + lane; i < end; i += 32) mine += kept_weight(i);
+    mine = warp_sum_u64(mine);
+    unsigned long long all;
+    unsigned long long before = block_prefix(lane == 0 ? mine : 0ull, all);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    const unsigned long long* of_cta = gather(all);
+    unsigned long long total = 0ull;
+    for (int c = 0; c < ctas; ++c) {
+      if (c < rank) before += of_cta[c];
+      total += of_cta[c];
+    }
+    const unsigned long long target = target_of(u, total);
+    if (target >= before && target < before + mine) {
+      for (int i0 = begin; i0 < end; i0 += 32) {
+        const unsigned long long w = i0 + lane < end ? kept_weight(i0 + lane) : 0ull;
+        const unsigned long long upto = before + warp_prefix_u64(w, lane);
+        const unsigned past = __ballot_sync(0xffffffffu, target < upto);
+        if (past != 0u) {
+          if (lane == __ffs(past) - 1) *at_first(&sh.chosen) = first_id + i0 + lane;
+          break;
+        }
+        before = __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    sync();
+    return sh.chosen;
+  }
+};
+
 __global__ void __launch_bounds__(kFilterThreads)
-    sample_filtered_kernel(const float* __restrict__ logits, long long row_stride, int all_rows, int vocab, const int* __restrict__ rows, const float* __restrict__ temperature,
+    sample_filtered_kernel(const float* __restrict__ logits, long long row_stride, int all_rows, int vocab, int slice, const int* __restrict__ rows, const float* __restrict__ temperature,
                            const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniforms,
                            int* __restrict__ out) {
-  __shared__ unsigned long long scratch[32];
-  __shared__ unsigned long long prefix[kFilterThreads];
-  __shared__ unsigned long long best;
-  __shared__ int chosen;
-  const int index = rows != nullptr ? rows[blockIdx.x] : (int)blockIdx.x;
-  if (index < 0 || index >= all_rows) return;
-  const float* row = logits + (size_t)index * row_stride;
-
-  if (threadIdx.x == 0) best = 0ull;
-  __syncthreads();
-  unsigned long long mine = 0ull;   // key, then the id's complement: the larger of two is the earlier in the order
-  for (int i = threadIdx.x; i < vocab; i += blockDim.x) mine = max(mine, ((unsigned long long)logit_key(row[i]) << 32) | (unsigned)~i);
-  atomicMax(&best, mine);
-  __syncthreads();
-  const int first = (int)~(unsigned)best;
-  const float m = row[first];
-  const float temp = temperature[blockIdx.x];
-  if (!(temp > 0.0f) || !(m > -INFINITY)) {
-    if (threadIdx.x == 0) out[index] = m == m ? first : 0;   // a row of NaN: token 0
-    return;
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  __shared__ FilterShared shared;
+  const int set = blockIdx.x / cooperative_groups::this_cluster().num_blocks();
+  grid_dependency_wait();
+  const int index = rows != nullptr ? rows[set] : set;
+  if (index < 0 || index >= all_rows) return;   // (the whole cluster)
+  if (threadIdx.x == 0) {
+    shared.list = reinterpret_cast<unsigned long long*>(dynamic);
+    shared.low = reinterpret_cast<unsigned*>(dynamic + kListed * 8);
+    shared.high = shared.low + kBins;
+    shared.tokens = reinterpret_cast<float*>(shared.high + kBins);
   }
-  const Scale scale = weight_scale(temp);
-  const Border all = {0u, vocab};
-
-  // What the tokens of `within` bring that `border` holds: their number or their weight.
-  auto measure = [&](const Border& within, const Border& border, bool weights) {
-    unsigned long long sum = 0ull;
-    for (int i = threadIdx.x; i < vocab; i += blockDim.x) {
-      const float l = row[i];
-      const unsigned k = logit_key(l);
-      if (within.holds(k, i) && border.holds(k, i)) sum += weights ? token_weight(l, m, scale) : 1ull;
-    }
-    return block_sum_u64(sum, scratch);
-  };
-  // The shortest prefix of the order that brings `wanted` (which all of `within` does).
-  auto find = [&](const Border& within, unsigned long long wanted, bool weights) {
-    unsigned low = 0u, high = 0xffffffffu;   // the tokens with key >= low bring it, those with key >= high (NaN has no such key) do not
-    while (high - low > 1u) {
-      const unsigned middle = low + (high - low) / 2u;
-      if (measure(within, {middle, vocab}, weights) >= wanted) low = middle;
-      else high = middle;
-    }
-    int none = -1, enough = vocab;
-    while (enough - none > 1) {
-      const int middle = none + (enough - none) / 2;
-      if (measure(within, {low, middle}, weights) >= wanted) enough = middle;
-      else none = middle;
-    }
-    return Border{low, enough};
-  };
-
-  Border kept = all;
-  const int k = top_k[blockIdx.x];
-  if (k > 0 && k < vocab) kept = find(all, (unsigned long long)k, false);
-  const float p = top_p[blockIdx.x];
-  const float smallest = min_p[blockIdx.x];
-  unsigned long long floor_weight = 0ull;
-  if (smallest > 0.0f) floor_weight = smallest >= 1.0f ? 1ull << kWeightBits : (unsigned long long)ceil((double)smallest * (double)(1ull << kWeightBits));
-  if (p < 1.0f) {
-    const unsigned long long total = measure(all, kept, true);
-    const unsigned long long wanted = p > 0.0f ? (unsigned long long)ceil((double)p * (double)total) : 1ull;
-    kept = find(kept, max(1ull, min(wanted, total)), true);
-  }
-  const bool first_only = smallest > 1.0f;
-  auto weight = [&](int i) -> unsigned long long {
-    const float l = row[i];
-    if (!kept.holds(logit_key(l), i) || (first_only && i != first)) return 0ull;
-    const unsigned long long w = token_weight(l, m, scale);
-    return w >= floor_weight ? w : 0ull;
-  };
-
-  // consecutive tokens per thread, so that the walk is in order of ids
-  const int each = (vocab + blockDim.x - 1) / blockDim.x;
-  const int begin = min(vocab, (int)threadIdx.x * each), end = min(vocab, begin + each);
-  unsigned long long sum = 0ull;
-  for (int i = begin; i < end; ++i) sum += weight(i);
-  const unsigned long long total = block_sum_u64(sum, scratch);
-  prefix[threadIdx.x] = sum;
-  __syncthreads();
-  unsigned long long start = 0ull;
-  for (int t = 0; t < (int)threadIdx.x; ++t) start += prefix[t];
-  const float u = uniforms[blockIdx.x];
-  unsigned long long target = u > 0.0f ? (unsigned long long)((double)fminf(u, 1.0f) * (double)total) : 0ull;
-  if (target >= total) target = total - 1ull;
-  if (threadIdx.x == 0) chosen = first;
-  __syncthreads();
-  if (target >= start && target < start + sum) {
-    int i = begin;
-    for (unsigned long long running = start + weight(i); running <= target; running += weight(i)) ++i;
-    chosen = i;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) out[index] = chosen;
+  if (cooperative_groups::this_cluster().num_blocks() > 1) cooperative_groups::this_cluster().sync();   // (a CTA's shared memory may be written once the CTA runs)
+  else __syncthreads();
+  RowFilter filter(shared, logits + (size_t)index * row_stride, vocab, slice);
+  filter.load();
+  const int token = filter.choose(temperature[set], top_k[set], top_p[set], min_p[set], uniforms[set]);
+  if (cooperative_groups::this_cluster().block_rank() == 0 && threadIdx.x == 0) out[index] = token;
+  if (cooperative_groups::this_cluster().num_blocks() > 1) cooperative_groups::this_cluster().sync();   // nobody leaves while another reads what it holds
 }
 
 __global__ void uniforms_kernel(const long long* __restrict__ seeds, const long long* __restrict__ counters, float* __restrict__ out, int count) {
@@ -202,8 +587,28 @@ TLIE_EXPORT int tlie_sample_filtered(const float* logits, long long row_stride, 
                                      const int* top_k, const float* top_p, const float* min_p, const float* uniforms, int* out, cudaStream_t stream) {
   if (count <= 0) return 0;
   if (vocab <= 0 || vocab > kFilterMaxVocab || row_stride < 0) return (int)cudaErrorInvalidValue;
-  sample_filtered_kernel<<<count, kFilterThreads, 0, stream>>>(logits, row_stride, all_rows, vocab, rows, temperature, top_k, top_p, min_p, uniforms, out);
-  return (int)cudaGetLastError();
+  // CTAs of a row's cluster: slices of at most 16,384 tokens (two CTAs' fit an SM, one loads while the other works), and for few rows down to 2,048.
+  int ctas = 1;
+  while (ctas < 8 && (vocab > ctas * 16384 || (vocab > ctas * 2048 && (long long)count * ctas * 2 <= 2 * device_sm_count()))) ctas *= 2;
+  const int slice = ((vocab + ctas - 1) / ctas + 3) & ~3;
+  const size_t smem = kListed * 8 + kBins * 8 + (size_t)slice * 4;
+  static std::atomic<unsigned long long> devices{0};
+  cudaError_t e = allow_shared_memory(sample_filtered_kernel, kListed * 8 + kBins * 8 + kMostSlice * 4, devices);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)count * ctas);
+  config.blockDim = dim3(kFilterThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute[2];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = ctas;
+  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 2;
+  return (int)cudaLaunchKernelEx(&config, sample_filtered_kernel, logits, row_stride, all_rows, vocab, slice, rows, temperature, top_k, top_p, min_p, uniforms, out);
 }
 
 TLIE_EXPORT int tlie_uniforms(const long long* seeds, const long long* counters, float* out, int count, cudaStream_t stream) {
