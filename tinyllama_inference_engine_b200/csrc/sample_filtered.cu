@@ -17,8 +17,8 @@
 namespace tlie {
 
 constexpr int kFilterThreads = 512, kFilterWarps = kFilterThreads / 32;
-constexpr int kBinBits = 10, kBins = 1 << kBinBits;
-constexpr int kListed = 2048;                            // tokens that the first CTA of a cluster can sort
+constexpr int kBinBits = 10, kBins = 1 << kBinBits, kBinsEach = kBins / kFilterThreads;
+constexpr int kListed = 2048, kListedEach = kListed / kFilterThreads;   // tokens that the first CTA of a cluster can sort
 constexpr int kMostSlice = 49152;                        // tokens of a CTA: 192 KB
 constexpr int kFilterMaxVocab = 8 * kMostSlice;          // (weights of 2^44 and less, fewer than 2^19 of them: sums fit 64 bits, a token's id and weight one number)
 constexpr int kWeightBits = 44;
@@ -74,24 +74,27 @@ struct Border {
   __device__ bool holds(unsigned k, int i) const { return k > key || (k == key && i <= id); }
 };
 
-// A row's tokens lie in the shared memory of a cluster of CTAs, consecutive ones in each.
+// A row's tokens lie in the shared memory of a cluster of CTAs, consecutive ones in each; what follows its first maximum is mostly done by the first CTA on a short
+// list of the order's first tokens.  As many threads' maxima as are asked for bound the list from below (so many tokens at least are not below the least of them), and the highest
+// of the CTAs' bounds holds for all.  With top_k so many tokens are asked for and all others are out of it; with top_p alone some hundred, and the exact weight of all
+// tokens tells whether they suffice; min_p alone says itself which tokens it leaves.  Bound by the reading of the logits then, or, with top_p alone, by the 35 instructions of a
+// token's exact weight; one row by the chain of its steps.
 //
-// Bound by the reading of the logits where there are many rows, else by the chain of steps that each need the cluster's answer before.  So a step asks for much: a
-// border (of top_k by number of tokens, of top_p by weight) is found from a histogram over 1,024 runs of logits, 1/32 wide, below the largest, and the tokens of
-// the run that it falls in, which the first CTA sorts.  Where those are too many (equal logits, or very close ones) the run is cut by the bits of the logits, and equal ones by id.
-// top_k of up to some hundred needs less: as many threads' maxima as top_k asks for bound the last logit that counts from below, what is not
-// below that bound is a short list, and the rest is done on the list by the first CTA.
+// Where the list does not do (top_k beyond it, flat rows), a border is found from a histogram over 1,024 runs of logits, 1/32 wide, below the largest, of numbers or
+// of exact weights, and from the tokens of the run that it falls in, which the first CTA sorts.  Where those are too many (equal logits, or very close ones) the run is
+// cut by the bits of the logits, and equal ones by id.
 struct FilterShared {
   float* tokens;                  // this CTA's
   unsigned *low, *high;           // a histogram's numbers, 64 bits in two words: an atomic of 64 bits on shared memory is a loop
-  unsigned long long* list;
+  unsigned long long* list;       // (over the histogram: one is done with before the other begins)
   unsigned long long scan[kFilterWarps];
-  unsigned long long gather[2][8];   // one number per CTA
-  unsigned long long weight_of_warp[kFilterWarps];
+  unsigned long long gather[2][2][8];   // two numbers per CTA
   unsigned long long above;       // the first CTA's are the cluster's, as are:
-  unsigned long long total;
+  unsigned long long wanted;
   int bin, listed, chosen, found_id;
   unsigned found_key;
+  int last_run[2];
+  unsigned least[2];
 };
 
 __device__ __forceinline__ unsigned long long warp_sum_u64(unsigned long long v) {
@@ -107,6 +110,42 @@ __device__ __forceinline__ unsigned long long warp_prefix_u64(unsigned long long
   }
   return v;
 }
+// Sum over the CTA's threads before this one, and of all.
+__device__ __noinline__ unsigned long long block_prefix(unsigned long long v, unsigned long long* scan, unsigned long long& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned long long upto = warp_prefix_u64(v, lane);
+  __syncthreads();
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  unsigned long long before = 0ull, sum = 0ull;
+#pragma unroll
+  for (int w = 0; w < kFilterWarps; ++w) {
+    const unsigned long long here = scan[w];
+    if (w < warp) before += here;
+    sum += here;
+  }
+  all = sum;
+  return before + upto - v;
+}
+// Sorts n numbers of a list, falling or rising, by the CTA's threads.
+__device__ __noinline__ void sort_list(unsigned long long* list, int n, bool falling) {
+  int size = 2;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += kFilterThreads) list[i] = falling ? 0ull : ~0ull;
+  __syncthreads();
+  for (int run = 2; run <= size; run *= 2)
+    for (int reach = run / 2; reach > 0; reach /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += kFilterThreads) {
+        const int a = 2 * i - (i & (reach - 1)), b = a + reach;
+        const unsigned long long x = list[a], y = list[b];
+        if ((x < y) == (((a & run) == 0) == falling)) list[a] = y, list[b] = x;
+      }
+      if (reach > 32 || size > 64) __syncthreads();
+      else __syncwarp();   // (one warp has it all)
+    }
+  __syncthreads();
+}
+__device__ __forceinline__ float key_logit(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 // One row, by the threads of a cluster.
 class RowFilter {
@@ -115,17 +154,97 @@ class RowFilter {
       : sh(shared), cluster(cooperative_groups::this_cluster()), row(row), vocab(vocab), ctas(cluster.num_blocks()), rank(cluster.block_rank()),
         lane(threadIdx.x & 31), warp(threadIdx.x >> 5), first_id(min(vocab, rank * slice)), count(min(vocab, (rank + 1) * slice) - first_id) {}
 
-  // Brings the tokens into shared memory; the first one of the order.
-  __device__ void load() {
+  // The row's token, in the first CTA.
+  __device__ int choose(float temperature, int top_k, float top_p, float min_p, float u) {
+    const bool by_number = top_k > 0 && top_k < vocab, by_weight = top_p < 1.0f;
+    const bool first_only = !(temperature > 0.0f) || top_k == 1 || min_p > 1.0f || top_p <= 0.0f;
+    load();
+    // this CTA's maximum, and its bound for the list
+    const float largest = block_max(thread_max);
+    const int asked = first_only ? 0 : by_number ? top_k : by_weight ? kGuess : 0;
+    // What all of the tokens asked for are not below in one CTA, and what a CTA's share of them is not below in any.
+    uint2 bounds = make_uint2(logit_key(-INFINITY), logit_key(-INFINITY));
+    if (asked > 0 && largest > -INFINITY) bounds = least_of_maxima(largest, asked, (asked + ctas - 1) / ctas);
+    arrived();
+    const unsigned long long* all = gather(logit_key(largest), ((unsigned long long)bounds.x << 32) | bounds.y);
+    unsigned key = 0u, in_one = 0u, in_any = 0xffffffffu;
+    for (int c = 0; c < ctas; ++c) key = max(key, (unsigned)all[c]), in_one = max(in_one, (unsigned)(all[8 + c] >> 32)), in_any = min(in_any, (unsigned)all[8 + c]);
+    m = key_logit(key);
+    float bound = key_logit(max(in_one, in_any));
+    if (!any_token(key)) return 0;                        // a row of NaN
+    if (first_only || !(m > -INFINITY)) return first_of_order();
+
+    scale = weight_scale(temperature);
+    floor_weight = min_p > 0.0f ? (unsigned long long)ceil((double)min_p * (double)(1ull << kWeightBits)) : 0ull;
+    const bool by_floor = !by_number && !by_weight && floor_weight > 0ull;
+    if (by_floor) bound = m + temperature * (logf(min_p) * 1.0001f - 0.001f);   // (a little low: the list is longer than what stays of it)
+    if (bound > -INFINITY) {
+      unsigned long long mine = 0ull, total = 0ull;
+      list_from(bound, by_weight && !by_number, mine);
+      if (by_weight && !by_number) {
+        block_prefix(mine, sh.scan, mine);
+        all = gather(mine, 0ull);
+        for (int c = 0; c < ctas; ++c) total += all[c];
+      } else {
+        sync();
+      }
+      if (*at_first(&sh.listed) <= kListed) {
+        if (by_number || by_floor) return rank == 0 ? choose_from_list(by_number ? top_k : kListed, top_p, 0ull, u) : 0;
+        if (rank == 0) {
+          const int token = choose_from_list(kListed, top_p, total, u);
+          if (threadIdx.x == 0) sh.chosen = token;
+        }
+        sync();
+        if (*at_first(&sh.chosen) >= 0) return sh.chosen;
+      }
+      sync();   // (all have read the list's length before the next search clears it)
+    }
+    Border kept = {0u, vocab};
+#pragma unroll 1
+    for (int by = 0; by < 2; ++by)
+      if (by == 0 ? by_number : by_weight) kept = find(kept, (unsigned long long)top_k, by == 1, top_p);
+    return draw(kept, u);
+  }
+
+  __device__ void arrive() {   // (a CTA's shared memory may be written once the CTA runs)
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  }
+
+ private:
+  static constexpr int kGuess = 256;
+  FilterShared& sh;
+  cooperative_groups::cluster_group cluster;
+  const float* row;
+  const int vocab, ctas, rank, lane, warp, first_id, count;
+  float m, thread_max;
+  Scale scale;
+  unsigned long long floor_weight;
+  int gathers = 0;
+
+  __device__ static bool any_token(unsigned key) { return key != 0u; }
+  __device__ __forceinline__ unsigned long long weight(float l) const { return token_weight(l, m, scale); }
+  __device__ void sync() {
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+  }
+  __device__ void arrived() {
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  }
+  template <typename T>
+  __device__ __forceinline__ T* at_first(T* mine) {   // the first CTA's
+    return ctas > 1 ? cluster.map_shared_rank(mine, 0) : mine;
+  }
+  // The run below `top` that a logit falls in: monotone, and the last one is for all that lies further below.
+  __device__ static int bin_below(float top, float l) { return l == top ? 0 : (int)fminf((top - l) * 32.0f, (float)(kBins - 1)); }
+
+  // Brings the tokens into shared memory; this thread's largest (NaN is none).
+  __device__ __forceinline__ void load() {
     float best = -INFINITY;
-    int id = 0x7fffffff;
-    auto take = [&](float l, int i) {
-      if (l > best || (l == best && i < id)) best = l, id = i;
-    };
+    bool some = false;   // a token that is not NaN
     const float* from = row + first_id;
+    constexpr int kFlight = 8;
     if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
       const int quads = count >> 2;
-      constexpr int kFlight = 8;
       for (int q0 = threadIdx.x; q0 < quads; q0 += kFlight * kFilterThreads) {
         float4 v[kFlight];
 #pragma unroll
@@ -133,18 +252,19 @@ class RowFilter {
           if (q0 + u * kFilterThreads < quads) v[u] = reinterpret_cast<const float4*>(from)[q0 + u * kFilterThreads];
 #pragma unroll
         for (int u = 0; u < kFlight; ++u) {
-          const int q = q0 + u * kFilterThreads;
-          if (q >= quads) break;
-          reinterpret_cast<float4*>(sh.tokens)[q] = v[u];
-          take(v[u].x, 4 * q), take(v[u].y, 4 * q + 1), take(v[u].z, 4 * q + 2), take(v[u].w, 4 * q + 3);
+          if (q0 + u * kFilterThreads >= quads) break;
+          reinterpret_cast<float4*>(sh.tokens)[q0 + u * kFilterThreads] = v[u];
+          best = fmaxf(fmaxf(best, fmaxf(v[u].x, v[u].y)), fmaxf(v[u].z, v[u].w));
+          some |= v[u].x == v[u].x || v[u].y == v[u].y || v[u].z == v[u].z || v[u].w == v[u].w;
         }
       }
-      for (int i = 4 * quads + threadIdx.x; i < count; i += kFilterThreads) {
+      const int i = 4 * quads + threadIdx.x;
+      if (i < count) {
         sh.tokens[i] = from[i];
-        take(sh.tokens[i], i);
+        best = fmaxf(best, sh.tokens[i]);
+        some |= sh.tokens[i] == sh.tokens[i];
       }
     } else {
-      constexpr int kFlight = 8;
       for (int i0 = threadIdx.x; i0 < count; i0 += kFlight * kFilterThreads) {
         float v[kFlight];
 #pragma unroll
@@ -152,125 +272,94 @@ class RowFilter {
           if (i0 + u * kFilterThreads < count) v[u] = from[i0 + u * kFilterThreads];
 #pragma unroll
         for (int u = 0; u < kFlight; ++u) {
-          const int i = i0 + u * kFilterThreads;
-          if (i >= count) break;
-          sh.tokens[i] = v[u];
-          take(v[u], i);
+          if (i0 + u * kFilterThreads >= count) break;
+          sh.tokens[i0 + u * kFilterThreads] = v[u];
+          best = fmaxf(best, v[u]);
+          some |= v[u] == v[u];
         }
       }
     }
-    thread_max = best;
-    unsigned long long mine = id == 0x7fffffff ? 0ull : ((unsigned long long)logit_key(best) << 32) | (unsigned)~(first_id + id);
-    mine = cluster_max(mine);
-    first = mine == 0ull ? 0 : (int)~(unsigned)mine;
-    m = mine == 0ull ? __int_as_float(0x7fffffff) : key_logit((unsigned)(mine >> 32));
+    thread_max = some ? best : __int_as_float(0x7fffffff);
   }
-
-  // The token of the row.
-  __device__ int choose(float temperature, int top_k, float top_p, float min_p, float u) {
-    if (mine_is_nan()) return 0;
-    if (!(temperature > 0.0f) || !(m > -INFINITY) || top_k == 1 || !(min_p <= 1.0f || min_p != min_p) || top_p <= 0.0f) return first;
-    scale = weight_scale(temperature);
-    floor_weight = min_p > 0.0f ? (unsigned long long)ceil((double)min_p * (double)(1ull << kWeightBits)) : 0ull;
-    const bool by_number = top_k > 0 && top_k < vocab, by_weight = top_p < 1.0f;
-    if (by_number && top_k <= kFilterThreads * ctas && list_top(top_k)) return choose_from_list(top_k, top_p, u);
-    Border kept = {0u, vocab};
-    if (by_number) kept = find(kept, (unsigned long long)top_k, false, 0.0f);
-    if (by_weight) kept = find(kept, 0ull, true, top_p);
-    return draw(kept, u);
-  }
-
- private:
-  FilterShared& sh;
-  cooperative_groups::cluster_group cluster;
-  const float* row;
-  const int vocab, ctas, rank, lane, warp, first_id, count;
-  float m, thread_max;
-  int first;
-  Scale scale;
-  unsigned long long floor_weight;
-  int gathers = 0;
-
-  __device__ bool mine_is_nan() const { return m != m; }
-  static __device__ float key_logit(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
-  __device__ unsigned long long weight(float l) const { return token_weight(l, m, scale); }
-  __device__ void sync() {
-    if (ctas > 1) cluster.sync();
-    else __syncthreads();
-  }
-  template <typename T>
-  __device__ T* at_first(T* mine) {   // the first CTA's
-    return ctas > 1 ? cluster.map_shared_rank(mine, 0) : mine;
-  }
-  // The run that a logit falls in: monotone, and the last one is for all that lies further below.
-  __device__ int bin_of(float l) const { return l == m ? 0 : (int)fminf((m - l) * 32.0f, (float)(kBins - 1)); }
-
-  // Every CTA's number, in every CTA (a CTA's threads bring the same).  Two places in turn: a CTA is past its reading of one when it brings the one after the next.
-  __device__ const unsigned long long* gather(unsigned long long mine) {
-    unsigned long long* place = sh.gather[gathers ^= 1];
-    if (threadIdx.x < ctas) *(ctas > 1 ? cluster.map_shared_rank(&place[rank], threadIdx.x) : &place[0]) = mine;
-    sync();
-    return place;
-  }
-  __device__ unsigned long long cluster_max(unsigned long long v) {
+  // NaN if all are.
+  __device__ __forceinline__ float block_max(float v) {
 #pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, offset));
+    for (int offset = 16; offset > 0; offset >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, offset));
+    if (lane == 0) sh.scan[warp] = __float_as_uint(v);
     __syncthreads();
-    if (lane == 0) sh.scan[warp] = v;
-    __syncthreads();
-    v = sh.scan[lane % kFilterWarps];
+    v = __uint_as_float((unsigned)sh.scan[lane % kFilterWarps]);
 #pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, offset));
-    const unsigned long long* all = gather(v);
-    for (int c = 0; c < ctas; ++c) v = max(v, all[c]);
+    for (int offset = 16; offset > 0; offset >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, offset));
     return v;
   }
-  // Sum over the threads before this one, and of all of this CTA.
-  __device__ unsigned long long block_prefix(unsigned long long v, unsigned long long& all) {
-    const unsigned long long upto = warp_prefix_u64(v, lane);
+  // Logits, as keys, that at least `asked` and at least `share` threads' maxima are not below: the least of those that lie in the runs which together hold so many.
+  __device__ __forceinline__ uint2 least_of_maxima(float largest, int asked, int share) {
+    for (int i = threadIdx.x; i < kBins; i += kFilterThreads) sh.low[i] = 0u;
+    if (threadIdx.x < 2) sh.last_run[threadIdx.x] = kBins - 1, sh.least[threadIdx.x] = 0xffffffffu;
     __syncthreads();
+    const int bin = bin_below(largest, thread_max);   // (of a thread without a token the last)
+    atomicAdd(&sh.low[bin], 1u);
+    __syncthreads();
+    const unsigned first = sh.low[threadIdx.x * kBinsEach], second = sh.low[threadIdx.x * kBinsEach + 1];
+    static_assert(kBinsEach == 2, "two runs per thread");
+    unsigned upto = first + second;
+#pragma unroll
+    for (int offset = 1; offset < 32; offset <<= 1) {
+      const unsigned other = __shfl_up_sync(0xffffffffu, upto, offset);
+      if (lane >= offset) upto += other;
+    }
     if (lane == 31) sh.scan[warp] = upto;
     __syncthreads();
-    unsigned long long before = 0ull;
-    all = 0ull;
+    unsigned before = upto - first - second;
+    for (int w = 0; w < warp; ++w) before += (unsigned)sh.scan[w];
 #pragma unroll
-    for (int w = 0; w < kFilterWarps; ++w) {
-      const unsigned long long here = sh.scan[w];
-      if (w < warp) before += here;
-      all += here;
+    for (int i = 0; i < 2; ++i) {
+      const unsigned number = i == 0 ? asked : share;
+      if (before < number && before + first >= number) sh.last_run[i] = threadIdx.x * kBinsEach;
+      else if (before + first < number && before + first + second >= number) sh.last_run[i] = threadIdx.x * kBinsEach + 1;
     }
-    return before + upto - v;
-  }
-  __device__ void clear_bins() {
-    for (int i = threadIdx.x; i < kBins; i += kFilterThreads) sh.low[i] = sh.high[i] = 0u;
-    if (threadIdx.x == 0) sh.listed = 0;
-  }
-  __device__ void add_to_bin(int bin, unsigned long long v) {
-    if (v == 0ull) return;
-    const unsigned part = (unsigned)v, before = atomicAdd(&sh.low[bin], part);
-    const unsigned rest = (unsigned)(v >> 32) + (before + part < before ? 1u : 0u);
-    if (rest != 0u) atomicAdd(&sh.high[bin], rest);
-  }
-  // What lies in the cluster's bins up to each of this thread's, and of all; by the first CTA's threads.
-  __device__ void scan_bins(unsigned long long (&upto)[kBins / kFilterThreads], unsigned long long& all) {
-    unsigned long long mine[kBins / kFilterThreads], sum = 0ull;
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kBins / kFilterThreads; ++i) {
-      const int bin = threadIdx.x * (kBins / kFilterThreads) + i;
-      mine[i] = 0ull;
-      for (int c = 0; c < ctas; ++c) {
-        const unsigned* low = ctas > 1 ? cluster.map_shared_rank(sh.low, c) : sh.low;
-        const unsigned* high = ctas > 1 ? cluster.map_shared_rank(sh.high, c) : sh.high;
-        mine[i] += ((unsigned long long)high[bin] << 32) + low[bin];
+    for (int i = 0; i < 2; ++i) {
+      const unsigned least = __reduce_min_sync(0xffffffffu, bin <= sh.last_run[i] && sh.last_run[i] < kBins - 1 ? logit_key(thread_max) : 0xffffffffu);
+      if (lane == 0) atomicMin(&sh.least[i], least);
+    }
+    __syncthreads();
+    const unsigned none = logit_key(-INFINITY);   // (so few, or so far below, that runs tell no more)
+    return make_uint2(sh.least[0] == 0xffffffffu ? none : sh.least[0], sh.least[1] == 0xffffffffu ? none : sh.least[1]);
+  }
+
+  // Two numbers of every CTA, in every CTA (a CTA's threads bring the same).  Two places in turn: a CTA is past its reading of one when it brings the one after the next.
+  __device__ __forceinline__ const unsigned long long* gather(unsigned long long mine, unsigned long long second) {
+    auto& place = sh.gather[gathers ^= 1];
+    if (threadIdx.x < ctas) {
+      auto* to = ctas > 1 ? cluster.map_shared_rank(&place[0][rank], threadIdx.x) : &place[0][0];
+      to[0] = mine;
+      to[8] = second;
+    }
+    sync();
+    return place[0];
+  }
+  // The first token of the order.
+  __device__ __forceinline__ int first_of_order() {
+    int id = 0x7fffffff;
+    for (int i = threadIdx.x; i < count; i += kFilterThreads)
+      if (sh.tokens[i] == m) {
+        id = first_id + i;
+        break;
       }
-      sum += mine[i];
-    }
-    unsigned long long running = block_prefix(sum, all);
-#pragma unroll
-    for (int i = 0; i < kBins / kFilterThreads; ++i) upto[i] = running += mine[i];
+    id = __reduce_min_sync(0xffffffffu, id);
+    if (threadIdx.x == 0) sh.found_id = 0x7fffffff;
+    __syncthreads();
+    if (lane == 0) atomicMin(&sh.found_id, id);
+    __syncthreads();
+    const unsigned long long* all = gather(sh.found_id, 0ull);
+    for (int c = 0; c < ctas; ++c) id = c == 0 ? (int)all[0] : min(id, (int)all[c]);
+    return id;
   }
+
   // Puts a token on the first CTA's list if `wanted`; a warp's threads come together.  The list may be too short: its length says so.
-  __device__ void put(bool wanted, float l, int id) {
+  __device__ __forceinline__ void put(bool wanted, float l, int id) {
     const unsigned who = __ballot_sync(0xffffffffu, wanted);
     if (who == 0u) return;
     int at = 0;
@@ -278,127 +367,101 @@ class RowFilter {
     at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
     if (wanted && at < kListed) at_first(sh.list)[at] = ((unsigned long long)logit_key(l) << 32) | (unsigned)~id;
   }
-  // Sorts n numbers of the list, falling (the order) or rising; by the first CTA's threads.
-  __device__ void sort(int n, bool falling) {
-    int size = 2;
-    while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += kFilterThreads) sh.list[i] = falling ? 0ull : ~0ull;
-    __syncthreads();
-    for (int run = 2; run <= size; run *= 2)
-      for (int reach = run / 2; reach > 0; reach /= 2) {
-        for (int i = threadIdx.x; i < size / 2; i += kFilterThreads) {
-          const int a = 2 * i - (i & (reach - 1)), b = a + reach;
-          const unsigned long long x = sh.list[a], y = sh.list[b];
-          if ((x < y) == (((a & run) == 0) == falling)) sh.list[a] = y, sh.list[b] = x;
-        }
-        __syncthreads();
+  // Lists the tokens that are not below the bound; with `weights` their weight and that of all others, this thread's share of it.
+  __device__ __forceinline__ void list_from(float bound, bool weights, unsigned long long& mine) {
+    if (weights) {
+      for (int i = threadIdx.x; i - (int)threadIdx.x < count; i += kFilterThreads) {
+        const float l = i < count ? sh.tokens[i] : __int_as_float(0x7fffffff);
+        mine += weight(l);
+        put(l >= bound, l, first_id + i);
       }
+      return;
+    }
+    const int quads = (count + 3) >> 2;   // (tokens behind the last one are NaN)
+    for (int q = threadIdx.x; q - (int)threadIdx.x < quads; q += kFilterThreads) {
+      const float nan = __int_as_float(0x7fffffff);
+      const float4 v = q < quads ? reinterpret_cast<const float4*>(sh.tokens)[q] : make_float4(nan, nan, nan, nan);
+      if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) continue;
+      put(v.x >= bound, v.x, first_id + 4 * q);
+      put(v.y >= bound, v.y, first_id + 4 * q + 1);
+      put(v.z >= bound, v.z, first_id + 4 * q + 2);
+      put(v.w >= bound, v.w, first_id + 4 * q + 3);
+    }
   }
 
-  // Lists the tokens from the first of the order down to a bound with at least top_k of them above it; false if they are too many.
-  __device__ bool list_top(int top_k) {
-    clear_bins();
-    __syncthreads();
-    atomicAdd(&sh.low[thread_max == thread_max ? bin_of(thread_max) : kBins - 1], 1u);
-    sync();
-    if (rank == 0) {
-      unsigned long long upto[kBins / kFilterThreads], all;
-      scan_bins(upto, all);
-#pragma unroll
-      for (int i = 0; i < kBins / kFilterThreads; ++i) {
-        const unsigned long long before = i > 0 ? upto[i - 1] : upto[0] - bin_total(threadIdx.x * (kBins / kFilterThreads));
-        if (before < (unsigned long long)top_k && upto[i] >= (unsigned long long)top_k) sh.bin = threadIdx.x * (kBins / kFilterThreads) + i;
-      }
-    }
-    sync();
-    const int last = *at_first(&sh.bin);
-    if (last == kBins - 1) return false;   // (the same in all CTAs)
-    for (int i = threadIdx.x; i - (int)threadIdx.x < count; i += kFilterThreads) {
-      const float l = i < count ? sh.tokens[i] : __int_as_float(0x7fffffff);
-      put(i < count && bin_of(l) <= last, l, first_id + i);
-    }
-    sync();
-    const bool fits = *at_first(&sh.listed) <= kListed;
-    if (!fits) sync();   // (all have read it before the next search clears it)
-    return fits;
-  }
-  __device__ unsigned long long bin_total(int bin) {
-    unsigned long long sum = 0ull;
-    for (int c = 0; c < ctas; ++c) {
-      const unsigned* low = ctas > 1 ? cluster.map_shared_rank(sh.low, c) : sh.low;
-      const unsigned* high = ctas > 1 ? cluster.map_shared_rank(sh.high, c) : sh.high;
-      sum += ((unsigned long long)high[bin] << 32) + low[bin];
-    }
-    return sum;
-  }
-
-  // The rest of a row whose first top_k tokens are on the list; by the first CTA.
-  __device__ int choose_from_list(int top_k, float top_p, float u) {
-    if (rank != 0) return -1;
-    constexpr int kEach = kListed / kFilterThreads;
+  // The row's token if its first top_k tokens (or all that min_p leaves, or, where `total` is the weight of all tokens, all that top_p leaves) are on the list; by the first CTA.  -1: the
+  // list's weight does not reach top_p of `total`.
+  __device__ __forceinline__ int choose_from_list(int top_k, float top_p, unsigned long long total, float u) {
     const int listed = sh.listed;
-    sort(listed, true);
+    __syncthreads();
+    sort_list(sh.list, listed, true);
     const int number = min(top_k, listed);
     // consecutive tokens of the order per thread
-    unsigned long long w[kEach], sum = 0ull, total;
-    int above_floor = 0;
+    unsigned long long w[kListedEach], sum = 0ull, on_list;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = threadIdx.x * kEach + i;
+    for (int i = 0; i < kListedEach; ++i) {
+      const int at = threadIdx.x * kListedEach + i;
       w[i] = at < number ? weight(key_logit((unsigned)(sh.list[at] >> 32))) : 0ull;
       sum += w[i];
-      above_floor += at < number && w[i] >= floor_weight;
     }
-    unsigned long long before = block_prefix(sum, total);
-    const unsigned long long wanted = top_p < 1.0f ? max(1ull, min(total, (unsigned long long)ceil((double)top_p * (double)total))) : ~0ull;
-    int kept_here = 0;   // of this thread's tokens: those in front of which top_p has not been reached, that are heavy enough (both stand in front of the others)
+    unsigned long long before = block_prefix(sum, sh.scan, on_list);
+    const unsigned long long of = total != 0ull ? total : on_list;
+    const unsigned long long wanted = top_p < 1.0f ? max(1ull, min(of, (unsigned long long)ceil((double)top_p * (double)of))) : ~0ull;
+    if (total != 0ull && on_list < wanted) return -1;
+    unsigned long long here = 0ull, kept;   // of this thread's tokens: those in front of which top_p has not been reached, that are heavy enough (both stand in front of the others)
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = threadIdx.x * kEach + i;
-      kept_here += at < number && before < wanted && w[i] >= floor_weight;
+    for (int i = 0; i < kListedEach; ++i) {
+      here += threadIdx.x * kListedEach + i < number && before < wanted && w[i] >= floor_weight;
       before += w[i];
     }
-    unsigned long long kept;
-    block_prefix((unsigned long long)kept_here, kept);
+    block_prefix(here, sh.scan, kept);
     const int many = max(1, (int)kept);
     // in order of ids, the weight behind the id
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = threadIdx.x * kEach + i;
+    for (int i = 0; i < kListedEach; ++i) {
+      const int at = threadIdx.x * kListedEach + i;
       if (at < many) sh.list[at] = ((unsigned long long)~(unsigned)sh.list[at] << (kWeightBits + 1)) | w[i];
     }
     __syncthreads();
-    sort(many, false);
+    sort_list(sh.list, many, false);
     sum = 0ull;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = threadIdx.x * kEach + i;
+    for (int i = 0; i < kListedEach; ++i) {
+      const int at = threadIdx.x * kListedEach + i;
       w[i] = at < many ? sh.list[at] & ((2ull << kWeightBits) - 1ull) : 0ull;
       sum += w[i];
     }
-    before = block_prefix(sum, total);
+    before = block_prefix(sum, sh.scan, total);
     const unsigned long long target = target_of(u, total);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (target >= before && target < before + w[i]) sh.chosen = (int)(sh.list[threadIdx.x * kEach + i] >> (kWeightBits + 1));
+    for (int i = 0; i < kListedEach; ++i) {
+      if (target >= before && target < before + w[i]) sh.found_id = (int)(sh.list[threadIdx.x * kListedEach + i] >> (kWeightBits + 1));
       before += w[i];
     }
     __syncthreads();
-    return sh.chosen;
+    return sh.found_id;
   }
-  static __device__ unsigned long long target_of(float u, unsigned long long total) {
+  __device__ static unsigned long long target_of(float u, unsigned long long total) {
     const unsigned long long target = u > 0.0f ? (unsigned long long)((double)fminf(u, 1.0f) * (double)total) : 0ull;
     return target >= total ? total - 1ull : target;
   }
 
-  // The shortest prefix of the order that brings `wanted`, or `share` of all that `within` holds, in number of tokens or in weight.
-  __device__ Border find(const Border& within, unsigned long long wanted, bool weights, float share) {
+  // --- where the list does not do ---------------------------------------------------------------
+  __device__ __forceinline__ void add_to_bin(int bin, unsigned long long v) {
+    if (v == 0ull) return;
+    const unsigned part = (unsigned)v, before = atomicAdd(&sh.low[bin], part);
+    const unsigned rest = (unsigned)(v >> 32) + (before + part < before ? 1u : 0u);
+    if (rest != 0u) atomicAdd(&sh.high[bin], rest);
+  }
+  // The shortest prefix of the order that brings `wanted` tokens, or `share` of the weight of all that `within` holds.
+  __device__ __forceinline__ Border find(const Border& within, unsigned long long wanted, bool weights, float share) {
     unsigned from = 0u, to = 0xffffffffu;   // keys among which the border lies (from level 1 on)
     int shift = 0;
+#pragma unroll 1
     for (int level = 0;; ++level) {
-      auto bin = [&](float l, unsigned key) { return level == 0 ? bin_of(l) : (int)((to - key) >> shift); };
+      auto bin = [&](float l, unsigned key) { return level == 0 ? bin_below(m, l) : (int)((to - key) >> shift); };
       auto counts = [&](unsigned key, int id) { return within.holds(key, id) && (level == 0 || (key >= from && key <= to)); };
-      clear_bins();
+      for (int i = threadIdx.x; i < kBins; i += kFilterThreads) sh.low[i] = sh.high[i] = 0u;
       __syncthreads();
       for (int i = threadIdx.x; i < count; i += kFilterThreads) {
         const float l = sh.tokens[i];
@@ -406,26 +469,35 @@ class RowFilter {
         if (counts(key, first_id + i)) add_to_bin(bin(l, key), weights ? weight(l) : 1ull);
       }
       sync();
-      if (rank == 0) {
-        unsigned long long upto[kBins / kFilterThreads], all;
-        scan_bins(upto, all);
-        const unsigned long long above = level == 0 ? 0ull : sh.above;
+      if (rank == 0) {   // what lies in the cluster's bins, those of this thread and those before
+        unsigned long long of_bin[kBinsEach], sum = 0ull, all;
+#pragma unroll
+        for (int i = 0; i < kBinsEach; ++i) {
+          of_bin[i] = 0ull;
+          for (int c = 0; c < ctas; ++c) {
+            const unsigned* low = (ctas > 1 ? cluster.map_shared_rank(sh.low, c) : sh.low) + threadIdx.x * kBinsEach + i;
+            of_bin[i] += ((unsigned long long)low[kBins] << 32) + low[0];   // (the upper words lie behind the lower ones)
+          }
+          sum += of_bin[i];
+        }
+        unsigned long long before = block_prefix(sum, sh.scan, all);
         if (level == 0 && weights) wanted = max(1ull, min(all, (unsigned long long)ceil((double)share * (double)all)));
+        before += level == 0 ? 0ull : sh.above;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kBins / kFilterThreads; ++i) {
-          const int here = threadIdx.x * (kBins / kFilterThreads) + i;
-          const unsigned long long before = i > 0 ? upto[i - 1] : upto[0] - bin_total(here);
-          if (above + before < wanted && above + upto[i] >= wanted) {
-            sh.bin = here;
-            sh.above = above + before;
-            sh.total = wanted;
+        for (int i = 0; i < kBinsEach; ++i) {
+          if (before < wanted && before + of_bin[i] >= wanted) {
+            sh.bin = threadIdx.x * kBinsEach + i;
+            sh.above = before;
+            sh.wanted = wanted;
           }
+          before += of_bin[i];
         }
+        if (threadIdx.x == 0) sh.listed = 0;
       }
       sync();
       const int border_bin = *at_first(&sh.bin);
-      wanted = *at_first(&sh.total);
+      wanted = *at_first(&sh.wanted);
       unsigned lowest = 0xffffffffu, highest = 0u;
       for (int i = threadIdx.x; i - (int)threadIdx.x < count; i += kFilterThreads) {
         const float l = i < count ? sh.tokens[i] : 0.0f;
@@ -434,35 +506,41 @@ class RowFilter {
         if (in_bin) lowest = min(lowest, key), highest = max(highest, key);
         put(in_bin, l, first_id + i);
       }
-      sync();
+      lowest = __reduce_min_sync(0xffffffffu, lowest);
+      highest = __reduce_max_sync(0xffffffffu, highest);
+      if (lane == 0) sh.scan[warp] = ((unsigned long long)highest << 32) | lowest;
+      __syncthreads();
+      for (int w = 0; w < kFilterWarps; ++w) lowest = min(lowest, (unsigned)sh.scan[w]), highest = max(highest, (unsigned)(sh.scan[w] >> 32));
+      const unsigned long long* all = gather(lowest, highest);
       if (*at_first(&sh.listed) <= kListed) {
         if (rank == 0) border_of_list(wanted, weights);
         sync();
         return Border{*at_first(&sh.found_key), *at_first(&sh.found_id)};
       }
-      to = (unsigned)cluster_max(highest);
-      from = ~(unsigned)cluster_max((unsigned)~lowest);
+      from = 0xffffffffu, to = 0u;
+      for (int c = 0; c < ctas; ++c) from = min(from, (unsigned)all[c]), to = max(to, (unsigned)all[8 + c]);
       if (from == to) return border_of_equals(within, to, wanted, weights);
       shift = max(0, 32 - __clz(to - from) - kBinBits);
+      sync();   // (all have read the list's length before the next level clears it)
     }
   }
   // Where on the first CTA's list (the border's run) the border lies.
-  __device__ void border_of_list(unsigned long long wanted, bool weights) {
-    constexpr int kEach = kListed / kFilterThreads;
+  __device__ __forceinline__ void border_of_list(unsigned long long wanted, bool weights) {
     const int listed = sh.listed;
-    sort(listed, true);
-    unsigned long long w[kEach], sum = 0ull, all;
+    __syncthreads();
+    sort_list(sh.list, listed, true);
+    unsigned long long w[kListedEach], sum = 0ull, all;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = threadIdx.x * kEach + i;
+    for (int i = 0; i < kListedEach; ++i) {
+      const int at = threadIdx.x * kListedEach + i;
       w[i] = at >= listed ? 0ull : weights ? weight(key_logit((unsigned)(sh.list[at] >> 32))) : 1ull;
       sum += w[i];
     }
-    unsigned long long before = sh.above + block_prefix(sum, all);
+    unsigned long long before = sh.above + block_prefix(sum, sh.scan, all);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = 0; i < kListedEach; ++i) {
       if (before < wanted && before + w[i] >= wanted) {
-        const unsigned long long token = sh.list[threadIdx.x * kEach + i];
+        const unsigned long long token = sh.list[threadIdx.x * kListedEach + i];
         sh.found_key = (unsigned)(token >> 32);
         sh.found_id = (int)~(unsigned)token;
       }
@@ -470,20 +548,18 @@ class RowFilter {
     }
   }
   // The border among more tokens of one key than the list holds: so many of them, in order of ids, as are still wanted.
-  __device__ Border border_of_equals(const Border& within, unsigned key, unsigned long long wanted, bool weights) {
+  __device__ __forceinline__ Border border_of_equals(const Border& within, unsigned key, unsigned long long wanted, bool weights) {
     const unsigned long long each = weights ? weight(key_logit(key)) : 1ull, above = *at_first(&sh.above);
     const unsigned long long number = (wanted - above + each - 1ull) / each;   // (a border in weight lies where there is some)
     const int segment = (count + kFilterWarps - 1) / kFilterWarps, begin = min(count, warp * segment), end = min(count, begin + segment);
     unsigned mine = 0u;
     for (int i0 = begin; i0 < end; i0 += 32) {
       const int i = i0 + lane;
-      const bool equal = i < end && logit_key(sh.tokens[i]) == key && within.holds(key, first_id + i);
-      mine += __popc(__ballot_sync(0xffffffffu, equal));
+      mine += __popc(__ballot_sync(0xffffffffu, i < end && logit_key(sh.tokens[i]) == key && within.holds(key, first_id + i)));
     }
-    unsigned long long before, all;
-    before = block_prefix(lane == 0 ? (unsigned long long)mine : 0ull, all);
+    unsigned long long all, before = block_prefix(lane == 0 ? (unsigned long long)mine : 0ull, sh.scan, all);
     before = __shfl_sync(0xffffffffu, before, 0);
-    const unsigned long long* of_cta = gather(all);
+    const unsigned long long* of_cta = gather(all, 0ull);
     for (int c = 0; c < rank; ++c) before += of_cta[c];
     if (before < number && before + mine >= number) {
       unsigned left = (unsigned)(number - before);
@@ -501,9 +577,8 @@ class RowFilter {
     sync();
     return Border{key, *at_first(&sh.found_id)};
   }
-
-  // The token that the number falls on among the kept ones, in order of ids; in the first CTA.
-  __device__ int draw(const Border& kept, float u) {
+  // The token that the number falls on among the kept ones, in order of ids.
+  __device__ __forceinline__ int draw(const Border& kept, float u) {
     const int segment = (count + kFilterWarps - 1) / kFilterWarps, begin = min(count, warp * segment), end = min(count, begin + segment);
     auto kept_weight = [&](int i) {
       const float l = sh.tokens[i];
@@ -514,10 +589,9 @@ class RowFilter {
     unsigned long long mine = 0ull;
     for (int i = begin + lane; i < end; i += 32) mine += kept_weight(i);
     mine = warp_sum_u64(mine);
-    unsigned long long all;
-    unsigned long long before = block_prefix(lane == 0 ? mine : 0ull, all);
+    unsigned long long all, before = block_prefix(lane == 0 ? mine : 0ull, sh.scan, all);
     before = __shfl_sync(0xffffffffu, before, 0);
-    const unsigned long long* of_cta = gather(all);
+    const unsigned long long* of_cta = gather(all, 0ull);
     unsigned long long total = 0ull;
     for (int c = 0; c < ctas; ++c) {
       if (c < rank) before += of_cta[c];
@@ -530,40 +604,46 @@ class RowFilter {
         const unsigned long long upto = before + warp_prefix_u64(w, lane);
         const unsigned past = __ballot_sync(0xffffffffu, target < upto);
         if (past != 0u) {
-          if (lane == __ffs(past) - 1) *at_first(&sh.chosen) = first_id + i0 + lane;
+          if (lane == __ffs(past) - 1) *at_first(&sh.found_id) = first_id + i0 + lane;
           break;
         }
         before = __shfl_sync(0xffffffffu, upto, 31);
       }
     }
     sync();
-    return sh.chosen;
+    return sh.found_id;
   }
 };
 
-__global__ void __launch_bounds__(kFilterThreads)
+__global__ void __launch_bounds__(kFilterThreads, 2)
     sample_filtered_kernel(const float* __restrict__ logits, long long row_stride, int all_rows, int vocab, int slice, const int* __restrict__ rows, const float* __restrict__ temperature,
                            const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniforms,
                            int* __restrict__ out) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ FilterShared shared;
-  const int set = blockIdx.x / cooperative_groups::this_cluster().num_blocks();
+  const int ctas = cooperative_groups::this_cluster().num_blocks(), set = blockIdx.x / ctas;
   grid_dependency_wait();
   const int index = rows != nullptr ? rows[set] : set;
   if (index < 0 || index >= all_rows) return;   // (the whole cluster)
+  const float t = temperature[set], p = top_p[set], smallest = min_p[set], u = uniforms[set];
+  const int k = top_k[set];
   if (threadIdx.x == 0) {
     shared.list = reinterpret_cast<unsigned long long*>(dynamic);
-    shared.low = reinterpret_cast<unsigned*>(dynamic + kListed * 8);
+    shared.low = reinterpret_cast<unsigned*>(dynamic);
     shared.high = shared.low + kBins;
-    shared.tokens = reinterpret_cast<float*>(shared.high + kBins);
+    shared.tokens = reinterpret_cast<float*>(dynamic + kListed * 8);
+    shared.listed = 0;
   }
-  if (cooperative_groups::this_cluster().num_blocks() > 1) cooperative_groups::this_cluster().sync();   // (a CTA's shared memory may be written once the CTA runs)
-  else __syncthreads();
+  const int last = min(vocab, ((int)cooperative_groups::this_cluster().block_rank() + 1) * slice);   // the last quad's empty places hold no number
+  if (threadIdx.x < 3) reinterpret_cast<float*>(dynamic + kListed * 8)[max(0, last - (int)cooperative_groups::this_cluster().block_rank() * slice) + threadIdx.x] = __int_as_float(0x7fffffff);
+  __syncthreads();
   RowFilter filter(shared, logits + (size_t)index * row_stride, vocab, slice);
-  filter.load();
-  const int token = filter.choose(temperature[set], top_k[set], top_p[set], min_p[set], uniforms[set]);
-  if (cooperative_groups::this_cluster().block_rank() == 0 && threadIdx.x == 0) out[index] = token;
-  if (cooperative_groups::this_cluster().num_blocks() > 1) cooperative_groups::this_cluster().sync();   // nobody leaves while another reads what it holds
+  filter.arrive();
+  const int token = filter.choose(t, k, p, smallest, u);
+  if (cooperative_groups::this_cluster().block_rank() == 0) {
+    if (threadIdx.x == 0) out[index] = token;
+    if (ctas > 1) cooperative_groups::this_cluster().sync();   // the others leave when they are done; this CTA's memory stays until they have (who has left is not waited for)
+  }
 }
 
 __global__ void uniforms_kernel(const long long* __restrict__ seeds, const long long* __restrict__ counters, float* __restrict__ out, int count) {
@@ -591,9 +671,9 @@ TLIE_EXPORT int tlie_sample_filtered(const float* logits, long long row_stride, 
   int ctas = 1;
   while (ctas < 8 && (vocab > ctas * 16384 || (vocab > ctas * 2048 && (long long)count * ctas * 2 <= 2 * device_sm_count()))) ctas *= 2;
   const int slice = ((vocab + ctas - 1) / ctas + 3) & ~3;
-  const size_t smem = kListed * 8 + kBins * 8 + (size_t)slice * 4;
+  const size_t smem = kListed * 8 + (size_t)(slice + 4) * 4;
   static std::atomic<unsigned long long> devices{0};
-  cudaError_t e = allow_shared_memory(sample_filtered_kernel, kListed * 8 + kBins * 8 + kMostSlice * 4, devices);
+  cudaError_t e = allow_shared_memory(sample_filtered_kernel, kListed * 8 + (kMostSlice + 4) * 4, devices);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)count * ctas);
