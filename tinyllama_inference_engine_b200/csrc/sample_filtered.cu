@@ -12,15 +12,13 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
-#include "shared_memory_limit.cuh"
 
 namespace tlie {
 
 constexpr int kFilterThreads = 512, kFilterWarps = kFilterThreads / 32;
 constexpr int kBinBits = 10, kBins = 1 << kBinBits, kBinsEach = kBins / kFilterThreads;
-constexpr int kListed = 2048, kListedEach = kListed / kFilterThreads;   // tokens that the first CTA of a cluster can sort
-constexpr int kMostSlice = 49152;                        // tokens of a CTA: 192 KB
-constexpr int kFilterMaxVocab = 8 * kMostSlice;          // (weights of 2^44 and less, fewer than 2^19 of them: sums fit 64 bits, a token's id and weight one number)
+constexpr int kListed = kFilterThreads;    // tokens of the list, one per thread
+constexpr int kFilterMaxVocab = 1 << 19;   // (so many weights of 2^44 and less: sums fit 64 bits, a token's id and weight one number)
 constexpr int kWeightBits = 44;
 
 // Logits as unsigned numbers of the same order: equal floats are equal numbers (-0 counts as 0), NaN is below everything.
@@ -30,41 +28,34 @@ __device__ __forceinline__ unsigned logit_key(float l) {
   return bits < 0 ? ~(unsigned)bits : (unsigned)bits | 0x80000000u;
 }
 
-// log2(e) / T in two floats.  Temperatures below 1e-30 count as 1e-30: to differ there two logits would have to lie 1e-29 apart.
+// What a row's weights are made with: y = l c - m c in 64 bits is log2 of one, with c = log2(e) / T.  Temperatures outside 1e-30 to 1e30 count as the nearer of these: to
+// differ below two logits would have to lie 1e-29 apart, and above nothing differs.
 struct Scale {
-  float high, low;
+  double c, mc;
 };
-__device__ __forceinline__ Scale weight_scale(float temperature) {
-  const double c = 1.4426950408889634074 / (double)fmaxf(temperature, 1e-30f);
-  Scale s;
-  s.high = (float)c;
-  s.low = (float)(c - (double)s.high);
-  return s;
+__device__ __forceinline__ Scale weight_scale(float temperature, float m) {
+  const double c = 1.4426950408889634074 / (double)fminf(fmaxf(temperature, 1e-30f), 1e30f);
+  return Scale{c, (double)m * c};
 }
 
-// exp((l - m) / T) in units of 2^-44.  The exponent's difference and product are kept in two floats (what rounding takes off one is in the other), so that
-// its error does not grow with the distance from m.  2^f on [-1/2, 1/2] is a polynomial of degree 6 (least maximum of the relative error, 2e-9).
+// exp((l - m) / T) in units of 2^-44.  y with 23 bits behind the point stands in the lower word of y + 1.5 * 2^29, its whole part (rounded down) and the rest f, put behind a
+// 1, are what a float of 1 + f is made of.  2^(f - 1/2) sqrt(2) is a polynomial of degree 6 in f - 1/2 (least maximum of the relative error, 2e-8 with its coefficients rounded).
 __device__ __forceinline__ unsigned long long token_weight(float l, float m, Scale c) {
-  if (l == m) return 1ull << kWeightBits;
-  const float s = l - m, back = s - l;
-  const float e = (l - (s - back)) - (m + back);
-  const float high = s * c.high;
-  if (!(high >= -46.0f)) return 0ull;   // (NaN and infinities too)
-  const float low = fmaf(s, c.high, -high) + fmaf(s, c.low, e * c.high);
-  const float rounded = high + 12582912.0f;   // 1.5 * 2^23: the whole number nearest to it in the lower bits
-  const int n = __float_as_int(rounded) - 0x4B400000;
-  const float f = (high - (rounded - 12582912.0f)) + low;
-  float p = 1.5353153867181391e-4f;
-  p = fmaf(p, f, 1.339913229458034e-3f);
-  p = fmaf(p, f, 9.618439711630344e-3f);
-  p = fmaf(p, f, 5.550331994891167e-2f);
-  p = fmaf(p, f, 2.4022647738456726e-1f);
-  p = fmaf(p, f, 6.931471824645996e-1f);
-  p = fmaf(p, f, 1.0f);
+  const double y = fma((double)l, c.c, -c.mc);
+  const unsigned size = (unsigned)__double2hiint(y) ^ 0x80000000u;   // below that of 46 for -46 < y < 0; NaN, infinities and y >= 0 (the maximum itself) are above
+  const int fixed = __double2loint(y + 805306368.0);
+  const float f = __int_as_float((fixed & 0x7fffff) | 0x3f800000) - 1.5f;
+  float p = 2.170223742723465e-4f;
+  p = fmaf(p, f, 1.8950358498841524e-3f);
+  p = fmaf(p, f, 1.3602597638964653e-2f);
+  p = fmaf(p, f, 7.849350571632385e-2f);
+  p = fmaf(p, f, 3.397315442562103e-1f);
+  p = fmaf(p, f, 9.802581667900085e-1f);
+  p = fmaf(p, f, 1.4142135381698608f);
   const unsigned bits = __float_as_uint(p);
-  const int down = 127 - (int)(bits >> 23) - n;   // 0 to 47: how far below 1 the leading bit lies
-  const unsigned long long mantissa = (unsigned long long)((bits & 0x7fffffu) | 0x800000u) << (kWeightBits - 23);
-  return mantissa >> down;
+  const int down = 127 - (int)(bits >> 23) - (fixed >> 23);   // 0 to 47: how far below 1 the leading bit lies
+  const unsigned long long w = ((unsigned long long)((bits & 0x7fffffu) | 0x800000u) << (kWeightBits - 23)) >> down;
+  return l == m ? 1ull << kWeightBits : size < 0x40470000u ? w : 0ull;
 }
 
 // The last token of a prefix of the order: tokens with a larger key, and those of this key up to this id, belong to it.
@@ -74,7 +65,7 @@ struct Border {
   __device__ bool holds(unsigned k, int i) const { return k > key || (k == key && i <= id); }
 };
 
-// A row's tokens lie in the shared memory of a cluster of CTAs, consecutive ones in each; what follows its first maximum is mostly done by the first CTA on a short
+// A row belongs to a cluster of CTAs, consecutive tokens to each, which read them once for the maximum and again, from the caches, for what follows; that is mostly done by the first CTA on a short
 // list of the order's first tokens.  As many threads' maxima as are asked for bound the list from below (so many tokens at least are not below the least of them), and the highest
 // of the CTAs' bounds holds for all.  With top_k so many tokens are asked for and all others are out of it; with top_p alone some hundred, and the exact weight of all
 // tokens tells whether they suffice; min_p alone says itself which tokens it leaves.  Bound by the reading of the logits then, or, with top_p alone, by the 35 instructions of a
@@ -84,9 +75,13 @@ struct Border {
 // of exact weights, and from the tokens of the run that it falls in, which the first CTA sorts.  Where those are too many (equal logits, or very close ones) the run is
 // cut by the bits of the logits, and equal ones by id.
 struct FilterShared {
-  float* tokens;                  // this CTA's
-  unsigned *low, *high;           // a histogram's numbers, 64 bits in two words: an atomic of 64 bits on shared memory is a loop
-  unsigned long long* list;       // (over the histogram: one is done with before the other begins)
+  union {                         // (one is done with before the other begins)
+    struct {
+      unsigned low[kBins], high[kBins];   // a histogram's numbers, 64 bits in two words: an atomic of 64 bits on shared memory is a loop
+    };
+    unsigned long long list[kListed];
+  };
+  unsigned long long exchange[2][kFilterThreads];
   unsigned long long scan[kFilterWarps];
   unsigned long long gather[2][2][8];   // two numbers per CTA
   unsigned long long above;       // the first CTA's are the cluster's, as are:
@@ -127,23 +122,28 @@ __device__ __noinline__ unsigned long long block_prefix(unsigned long long v, un
   all = sum;
   return before + upto - v;
 }
-// Sorts n numbers of a list, falling or rising, by the CTA's threads.
-__device__ __noinline__ void sort_list(unsigned long long* list, int n, bool falling) {
-  int size = 2;
+// The first n threads' numbers in falling order, one per thread (n and more: whatever is there, below all others): exchanges with the thread 2^k further, by shuffles inside a warp.
+__device__ __noinline__ unsigned long long sort_falling(unsigned long long v, int n, unsigned long long (&exchange)[2][kFilterThreads]) {
+  int size = 32, turn = 0;
   while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += kFilterThreads) list[i] = falling ? 0ull : ~0ull;
-  __syncthreads();
+  if ((int)threadIdx.x >= n) v = 0ull;
+#pragma unroll 1
   for (int run = 2; run <= size; run *= 2)
+#pragma unroll 1
     for (int reach = run / 2; reach > 0; reach /= 2) {
-      for (int i = threadIdx.x; i < size / 2; i += kFilterThreads) {
-        const int a = 2 * i - (i & (reach - 1)), b = a + reach;
-        const unsigned long long x = list[a], y = list[b];
-        if ((x < y) == (((a & run) == 0) == falling)) list[a] = y, list[b] = x;
+      unsigned long long other = 0ull;
+      if (reach < 32) {
+        if ((int)threadIdx.x < size) other = __shfl_xor_sync(0xffffffffu, v, reach);
+      } else {
+        exchange[turn][threadIdx.x] = v;
+        __syncthreads();
+        other = exchange[turn][threadIdx.x ^ reach];
+        turn ^= 1;
       }
-      if (reach > 32 || size > 64) __syncthreads();
-      else __syncwarp();   // (one warp has it all)
+      if (((threadIdx.x & reach) == 0) == ((threadIdx.x & run) == 0)) v = max(v, other);   // (a last run of all is a falling one)
+      else v = min(v, other);
     }
-  __syncthreads();
+  return v;
 }
 __device__ __forceinline__ float key_logit(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
@@ -151,8 +151,9 @@ __device__ __forceinline__ float key_logit(unsigned key) { return __uint_as_floa
 class RowFilter {
  public:
   __device__ RowFilter(FilterShared& shared, const float* row, int vocab, int slice)
-      : sh(shared), cluster(cooperative_groups::this_cluster()), row(row), vocab(vocab), ctas(cluster.num_blocks()), rank(cluster.block_rank()),
-        lane(threadIdx.x & 31), warp(threadIdx.x >> 5), first_id(min(vocab, rank * slice)), count(min(vocab, (rank + 1) * slice) - first_id) {}
+      : sh(shared), cluster(cooperative_groups::this_cluster()), vocab(vocab), ctas(cluster.num_blocks()), rank(cluster.block_rank()),
+        lane(threadIdx.x & 31), warp(threadIdx.x >> 5), first_id(min(vocab, rank * slice)), count(min(vocab, (rank + 1) * slice) - first_id), tokens(row + first_id),
+        head(min(count, (int)((4 - (reinterpret_cast<uintptr_t>(row + first_id) >> 2 & 3)) & 3))), quads((count - head) >> 2) {}
 
   // The row's token, in the first CTA.
   __device__ int choose(float temperature, int top_k, float top_p, float min_p, float u) {
@@ -174,7 +175,7 @@ class RowFilter {
     if (!any_token(key)) return 0;                        // a row of NaN
     if (first_only || !(m > -INFINITY)) return first_of_order();
 
-    scale = weight_scale(temperature);
+    scale = weight_scale(temperature, m);
     floor_weight = min_p > 0.0f ? (unsigned long long)ceil((double)min_p * (double)(1ull << kWeightBits)) : 0ull;
     const bool by_floor = !by_number && !by_weight && floor_weight > 0ull;
     if (by_floor) bound = m + temperature * (logf(min_p) * 1.0001f - 0.001f);   // (a little low: the list is longer than what stays of it)
@@ -211,11 +212,12 @@ class RowFilter {
   }
 
  private:
-  static constexpr int kGuess = 256;
+  static constexpr int kGuess = 192;
   FilterShared& sh;
   cooperative_groups::cluster_group cluster;
-  const float* row;
   const int vocab, ctas, rank, lane, warp, first_id, count;
+  const float* tokens;     // this CTA's: `head` of them in front of the first 16 bytes, `quads` times four, and what is left
+  const int head, quads;
   float m, thread_max;
   Scale scale;
   unsigned long long floor_weight;
@@ -237,47 +239,33 @@ class RowFilter {
   // The run below `top` that a logit falls in: monotone, and the last one is for all that lies further below.
   __device__ static int bin_below(float top, float l) { return l == top ? 0 : (int)fminf((top - l) * 32.0f, (float)(kBins - 1)); }
 
-  // Brings the tokens into shared memory; this thread's largest (NaN is none).
+  // A token of this thread's among those that do not stand in whole quads, -1 if it has none.
+  __device__ __forceinline__ int edge_token() const {
+    const int t = threadIdx.x, tail = count - head - 4 * quads;
+    return t < head ? t : t - head < tail ? count - tail + t - head : -1;
+  }
+  __device__ __forceinline__ float4 quad(int q) const { return reinterpret_cast<const float4*>(tokens + head)[q]; }
+
+  // This thread's largest token (NaN is none).
   __device__ __forceinline__ void load() {
     float best = -INFINITY;
     bool some = false;   // a token that is not NaN
-    const float* from = row + first_id;
     constexpr int kFlight = 8;
-    if ((reinterpret_cast<uintptr_t>(from) & 15) == 0) {
-      const int quads = count >> 2;
-      for (int q0 = threadIdx.x; q0 < quads; q0 += kFlight * kFilterThreads) {
-        float4 v[kFlight];
+    for (int q0 = threadIdx.x; q0 < quads; q0 += kFlight * kFilterThreads) {
+      const float nan = __int_as_float(0x7fffffff);
+      float4 v[kFlight];
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u)
-          if (q0 + u * kFilterThreads < quads) v[u] = reinterpret_cast<const float4*>(from)[q0 + u * kFilterThreads];
+      for (int u = 0; u < kFlight; ++u) v[u] = q0 + u * kFilterThreads < quads ? quad(q0 + u * kFilterThreads) : make_float4(nan, nan, nan, nan);
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u) {
-          if (q0 + u * kFilterThreads >= quads) break;
-          reinterpret_cast<float4*>(sh.tokens)[q0 + u * kFilterThreads] = v[u];
-          best = fmaxf(fmaxf(best, fmaxf(v[u].x, v[u].y)), fmaxf(v[u].z, v[u].w));
-          some |= v[u].x == v[u].x || v[u].y == v[u].y || v[u].z == v[u].z || v[u].w == v[u].w;
-        }
+      for (int u = 0; u < kFlight; ++u) {
+        best = fmaxf(fmaxf(best, fmaxf(v[u].x, v[u].y)), fmaxf(v[u].z, v[u].w));
+        some |= v[u].x == v[u].x || v[u].y == v[u].y || v[u].z == v[u].z || v[u].w == v[u].w;
       }
-      const int i = 4 * quads + threadIdx.x;
-      if (i < count) {
-        sh.tokens[i] = from[i];
-        best = fmaxf(best, sh.tokens[i]);
-        some |= sh.tokens[i] == sh.tokens[i];
-      }
-    } else {
-      for (int i0 = threadIdx.x; i0 < count; i0 += kFlight * kFilterThreads) {
-        float v[kFlight];
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u)
-          if (i0 + u * kFilterThreads < count) v[u] = from[i0 + u * kFilterThreads];
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u) {
-          if (i0 + u * kFilterThreads >= count) break;
-          sh.tokens[i0 + u * kFilterThreads] = v[u];
-          best = fmaxf(best, v[u]);
-          some |= v[u] == v[u];
-        }
-      }
+    }
+    const int i = edge_token();
+    if (i >= 0) {
+      best = fmaxf(best, tokens[i]);
+      some |= tokens[i] == tokens[i];
     }
     thread_max = some ? best : __int_as_float(0x7fffffff);
   }
@@ -344,7 +332,7 @@ class RowFilter {
   __device__ __forceinline__ int first_of_order() {
     int id = 0x7fffffff;
     for (int i = threadIdx.x; i < count; i += kFilterThreads)
-      if (sh.tokens[i] == m) {
+      if (tokens[i] == m) {
         id = first_id + i;
         break;
       }
@@ -367,77 +355,54 @@ class RowFilter {
     at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
     if (wanted && at < kListed) at_first(sh.list)[at] = ((unsigned long long)logit_key(l) << 32) | (unsigned)~id;
   }
-  // Lists the tokens that are not below the bound; with `weights` their weight and that of all others, this thread's share of it.
+  // Lists the tokens that are not below the bound; with `weights` the weight of all tokens, this thread's share of it.
   __device__ __forceinline__ void list_from(float bound, bool weights, unsigned long long& mine) {
-    if (weights) {
-      for (int i = threadIdx.x; i - (int)threadIdx.x < count; i += kFilterThreads) {
-        const float l = i < count ? sh.tokens[i] : __int_as_float(0x7fffffff);
-        mine += weight(l);
-        put(l >= bound, l, first_id + i);
+    const float nan = __int_as_float(0x7fffffff);
+    constexpr int kFlight = 4;
+    for (int q0 = threadIdx.x; q0 - (int)threadIdx.x < quads; q0 += kFlight * kFilterThreads) {
+      float4 v[kFlight];
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) v[u] = q0 + u * kFilterThreads < quads ? quad(q0 + u * kFilterThreads) : make_float4(nan, nan, nan, nan);
+#pragma unroll 1
+      for (int u = 0; u < kFlight; ++u) {
+        if (weights) mine += (weight(v[0].x) + weight(v[0].y)) + (weight(v[0].z) + weight(v[0].w));
+        if (__any_sync(0xffffffffu, fmaxf(fmaxf(v[0].x, v[0].y), fmaxf(v[0].z, v[0].w)) >= bound)) {
+          const int id = first_id + head + 4 * (q0 + u * kFilterThreads);
+#pragma unroll 1
+          for (int e = 0; e < 4; ++e) {
+            put(v[0].x >= bound, v[0].x, id + e);
+            v[0].x = v[0].y, v[0].y = v[0].z, v[0].z = v[0].w;
+          }
+        }
+#pragma unroll
+        for (int other = 0; other + 1 < kFlight; ++other) v[other] = v[other + 1];
       }
-      return;
     }
-    const int quads = (count + 3) >> 2;   // (tokens behind the last one are NaN)
-    for (int q = threadIdx.x; q - (int)threadIdx.x < quads; q += kFilterThreads) {
-      const float nan = __int_as_float(0x7fffffff);
-      const float4 v = q < quads ? reinterpret_cast<const float4*>(sh.tokens)[q] : make_float4(nan, nan, nan, nan);
-      if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) continue;
-      put(v.x >= bound, v.x, first_id + 4 * q);
-      put(v.y >= bound, v.y, first_id + 4 * q + 1);
-      put(v.z >= bound, v.z, first_id + 4 * q + 2);
-      put(v.w >= bound, v.w, first_id + 4 * q + 3);
-    }
+    const int i = edge_token();
+    const float l = i >= 0 ? tokens[i] : nan;
+    if (weights) mine += weight(l);
+    put(l >= bound, l, first_id + i);
   }
 
   // The row's token if its first top_k tokens (or all that min_p leaves, or, where `total` is the weight of all tokens, all that top_p leaves) are on the list; by the first CTA.  -1: the
   // list's weight does not reach top_p of `total`.
   __device__ __forceinline__ int choose_from_list(int top_k, float top_p, unsigned long long total, float u) {
-    const int listed = sh.listed;
-    __syncthreads();
-    sort_list(sh.list, listed, true);
-    const int number = min(top_k, listed);
-    // consecutive tokens of the order per thread
-    unsigned long long w[kListedEach], sum = 0ull, on_list;
-#pragma unroll
-    for (int i = 0; i < kListedEach; ++i) {
-      const int at = threadIdx.x * kListedEach + i;
-      w[i] = at < number ? weight(key_logit((unsigned)(sh.list[at] >> 32))) : 0ull;
-      sum += w[i];
-    }
-    unsigned long long before = block_prefix(sum, sh.scan, on_list);
-    const unsigned long long of = total != 0ull ? total : on_list;
+    const int number = min(top_k, sh.listed), mine = threadIdx.x;
+    const unsigned long long token = sort_falling(sh.list[mine], sh.listed, sh.exchange);
+    const unsigned long long w = mine < number ? weight(key_logit((unsigned)(token >> 32))) : 0ull;
+    unsigned long long all, of_kept;
+    const unsigned long long before = block_prefix(w, sh.scan, all);
+    const unsigned long long of = total != 0ull ? total : all;
     const unsigned long long wanted = top_p < 1.0f ? max(1ull, min(of, (unsigned long long)ceil((double)top_p * (double)of))) : ~0ull;
-    if (total != 0ull && on_list < wanted) return -1;
-    unsigned long long here = 0ull, kept;   // of this thread's tokens: those in front of which top_p has not been reached, that are heavy enough (both stand in front of the others)
-#pragma unroll
-    for (int i = 0; i < kListedEach; ++i) {
-      here += threadIdx.x * kListedEach + i < number && before < wanted && w[i] >= floor_weight;
-      before += w[i];
-    }
-    block_prefix(here, sh.scan, kept);
-    const int many = max(1, (int)kept);
-    // in order of ids, the weight behind the id
-#pragma unroll
-    for (int i = 0; i < kListedEach; ++i) {
-      const int at = threadIdx.x * kListedEach + i;
-      if (at < many) sh.list[at] = ((unsigned long long)~(unsigned)sh.list[at] << (kWeightBits + 1)) | w[i];
-    }
-    __syncthreads();
-    sort_list(sh.list, many, false);
-    sum = 0ull;
-#pragma unroll
-    for (int i = 0; i < kListedEach; ++i) {
-      const int at = threadIdx.x * kListedEach + i;
-      w[i] = at < many ? sh.list[at] & ((2ull << kWeightBits) - 1ull) : 0ull;
-      sum += w[i];
-    }
-    before = block_prefix(sum, sh.scan, total);
-    const unsigned long long target = target_of(u, total);
-#pragma unroll
-    for (int i = 0; i < kListedEach; ++i) {
-      if (target >= before && target < before + w[i]) sh.found_id = (int)(sh.list[threadIdx.x * kListedEach + i] >> (kWeightBits + 1));
-      before += w[i];
-    }
+    if (total != 0ull && all < wanted) return -1;
+    // kept: in front of which top_p has not been reached, heavy enough; the first always
+    const bool kept = mine == 0 || (mine < number && before < wanted && w >= floor_weight);
+    const int many = __syncthreads_count(kept);
+    // in order of ids (the lower one's complement is the larger), the weight behind the id
+    const unsigned long long by_id = sort_falling(((unsigned long long)((unsigned)token & (kFilterMaxVocab - 1)) << (kWeightBits + 1)) | w, many, sh.exchange);
+    const unsigned long long kept_weight = mine < many ? by_id & ((2ull << kWeightBits) - 1ull) : 0ull;
+    const unsigned long long start = block_prefix(kept_weight, sh.scan, of_kept), target = target_of(u, of_kept);
+    if (target >= start && target < start + kept_weight) sh.found_id = (int)(~(unsigned)(by_id >> (kWeightBits + 1)) & (kFilterMaxVocab - 1));
     __syncthreads();
     return sh.found_id;
   }
@@ -447,6 +412,22 @@ class RowFilter {
   }
 
   // --- where the list does not do ---------------------------------------------------------------
+  // f(logit, id) for all tokens, a warp's threads together; where there is no token NaN and an id that is none.
+  template <typename F>
+  __device__ __forceinline__ void for_tokens(F f) {
+    const float nan = __int_as_float(0x7fffffff);
+    for (int q0 = threadIdx.x; q0 - (int)threadIdx.x < quads; q0 += kFilterThreads) {
+      float4 v = q0 < quads ? quad(q0) : make_float4(nan, nan, nan, nan);
+      const int id = q0 < quads ? first_id + head + 4 * q0 : -8;
+#pragma unroll 1
+      for (int e = 0; e < 4; ++e) {
+        f(v.x, id + e);
+        v.x = v.y, v.y = v.z, v.z = v.w;
+      }
+    }
+    const int i = edge_token();
+    f(i >= 0 ? tokens[i] : nan, i >= 0 ? first_id + i : -1);
+  }
   __device__ __forceinline__ void add_to_bin(int bin, unsigned long long v) {
     if (v == 0ull) return;
     const unsigned part = (unsigned)v, before = atomicAdd(&sh.low[bin], part);
@@ -459,15 +440,19 @@ class RowFilter {
     int shift = 0;
 #pragma unroll 1
     for (int level = 0;; ++level) {
-      auto bin = [&](float l, unsigned key) { return level == 0 ? bin_below(m, l) : (int)((to - key) >> shift); };
-      auto counts = [&](unsigned key, int id) { return within.holds(key, id) && (level == 0 || (key >= from && key <= to)); };
+      // the run of a token at this level, -1 if it does not count
+      auto run_of = [&](float l, int id) {
+        const unsigned key = logit_key(l);
+        if (id < 0 || !within.holds(key, id)) return -1;
+        if (level == 0) return bin_below(m, l);
+        return key >= from && key <= to ? (int)((to - key) >> shift) : -1;
+      };
       for (int i = threadIdx.x; i < kBins; i += kFilterThreads) sh.low[i] = sh.high[i] = 0u;
       __syncthreads();
-      for (int i = threadIdx.x; i < count; i += kFilterThreads) {
-        const float l = sh.tokens[i];
-        const unsigned key = logit_key(l);
-        if (counts(key, first_id + i)) add_to_bin(bin(l, key), weights ? weight(l) : 1ull);
-      }
+      for_tokens([&](float l, int id) {
+        const int run = run_of(l, id);
+        if (run >= 0) add_to_bin(run, weights ? weight(l) : 1ull);
+      });
       sync();
       if (rank == 0) {   // what lies in the cluster's bins, those of this thread and those before
         unsigned long long of_bin[kBinsEach], sum = 0ull, all;
@@ -496,16 +481,14 @@ class RowFilter {
         if (threadIdx.x == 0) sh.listed = 0;
       }
       sync();
-      const int border_bin = *at_first(&sh.bin);
+      const int border_run = *at_first(&sh.bin);
       wanted = *at_first(&sh.wanted);
       unsigned lowest = 0xffffffffu, highest = 0u;
-      for (int i = threadIdx.x; i - (int)threadIdx.x < count; i += kFilterThreads) {
-        const float l = i < count ? sh.tokens[i] : 0.0f;
-        const unsigned key = logit_key(l);
-        const bool in_bin = i < count && counts(key, first_id + i) && bin(l, key) == border_bin;
-        if (in_bin) lowest = min(lowest, key), highest = max(highest, key);
-        put(in_bin, l, first_id + i);
-      }
+      for_tokens([&](float l, int id) {
+        const bool in_run = run_of(l, id) == border_run;
+        if (in_run) lowest = min(lowest, logit_key(l)), highest = max(highest, logit_key(l));
+        put(in_run, l, id);
+      });
       lowest = __reduce_min_sync(0xffffffffu, lowest);
       highest = __reduce_max_sync(0xffffffffu, highest);
       if (lane == 0) sh.scan[warp] = ((unsigned long long)highest << 32) | lowest;
@@ -527,24 +510,13 @@ class RowFilter {
   // Where on the first CTA's list (the border's run) the border lies.
   __device__ __forceinline__ void border_of_list(unsigned long long wanted, bool weights) {
     const int listed = sh.listed;
-    __syncthreads();
-    sort_list(sh.list, listed, true);
-    unsigned long long w[kListedEach], sum = 0ull, all;
-#pragma unroll
-    for (int i = 0; i < kListedEach; ++i) {
-      const int at = threadIdx.x * kListedEach + i;
-      w[i] = at >= listed ? 0ull : weights ? weight(key_logit((unsigned)(sh.list[at] >> 32))) : 1ull;
-      sum += w[i];
-    }
-    unsigned long long before = sh.above + block_prefix(sum, sh.scan, all);
-#pragma unroll
-    for (int i = 0; i < kListedEach; ++i) {
-      if (before < wanted && before + w[i] >= wanted) {
-        const unsigned long long token = sh.list[threadIdx.x * kListedEach + i];
-        sh.found_key = (unsigned)(token >> 32);
-        sh.found_id = (int)~(unsigned)token;
-      }
-      before += w[i];
+    const unsigned long long token = sort_falling(sh.list[threadIdx.x], listed, sh.exchange);
+    const unsigned long long w = (int)threadIdx.x >= listed ? 0ull : weights ? weight(key_logit((unsigned)(token >> 32))) : 1ull;
+    unsigned long long all;
+    const unsigned long long before = sh.above + block_prefix(w, sh.scan, all);
+    if (before < wanted && before + w >= wanted) {
+      sh.found_key = (unsigned)(token >> 32);
+      sh.found_id = (int)~(unsigned)token;
     }
   }
   // The border among more tokens of one key than the list holds: so many of them, in order of ids, as are still wanted.
@@ -555,7 +527,7 @@ class RowFilter {
     unsigned mine = 0u;
     for (int i0 = begin; i0 < end; i0 += 32) {
       const int i = i0 + lane;
-      mine += __popc(__ballot_sync(0xffffffffu, i < end && logit_key(sh.tokens[i]) == key && within.holds(key, first_id + i)));
+      mine += __popc(__ballot_sync(0xffffffffu, i < end && logit_key(tokens[i]) == key && within.holds(key, first_id + i)));
     }
     unsigned long long all, before = block_prefix(lane == 0 ? (unsigned long long)mine : 0ull, sh.scan, all);
     before = __shfl_sync(0xffffffffu, before, 0);
@@ -565,7 +537,7 @@ class RowFilter {
       unsigned left = (unsigned)(number - before);
       for (int i0 = begin; i0 < end; i0 += 32) {
         const int i = i0 + lane;
-        const unsigned who = __ballot_sync(0xffffffffu, i < end && logit_key(sh.tokens[i]) == key && within.holds(key, first_id + i));
+        const unsigned who = __ballot_sync(0xffffffffu, i < end && logit_key(tokens[i]) == key && within.holds(key, first_id + i));
         const unsigned here = __popc(who);
         if (left <= here) {
           if ((who >> lane & 1u) && __popc(who & ((1u << lane) - 1u)) == (int)left - 1) *at_first(&sh.found_id) = first_id + i;
@@ -581,12 +553,13 @@ class RowFilter {
   __device__ __forceinline__ int draw(const Border& kept, float u) {
     const int segment = (count + kFilterWarps - 1) / kFilterWarps, begin = min(count, warp * segment), end = min(count, begin + segment);
     auto kept_weight = [&](int i) {
-      const float l = sh.tokens[i];
+      const float l = tokens[i];
       if (!kept.holds(logit_key(l), first_id + i)) return 0ull;
       const unsigned long long w = weight(l);
       return w >= floor_weight ? w : 0ull;
     };
     unsigned long long mine = 0ull;
+#pragma unroll 4
     for (int i = begin + lane; i < end; i += 32) mine += kept_weight(i);
     mine = warp_sum_u64(mine);
     unsigned long long all, before = block_prefix(lane == 0 ? mine : 0ull, sh.scan, all);
@@ -619,7 +592,6 @@ __global__ void __launch_bounds__(kFilterThreads, 2)
     sample_filtered_kernel(const float* __restrict__ logits, long long row_stride, int all_rows, int vocab, int slice, const int* __restrict__ rows, const float* __restrict__ temperature,
                            const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniforms,
                            int* __restrict__ out) {
-  extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ FilterShared shared;
   const int ctas = cooperative_groups::this_cluster().num_blocks(), set = blockIdx.x / ctas;
   grid_dependency_wait();
@@ -627,15 +599,7 @@ __global__ void __launch_bounds__(kFilterThreads, 2)
   if (index < 0 || index >= all_rows) return;   // (the whole cluster)
   const float t = temperature[set], p = top_p[set], smallest = min_p[set], u = uniforms[set];
   const int k = top_k[set];
-  if (threadIdx.x == 0) {
-    shared.list = reinterpret_cast<unsigned long long*>(dynamic);
-    shared.low = reinterpret_cast<unsigned*>(dynamic);
-    shared.high = shared.low + kBins;
-    shared.tokens = reinterpret_cast<float*>(dynamic + kListed * 8);
-    shared.listed = 0;
-  }
-  const int last = min(vocab, ((int)cooperative_groups::this_cluster().block_rank() + 1) * slice);   // the last quad's empty places hold no number
-  if (threadIdx.x < 3) reinterpret_cast<float*>(dynamic + kListed * 8)[max(0, last - (int)cooperative_groups::this_cluster().block_rank() * slice) + threadIdx.x] = __int_as_float(0x7fffffff);
+  if (threadIdx.x == 0) shared.listed = 0;
   __syncthreads();
   RowFilter filter(shared, logits + (size_t)index * row_stride, vocab, slice);
   filter.arrive();
@@ -667,18 +631,13 @@ TLIE_EXPORT int tlie_sample_filtered(const float* logits, long long row_stride, 
                                      const int* top_k, const float* top_p, const float* min_p, const float* uniforms, int* out, cudaStream_t stream) {
   if (count <= 0) return 0;
   if (vocab <= 0 || vocab > kFilterMaxVocab || row_stride < 0) return (int)cudaErrorInvalidValue;
-  // CTAs of a row's cluster: slices of at most 16,384 tokens (two CTAs' fit an SM, one loads while the other works), and for few rows down to 2,048.
+  // CTAs of a row's cluster: as many as the SMs hold one each of, with at least 2,048 tokens.
   int ctas = 1;
-  while (ctas < 8 && (vocab > ctas * 16384 || (vocab > ctas * 2048 && (long long)count * ctas * 2 <= 2 * device_sm_count()))) ctas *= 2;
+  while (ctas < 8 && vocab > ctas * 2048 && (long long)count * ctas * 2 <= device_sm_count()) ctas *= 2;
   const int slice = ((vocab + ctas - 1) / ctas + 3) & ~3;
-  const size_t smem = kListed * 8 + (size_t)(slice + 4) * 4;
-  static std::atomic<unsigned long long> devices{0};
-  cudaError_t e = allow_shared_memory(sample_filtered_kernel, kListed * 8 + (kMostSlice + 4) * 4, devices);
-  if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)count * ctas);
   config.blockDim = dim3(kFilterThreads);
-  config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeClusterDimension;

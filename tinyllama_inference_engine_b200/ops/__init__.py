@@ -1424,7 +1424,7 @@ def filtered_sampling():
     return load_library("tlie_sample_filtered", SAMPLE_FILTERED_SOURCES)
 
 
-SAMPLE_FILTERED_MAX_VOCAB = 8 * 49152    # what a cluster of eight CTAs holds in shared memory (csrc/sample_filtered.cu)
+SAMPLE_FILTERED_MAX_VOCAB = 1 << 19    # sums of that many weights of 2^44 and less fit 64 bits (csrc/sample_filtered.cu)
 
 
 def sample_filtered(logits, temperature, top_k, top_p, min_p, uniforms, out, rows=None) -> None:
