@@ -81,7 +81,7 @@ struct FilterShared {
     };
     unsigned long long list[kListed];
   };
-  unsigned long long exchange[2][kFilterThreads];
+  unsigned long long exchange[2][kFilterThreads], early[kListed];
   unsigned long long scan[kFilterWarps];
   unsigned long long gather[2][2][8];   // two numbers per CTA
   unsigned long long above;       // the first CTA's are the cluster's, as are:
@@ -124,9 +124,25 @@ __device__ __noinline__ unsigned long long block_prefix(unsigned long long v, un
 }
 // The first n threads' numbers in falling order, one per thread (n and more: whatever is there, below all others): exchanges with the thread 2^k further, by shuffles inside a warp.
 __device__ __noinline__ unsigned long long sort_falling(unsigned long long v, int n, unsigned long long (&exchange)[2][kFilterThreads]) {
+  if (n <= kFilterThreads / 2) {   // few: a number's place is how many are above it, counted by several threads side by side (64 numbers: 600 cycles, 4,700 by exchanges)
+    int each = 2;
+    while (each < 32 && n * each * 2 <= kFilterThreads) each *= 2;
+    __syncthreads();   // (a sort before may still be read)
+    exchange[0][threadIdx.x] = v;
+    __syncthreads();
+    const int i = threadIdx.x / each;
+    const unsigned long long mine = i < n ? exchange[0][i] : 0ull;
+    unsigned place = 0u;
+    for (int j = threadIdx.x & (each - 1); j < n; j += each) place += exchange[0][j] > mine;
+    for (int offset = 1; offset < each; offset <<= 1) place += __shfl_xor_sync(0xffffffffu, place, offset);
+    if (i < n && (threadIdx.x & (each - 1)) == 0) exchange[1][place] = mine;
+    __syncthreads();
+    return (int)threadIdx.x < n ? exchange[1][threadIdx.x] : 0ull;
+  }
   int size = 32, turn = 0;
   while (size < n) size *= 2;
   if ((int)threadIdx.x >= n) v = 0ull;
+  __syncthreads();
 #pragma unroll 1
   for (int run = 2; run <= size; run *= 2)
 #pragma unroll 1
@@ -159,10 +175,10 @@ class RowFilter {
   __device__ int choose(float temperature, int top_k, float top_p, float min_p, float u) {
     const bool by_number = top_k > 0 && top_k < vocab, by_weight = top_p < 1.0f;
     const bool first_only = !(temperature > 0.0f) || top_k == 1 || min_p > 1.0f || top_p <= 0.0f;
-    load();
-    // this CTA's maximum, and its bound for the list
-    const float largest = block_max(thread_max);
     const int asked = first_only ? 0 : by_number ? top_k : by_weight ? kGuess : 0;
+    const bool early = ctas == 1 && by_number && !first_only && top_k <= kFilterThreads;
+    load(early ? asked : 0);
+    const float largest = block_max(thread_max);   // this CTA's
     // What all of the tokens asked for are not below in one CTA, and what a CTA's share of them is not below in any.
     uint2 bounds = make_uint2(logit_key(-INFINITY), logit_key(-INFINITY));
     if (asked > 0 && largest > -INFINITY) bounds = least_of_maxima(largest, asked, (asked + ctas - 1) / ctas);
@@ -177,6 +193,18 @@ class RowFilter {
 
     scale = weight_scale(temperature, m);
     floor_weight = min_p > 0.0f ? (unsigned long long)ceil((double)min_p * (double)(1ull << kWeightBits)) : 0ull;
+    if (early) {   // of the tokens listed on the way those that are not below the bound of all
+      const int listed = sh.listed;
+      __syncthreads();
+      if (threadIdx.x == 0) sh.listed = 0;
+      __syncthreads();
+      if (listed >= top_k && listed <= kListed) {
+        const unsigned long long token = sh.early[threadIdx.x];
+        if ((int)threadIdx.x < listed && (unsigned)(token >> 32) >= bounds.x) sh.list[atomicAdd(&sh.listed, 1)] = token;
+        __syncthreads();
+        return choose_from_list(top_k, top_p, 0ull, u);
+      }
+    }
     const bool by_floor = !by_number && !by_weight && floor_weight > 0ull;
     if (by_floor) bound = m + temperature * (logf(min_p) * 1.0001f - 0.001f);   // (a little low: the list is longer than what stays of it)
     if (bound > -INFINITY) {
@@ -239,6 +267,26 @@ class RowFilter {
   // The run below `top` that a logit falls in: monotone, and the last one is for all that lies further below.
   __device__ static int bin_below(float top, float l) { return l == top ? 0 : (int)fminf((top - l) * 32.0f, (float)(kBins - 1)); }
 
+  // Puts a token on a list if `wanted`; a warp's threads come together.  The list may be too short: its length says so.
+  __device__ __forceinline__ void put_into(bool wanted, float l, int id, int* listed, unsigned long long* list) {
+    const unsigned who = __ballot_sync(0xffffffffu, wanted);
+    if (who == 0u) return;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(listed, __popc(who));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+    if (wanted && at < kListed) list[at] = ((unsigned long long)logit_key(l) << 32) | (unsigned)~id;
+  }
+  // ... on the first CTA's.
+  __device__ __forceinline__ void put(bool wanted, float l, int id) { put_into(wanted, l, id, at_first(&sh.listed), at_first(sh.list)); }
+  // Those of four tokens that are not below a bound.
+  __device__ __forceinline__ void put_quad(float4 v, float bound, int q, int* listed, unsigned long long* list) {
+    if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) return;
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) {
+      put_into(v.x >= bound, v.x, first_id + head + 4 * q + e, listed, list);
+      v.x = v.y, v.y = v.z, v.z = v.w;
+    }
+  }
   // A token of this thread's among those that do not stand in whole quads, -1 if it has none.
   __device__ __forceinline__ int edge_token() const {
     const int t = threadIdx.x, tail = count - head - 4 * quads;
@@ -246,28 +294,35 @@ class RowFilter {
   }
   __device__ __forceinline__ float4 quad(int q) const { return reinterpret_cast<const float4*>(tokens + head)[q]; }
 
-  // This thread's largest token (NaN is none).
-  __device__ __forceinline__ void load() {
-    float best = -INFINITY;
-    bool some = false;   // a token that is not NaN
+  // This thread's largest token (NaN is none).  With `asked` (and one CTA) tokens go on the list as they come, those that are not below a bound that so many tokens before are not
+  // below; the bound is taken anew when twice as many tokens have been seen.
+  __device__ __forceinline__ void load(int asked) {
+    const float nan = __int_as_float(0x7fffffff);
+    thread_max = nan;
     constexpr int kFlight = 8;
-    for (int q0 = threadIdx.x; q0 < quads; q0 += kFlight * kFilterThreads) {
-      const float nan = __int_as_float(0x7fffffff);
+    float bound = INFINITY;
+    int next_bound = kFlight * kFilterThreads;
+    for (int q0 = threadIdx.x; q0 - (int)threadIdx.x < quads; q0 += kFlight * kFilterThreads) {
       float4 v[kFlight];
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) v[u] = q0 + u * kFilterThreads < quads ? quad(q0 + u * kFilterThreads) : make_float4(nan, nan, nan, nan);
 #pragma unroll
-      for (int u = 0; u < kFlight; ++u) {
-        best = fmaxf(fmaxf(best, fmaxf(v[u].x, v[u].y)), fmaxf(v[u].z, v[u].w));
-        some |= v[u].x == v[u].x || v[u].y == v[u].y || v[u].z == v[u].z || v[u].w == v[u].w;
+      for (int u = 0; u < kFlight; ++u) thread_max = fmaxf(fmaxf(thread_max, fmaxf(v[u].x, v[u].y)), fmaxf(v[u].z, v[u].w));
+      if (asked == 0) continue;
+      const int seen = q0 - (int)threadIdx.x + kFlight * kFilterThreads;
+      if (seen >= next_bound) {   // (the same for all threads)
+        next_bound = 2 * seen;
+        const float largest = block_max(thread_max);
+        bound = largest > -INFINITY ? key_logit(least_of_maxima(largest, asked, asked).x) : INFINITY;   // (INFINITY: whole runs of tokens without one above -infinity)
+        __syncthreads();
       }
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) put_quad(v[u], bound, q0 + u * kFilterThreads, &sh.listed, sh.early);
     }
     const int i = edge_token();
-    if (i >= 0) {
-      best = fmaxf(best, tokens[i]);
-      some |= tokens[i] == tokens[i];
-    }
-    thread_max = some ? best : __int_as_float(0x7fffffff);
+    const float l = i >= 0 ? tokens[i] : nan;
+    thread_max = fmaxf(thread_max, l);
+    if (asked != 0) put_into(l >= bound, l, first_id + i, &sh.listed, sh.early);
   }
   // NaN if all are.
   __device__ __forceinline__ float block_max(float v) {
@@ -346,15 +401,6 @@ class RowFilter {
     return id;
   }
 
-  // Puts a token on the first CTA's list if `wanted`; a warp's threads come together.  The list may be too short: its length says so.
-  __device__ __forceinline__ void put(bool wanted, float l, int id) {
-    const unsigned who = __ballot_sync(0xffffffffu, wanted);
-    if (who == 0u) return;
-    int at = 0;
-    if (lane == 0) at = atomicAdd(at_first(&sh.listed), __popc(who));
-    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-    if (wanted && at < kListed) at_first(sh.list)[at] = ((unsigned long long)logit_key(l) << 32) | (unsigned)~id;
-  }
   // Lists the tokens that are not below the bound; with `weights` the weight of all tokens, this thread's share of it.
   __device__ __forceinline__ void list_from(float bound, bool weights, unsigned long long& mine) {
     const float nan = __int_as_float(0x7fffffff);
@@ -363,17 +409,15 @@ class RowFilter {
       float4 v[kFlight];
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) v[u] = q0 + u * kFilterThreads < quads ? quad(q0 + u * kFilterThreads) : make_float4(nan, nan, nan, nan);
+      if (!weights) {
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) put_quad(v[u], bound, q0 + u * kFilterThreads, at_first(&sh.listed), at_first(sh.list));
+        continue;
+      }
 #pragma unroll 1
       for (int u = 0; u < kFlight; ++u) {
-        if (weights) mine += (weight(v[0].x) + weight(v[0].y)) + (weight(v[0].z) + weight(v[0].w));
-        if (__any_sync(0xffffffffu, fmaxf(fmaxf(v[0].x, v[0].y), fmaxf(v[0].z, v[0].w)) >= bound)) {
-          const int id = first_id + head + 4 * (q0 + u * kFilterThreads);
-#pragma unroll 1
-          for (int e = 0; e < 4; ++e) {
-            put(v[0].x >= bound, v[0].x, id + e);
-            v[0].x = v[0].y, v[0].y = v[0].z, v[0].z = v[0].w;
-          }
-        }
+        mine += (weight(v[0].x) + weight(v[0].y)) + (weight(v[0].z) + weight(v[0].w));
+        put_quad(v[0], bound, q0 + u * kFilterThreads, at_first(&sh.listed), at_first(sh.list));
 #pragma unroll
         for (int other = 0; other + 1 < kFlight; ++other) v[other] = v[other + 1];
       }
@@ -416,13 +460,20 @@ class RowFilter {
   template <typename F>
   __device__ __forceinline__ void for_tokens(F f) {
     const float nan = __int_as_float(0x7fffffff);
-    for (int q0 = threadIdx.x; q0 - (int)threadIdx.x < quads; q0 += kFilterThreads) {
-      float4 v = q0 < quads ? quad(q0) : make_float4(nan, nan, nan, nan);
-      const int id = q0 < quads ? first_id + head + 4 * q0 : -8;
+    constexpr int kFlight = 4;
+    for (int q0 = threadIdx.x; q0 - (int)threadIdx.x < quads; q0 += kFlight * kFilterThreads) {
+      float4 v[kFlight];
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) v[u] = q0 + u * kFilterThreads < quads ? quad(q0 + u * kFilterThreads) : make_float4(nan, nan, nan, nan);
 #pragma unroll 1
-      for (int e = 0; e < 4; ++e) {
-        f(v.x, id + e);
-        v.x = v.y, v.y = v.z, v.z = v.w;
+      for (int u = 0; u < kFlight; ++u) {
+        const int q = q0 + u * kFilterThreads, id = q < quads ? first_id + head + 4 * q : -8;
+        f(v[0].x, id);
+        f(v[0].y, id + 1);
+        f(v[0].z, id + 2);
+        f(v[0].w, id + 3);
+#pragma unroll
+        for (int other = 0; other + 1 < kFlight; ++other) v[other] = v[other + 1];
       }
     }
     const int i = edge_token();
@@ -551,36 +602,55 @@ class RowFilter {
   }
   // The token that the number falls on among the kept ones, in order of ids.
   __device__ __forceinline__ int draw(const Border& kept, float u) {
-    const int segment = (count + kFilterWarps - 1) / kFilterWarps, begin = min(count, warp * segment), end = min(count, begin + segment);
-    auto kept_weight = [&](int i) {
-      const float l = tokens[i];
-      if (!kept.holds(logit_key(l), first_id + i)) return 0ull;
+    auto kept_weight = [&](float l, int i) {
       const unsigned long long w = weight(l);
-      return w >= floor_weight ? w : 0ull;
+      return kept.holds(logit_key(l), first_id + i) && w >= floor_weight ? w : 0ull;
     };
+    // consecutive quads per warp; what stands in front of the first and behind the last one is the first and the last warp's
+    const int segment = (quads + kFilterWarps - 1) / kFilterWarps, begin = min(quads, warp * segment), end = min(quads, begin + segment);
+    const float nan = __int_as_float(0x7fffffff);
     unsigned long long mine = 0ull;
-#pragma unroll 4
-    for (int i = begin + lane; i < end; i += 32) mine += kept_weight(i);
+    constexpr int kFlight = 4;
+    for (int q0 = begin + lane; q0 < end; q0 += 32 * kFlight) {
+      float4 v[kFlight];
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) v[f] = q0 + 32 * f < end ? quad(q0 + 32 * f) : make_float4(nan, nan, nan, nan);
+#pragma unroll 1
+      for (int f = 0; f < kFlight; ++f) {
+        const int i = head + 4 * (q0 + 32 * f);
+        mine += (kept_weight(v[0].x, i) + kept_weight(v[0].y, i + 1)) + (kept_weight(v[0].z, i + 2) + kept_weight(v[0].w, i + 3));
+#pragma unroll
+        for (int other = 0; other + 1 < kFlight; ++other) v[other] = v[other + 1];
+      }
+    }
+    const int first = warp == 0 ? 0 : head + 4 * begin, last = warp == kFilterWarps - 1 ? count : head + 4 * end;   // this warp's tokens
+    if (warp == 0 && lane < head) mine += kept_weight(tokens[lane], lane);
+    if (warp == kFilterWarps - 1 && head + 4 * quads + lane < count) mine += kept_weight(tokens[head + 4 * quads + lane], head + 4 * quads + lane);
     mine = warp_sum_u64(mine);
     unsigned long long all, before = block_prefix(lane == 0 ? mine : 0ull, sh.scan, all);
     before = __shfl_sync(0xffffffffu, before, 0);
     const unsigned long long* of_cta = gather(all, 0ull);
-    unsigned long long total = 0ull;
+    unsigned long long total = 0ull, start = 0ull;
     for (int c = 0; c < ctas; ++c) {
-      if (c < rank) before += of_cta[c];
+      if (c < rank) start += of_cta[c];
       total += of_cta[c];
     }
     const unsigned long long target = target_of(u, total);
-    if (target >= before && target < before + mine) {
-      for (int i0 = begin; i0 < end; i0 += 32) {
-        const unsigned long long w = i0 + lane < end ? kept_weight(i0 + lane) : 0ull;
-        const unsigned long long upto = before + warp_prefix_u64(w, lane);
-        const unsigned past = __ballot_sync(0xffffffffu, target < upto);
-        if (past != 0u) {
-          if (lane == __ffs(past) - 1) *at_first(&sh.found_id) = first_id + i0 + lane;
-          break;
+    if (target >= start && target < start + all) {   // in this CTA: all its threads look through the warp's tokens that it falls on
+      if (lane == 0 && target >= start + before && target < start + before + mine) sh.last_run[0] = first, sh.last_run[1] = last, sh.above = start + before;
+      __syncthreads();
+      const int from = sh.last_run[0], to = sh.last_run[1], each = (to - from + kFilterThreads - 1) / kFilterThreads;
+      const int a = min(to, from + (int)threadIdx.x * each), b = min(to, a + each);
+      unsigned long long part = 0ull, sum;
+      for (int i = a; i < b; ++i) part += kept_weight(tokens[i], i);
+      unsigned long long running = sh.above + block_prefix(part, sh.scan, sum);
+      if (target >= running && target < running + part) {
+        int i = a;
+        for (; i < b; ++i) {
+          running += kept_weight(tokens[i], i);
+          if (target < running) break;
         }
-        before = __shfl_sync(0xffffffffu, upto, 31);
+        *at_first(&sh.found_id) = first_id + i;
       }
     }
     sync();
@@ -631,9 +701,9 @@ TLIE_EXPORT int tlie_sample_filtered(const float* logits, long long row_stride, 
                                      const int* top_k, const float* top_p, const float* min_p, const float* uniforms, int* out, cudaStream_t stream) {
   if (count <= 0) return 0;
   if (vocab <= 0 || vocab > kFilterMaxVocab || row_stride < 0) return (int)cudaErrorInvalidValue;
-  // CTAs of a row's cluster: as many as the SMs hold one each of, with at least 2,048 tokens.
+  // CTAs of a row's cluster: at most two per SM in all, with at least 8,192 tokens each.
   int ctas = 1;
-  while (ctas < 8 && vocab > ctas * 2048 && (long long)count * ctas * 2 <= device_sm_count()) ctas *= 2;
+  while (ctas < 8 && vocab > ctas * 8192 && (long long)count * ctas <= device_sm_count()) ctas *= 2;
   const int slice = ((vocab + ctas - 1) / ctas + 3) & ~3;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)count * ctas);
