@@ -16,7 +16,7 @@
 namespace tlie {
 
 constexpr int kFilterThreads = 512, kFilterWarps = kFilterThreads / 32;
-constexpr int kBinBits = 10, kBins = 1 << kBinBits, kBinsEach = kBins / kFilterThreads;
+constexpr int kBinBits = 11, kBins = 1 << kBinBits, kBinsEach = kBins / kFilterThreads;
 constexpr int kListed = kFilterThreads;    // tokens of the list, one per thread
 constexpr int kFilterMaxVocab = 1 << 19;   // (so many weights of 2^44 and less: sums fit 64 bits, a token's id and weight one number)
 constexpr int kWeightBits = 44;
@@ -71,7 +71,7 @@ struct Border {
 // tokens tells whether they suffice; min_p alone says itself which tokens it leaves.  Bound by the reading of the logits then, or, with top_p alone, by the 35 instructions of a
 // token's exact weight; one row by the chain of its steps.
 //
-// Where the list does not do (top_k beyond it, flat rows), a border is found from a histogram over 1,024 runs of logits, 1/32 wide, below the largest, of numbers or
+// Where the list does not do (top_k beyond it, flat rows), a border is found from a histogram over 2,048 runs of logits, 1/64 wide, below the largest, of numbers or
 // of exact weights, and from the tokens of the run that it falls in, which the first CTA sorts.  Where those are too many (equal logits, or very close ones) the run is
 // cut by the bits of the logits, and equal ones by id.
 struct FilterShared {
@@ -265,7 +265,7 @@ class RowFilter {
     return ctas > 1 ? cluster.map_shared_rank(mine, 0) : mine;
   }
   // The run below `top` that a logit falls in: monotone, and the last one is for all that lies further below.
-  __device__ static int bin_below(float top, float l) { return l == top ? 0 : (int)fminf((top - l) * 32.0f, (float)(kBins - 1)); }
+  __device__ static int bin_below(float top, float l) { return l == top ? 0 : (int)fminf((top - l) * 64.0f, (float)(kBins - 1)); }
 
   // Puts a token on a list if `wanted`; a warp's threads come together.  The list may be too short: its length says so.
   __device__ __forceinline__ void put_into(bool wanted, float l, int id, int* listed, unsigned long long* list) {
@@ -343,9 +343,10 @@ class RowFilter {
     const int bin = bin_below(largest, thread_max);   // (of a thread without a token the last)
     atomicAdd(&sh.low[bin], 1u);
     __syncthreads();
-    const unsigned first = sh.low[threadIdx.x * kBinsEach], second = sh.low[threadIdx.x * kBinsEach + 1];
-    static_assert(kBinsEach == 2, "two runs per thread");
-    unsigned upto = first + second;
+    unsigned of_run[kBinsEach], here = 0u;
+#pragma unroll
+    for (int i = 0; i < kBinsEach; ++i) here += of_run[i] = sh.low[threadIdx.x * kBinsEach + i];
+    unsigned upto = here;
 #pragma unroll
     for (int offset = 1; offset < 32; offset <<= 1) {
       const unsigned other = __shfl_up_sync(0xffffffffu, upto, offset);
@@ -353,13 +354,13 @@ class RowFilter {
     }
     if (lane == 31) sh.scan[warp] = upto;
     __syncthreads();
-    unsigned before = upto - first - second;
+    unsigned before = upto - here;
     for (int w = 0; w < warp; ++w) before += (unsigned)sh.scan[w];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const unsigned number = i == 0 ? asked : share;
-      if (before < number && before + first >= number) sh.last_run[i] = threadIdx.x * kBinsEach;
-      else if (before + first < number && before + first + second >= number) sh.last_run[i] = threadIdx.x * kBinsEach + 1;
+    for (int i = 0; i < kBinsEach; ++i) {
+      if (before < (unsigned)asked && before + of_run[i] >= (unsigned)asked) sh.last_run[0] = threadIdx.x * kBinsEach + i;
+      if (before < (unsigned)share && before + of_run[i] >= (unsigned)share) sh.last_run[1] = threadIdx.x * kBinsEach + i;
+      before += of_run[i];
     }
     __syncthreads();
 #pragma unroll
