@@ -16,7 +16,7 @@ exit status 1 (app/reference_cli.cpp:20-25).  PROMPT is text when MODEL_DIR hold
 otherwise a list of token ids separated by commas or spaces; with ``--prompt-len N``
 (and ``--prompt-seed S``) the PROMPT argument is left out and N seeded random token ids
 stand in for it.  Options, before or after the positionals: ``--dtype bfloat16|float32``,
-``--temperature``, ``--top-p``, ``--seed``, ``--batch``, ``--max-batch-tokens``,
+``--temperature``, ``--top-p``, ``--top-k``, ``--min-p``, ``--seed``, ``--batch``, ``--max-batch-tokens``,
 ``--page-size``, ``--num-pages`` (cache pages; by default what the request needs),
 ``--device`` (a CUDA device; there is no CPU path and ``cpu`` is refused with an error), ``--random-config FILE --weights-seed N``
 (the command runs on a model of that config.json with seeded random weights, written to MODEL_DIR, or to a temporary folder
@@ -116,7 +116,8 @@ def _generate(args) -> int:
 
     prefill, decode = StepTimings(), StepTimings()   # device time of compute and of copies, as the reference reports them (app/cuda_reference.cu:149-226)
     started = time.perf_counter()
-    request_id = engine.add_request(prompt, SamplingParams(max_tokens=max_tokens, temperature=args.temperature, top_p=args.top_p, seed=args.seed))
+    request_id = engine.add_request(prompt, SamplingParams(max_tokens=max_tokens, temperature=args.temperature, top_p=args.top_p, seed=args.seed,
+                                                                  top_k=args.top_k, min_p=args.min_p))
     while not engine.requests[request_id].generated and engine.has_unfinished():
         engine.step(prefill)
     prefill_ms = (time.perf_counter() - started) * 1e3
@@ -331,6 +332,8 @@ def main(argv: list[str] | None = None) -> int:
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     parser.add_argument("--temperature", type=float, default=0.0)
     parser.add_argument("--top-p", type=float, default=1.0)
+    parser.add_argument("--top-k", type=int, default=0)
+    parser.add_argument("--min-p", type=float, default=0.0)
     parser.add_argument("--seed", type=int, default=0)
     parser.add_argument("--batch", type=int, default=1)
     parser.add_argument("--max-batch-tokens", type=int, default=2048)

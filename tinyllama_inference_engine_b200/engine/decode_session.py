@@ -66,6 +66,13 @@ class DecodeSession:
         self.top_p = torch.ones(count, dtype=torch.float32, device=device)
         self.seeds = torch.zeros(count, dtype=torch.int64, device=device)
         self.counters = torch.zeros(count, dtype=torch.int64, device=device)
+        # what the rows whose request has top_k or min_p are chosen with (a row number, or -1 where the request has neither)
+        self.filtered_rows = torch.full((count,), -1, dtype=torch.int32, device=device)
+        self.top_k = torch.zeros(count, dtype=torch.int32, device=device)
+        self.min_p = torch.zeros(count, dtype=torch.float32, device=device)
+        self.uniforms = torch.zeros(count, dtype=torch.float32, device=device)
+        self.filtered = False              # whether a loaded request has such options: a step of such requests is a graph of its own
+        self._other: tuple = (0, None, None)   # (steps run kernel by kernel, graph, logits) of the kind of step that ``filtered`` does not say
         self.positions = [0] * count      # host mirror: position of the token each request runs next
         self.use_graph = use_graph
         self._fresh = True
@@ -110,6 +117,15 @@ class DecodeSession:
             self.top_p.copy_(torch.tensor([p.top_p for p in params], dtype=torch.float32))
             self.seeds.copy_(torch.tensor([p.seed for p in params], dtype=torch.int64))
             self.counters.copy_(torch.tensor(draw_indices or [0] * self.count, dtype=torch.int64))
+            rows = [i if p.filtered else -1 for i, p in enumerate(params)]
+            filtered = any(row >= 0 for row in rows)
+            if filtered:
+                self.filtered_rows.copy_(torch.tensor(rows, dtype=torch.int32))
+                self.top_k.copy_(torch.tensor([p.top_k for p in params], dtype=torch.int32))
+                self.min_p.copy_(torch.tensor([p.min_p for p in params], dtype=torch.float32))
+            if filtered != self.filtered:
+                self.filtered = filtered
+                self._other, (self._eager_steps, self.graph, self.logits) = (self._eager_steps, self.graph, self.logits), self._other
 
     def _reserve_and_fill_tables(self) -> bool:
         """Pages for this step's positions; returns whether any block-table row changed."""
@@ -141,6 +157,9 @@ class DecodeSession:
         caches = self.cache.layer_caches(self.d_tables)
         self.logits = self.runner.model.forward(self.ctx, caches)
         ops.sample(self.logits, self.temperature, self.top_p, self.seeds, self.counters, self.sampled)
+        if self.filtered:
+            ops.uniforms(self.seeds, self.counters, self.uniforms)
+            ops.sample_filtered(self.logits, self.temperature, self.top_k, self.top_p, self.min_p, self.uniforms, self.sampled, rows=self.filtered_rows)
         c = self.ctx
         if self.publish:
             ops.decode_advance(c.token_ids, self.sampled, c.positions, c.seq_lens, c.first_positions, self.counters, self._mailbox, self._steps_done)

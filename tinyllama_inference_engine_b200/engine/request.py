@@ -16,6 +16,8 @@ class SamplingParams:
     seed         seed of the request's own random stream; draws do not depend on the batch.
     ignore_eos   the reference never stops at the end-of-sequence token (it runs exactly
                  max_tokens, app/server.cpp:468-470); False stops when ``eos_token_id`` is drawn.
+    top_k        keep that many of the most probable tokens (0 keeps all); top_p is then a share of what they weigh.
+    min_p        keep tokens with at least this share of the most probable one's probability (0 keeps all).
     """
 
     max_tokens: int = 16
@@ -23,6 +25,13 @@ class SamplingParams:
     top_p: float = 1.0
     seed: int = 0
     ignore_eos: bool = True
+    top_k: int = 0
+    min_p: float = 0.0
+
+    @property
+    def filtered(self) -> bool:
+        """Whether the choice of tokens needs ``ops.sample_filtered`` (requests without these options keep ``ops.sample`` and its draws)."""
+        return self.temperature > 0.0 and (self.top_k > 0 or self.min_p > 0.0)
 
     def __post_init__(self) -> None:
         if isinstance(self.max_tokens, bool) or not isinstance(self.max_tokens, int) or self.max_tokens < 1:
@@ -31,6 +40,10 @@ class SamplingParams:
             raise EngineError("temperature must be >= 0")
         if not 0.0 < self.top_p <= 1.0:
             raise EngineError("top_p must be in (0, 1]")
+        if isinstance(self.top_k, bool) or not isinstance(self.top_k, int) or not 0 <= self.top_k < 1 << 31:
+            raise EngineError("top_k must be an integer >= 0 (0 keeps all tokens)")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise EngineError("min_p must be in [0, 1]")
 
 
 WAITING, RUNNING, FINISHED = "waiting", "running", "finished"
