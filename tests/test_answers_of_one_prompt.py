@@ -124,6 +124,56 @@ def test_attention_over_a_shared_prefix(ops, dtype, heads, shape):
     compare_attention(call_attention(ops, case), case, *plain_attention(case))
 
 
+# (prefix once for all rows, own keys on the tensor cores): every way that the bfloat16 kernels can be put together, whatever the sizes would choose
+WAYS = {"row by row": (0, 0), "prefix once, own by rows": (1, 0), "prefix once, own by entries": (1, 1), "all by entries": (0, 1)}
+
+
+@pytest.fixture
+def way(request, ops, monkeypatch):
+    prefix, own, parts, ctas = request.param
+    monkeypatch.setattr(ops.fast, "use_prefix", prefix)
+    monkeypatch.setattr(ops.fast, "use_own", own)
+    if parts:
+        monkeypatch.setattr(ops.fast, "prefix_tc_parts", lambda rows, kv_heads, group, head_dim, shared: (max(1, min(parts, -(-shared // ops.fast.PREFIX_TC_KEYS[head_dim]))), 1.0))
+    if ctas:
+        monkeypatch.setattr(ops.fast, "prefix_rows_ctas", lambda *_: ctas)
+    ops.fast.shared_prefix_plan.cache_clear()
+    yield request.param
+    ops.fast.shared_prefix_plan.cache_clear()
+
+
+EVERY_WAY = pytest.mark.parametrize("way", [(*w, 0, 0) for w in WAYS.values()], ids=WAYS.keys(), indirect=True)
+TC_HEADS = [h for h in HEADS if h[2] in (64, 128)] + [(72, 2, 128), (128, 1, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("heads", TC_HEADS, ids=lambda h: f"{h[0]}-{h[1]}x{h[2]}")
+@EVERY_WAY
+def test_every_way_to_put_the_kernels_together(ops, way, heads, shape):
+    page_size, shared, entries = SHAPES[shape]
+    case = attention_case(len(shape) + 1, torch.bfloat16, *heads, page_size, shared, entries)
+    compare_attention(call_attention(ops, case), case, *plain_attention(case))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", [(1, 0, 32, 1), (1, 0, 7, 2), (1, 1, 3, 0), (0, 0, 0, 1), (0, 0, 0, 4), (0, 0, 0, 8), (1, 0, 1, 8)], ids=lambda w: "-".join(map(str, w)), indirect=True)
+@pytest.mark.parametrize("heads", [(16, 2, 64), (12, 4, 128)], ids=lambda h: f"{h[0]}-{h[1]}x{h[2]}")
+@pytest.mark.parametrize("shape", ["long", "answers of several lengths", "rows inside the prefix"])
+def test_runs_of_the_prefix_and_ctas_of_a_row(ops, way, heads, shape):
+    page_size, shared, entries = SHAPES[shape]
+    case = attention_case(len(shape) + 2, torch.bfloat16, *heads, page_size, 3 * shared + 5, entries, front=1, behind=1, wider=16)
+    compare_attention(call_attention(ops, case), case, *plain_attention(case))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,page_size,wider", [((8, 2, 64), 24, 0), ((8, 2, 128), 64, 3), ((160, 1, 64), 16, 0), ((7, 7, 176), 1, 0), ((4, 2, 240), 40, 0)])
+def test_sizes_of_the_general_kernel(ops, dtype, heads, page_size, wider):
+    case = attention_case(11, dtype, *heads, page_size, 210, [(31, 1), (1, 1), (64, 33), (0, 0), (95, 2)], front=1, behind=2, wider=wider)
+    compare_attention(call_attention(ops, case), case, *plain_attention(case))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
 @pytest.mark.parametrize("dim", [64, 128, 96])
@@ -164,6 +214,96 @@ def test_later_keys_and_values_that_are_no_numbers_stay_out(ops, dtype, bad):
                 assert (torch.isnan(column) if math.isnan(bad) else column == bad).all()
                 other = torch.arange(dim) != 5
                 assert torch.equal(got[19:30].view(11, 8, dim)[:, :, other], clean[19:30].view(11, 8, dim)[:, :, other])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dim", [64, 128])
+@EVERY_WAY
+def test_numbers_that_are_none_in_every_way(ops, way, dim, bad):
+    """Behind a row's position they stay out, in the prefix and behind it; a value among a row's keys shows in its column alone, a key or a query in its heads."""
+    case = attention_case(12, torch.bfloat16, 8, 2, dim, 32, 200, [(0, 150), (40, 3), (3, 1)])
+    clean = call_attention(ops, case)
+    position = case["positions"].cuda()
+    for place in (7, 130, 199):
+        page, slot = case["table"][:, place // 32].long(), place % 32   # every entry's: key 199 lies in a page that each has a copy of
+        sees = position >= place
+        spoiled = {**case, "pages": case["pages"].clone()}
+        spoiled["pages"][page, 1, 1, slot, 9] = bad
+        got = call_attention(ops, spoiled).view(-1, 8, dim)
+        touched = torch.zeros(got.shape, dtype=torch.bool, device="cuda")
+        touched[:, 4:, 9] = sees[:, None]
+        assert torch.equal(got[~touched], clean.view(-1, 8, dim)[~touched])
+        column = got[touched].float()
+        assert (torch.isnan(column) if math.isnan(bad) else column == bad).all()
+        spoiled["pages"][page] = case["pages"][page]
+        spoiled["pages"][page, 0, 1, slot, 9] = bad
+        got = call_attention(ops, spoiled).view(-1, 8, dim)
+        touched[:, 4:] = sees[:, None, None]
+        assert torch.equal(got[~touched], clean.view(-1, 8, dim)[~touched])
+        if math.isnan(bad):
+            assert torch.isnan(got[touched]).all()
+    spoiled = {**case, "qkv": case["qkv"].clone()}
+    spoiled["qkv"][151, 3 * dim + 2] = bad
+    got = call_attention(ops, spoiled).view(-1, 8, dim)
+    touched = torch.zeros(got.shape, dtype=torch.bool, device="cuda")
+    touched[151, 3] = True
+    assert torch.equal(got[~touched], clean.view(-1, 8, dim)[~touched]) and torch.isnan(got[151, 3]).all()
+
+
+@pytest.mark.gpu
+@EVERY_WAY
+def test_rows_without_keys_and_bad_pages_in_every_way(ops, way):
+    from tinyllama_inference_engine_b200.errors import KernelError
+
+    for dim in (64, 128):
+        case = attention_case(13, torch.bfloat16, 8, 2, dim, 16, 100, [(20, 4), (6, 1), (30, 0), (9, 70)])
+        for row, at in ((0, -1), (3, -100), (4, -2147483648), (30, -1)):
+            case["positions"][row] = at
+        got = call_attention(ops, case)
+        assert (got[[0, 3, 4, 30]] == 0).all()
+        compare_attention(got, case, *plain_attention(case))
+        for entry, page, message in ((0, 2, "outside the pool"), (3, 8, "outside the pool"), (1, None, "beyond the block table")):
+            case = attention_case(14, torch.bfloat16, 8, 2, dim, 16, 100, [(20, 4), (6, 1), (30, 0), (70, 70)], poison=False)
+            if page is None:
+                case["table"] = case["table"].clamp(min=0)
+                case["positions"][4] = 2147483647
+            else:
+                case["table"][entry, page] = 1 << 30
+            call_attention(ops, case)
+            with pytest.raises(KernelError, match=message):
+                ops.check_device_errors(torch.device("cuda:0"))
+
+
+@pytest.mark.gpu
+@EVERY_WAY
+def test_every_way_in_a_graph_beside_another_stream(ops, way):
+    case = attention_case(15, torch.bfloat16, 8, 2, 128, 64, 300, [(30, 1), (70, 4), (1, 1)])
+    want, off = plain_attention(case)
+    c = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in case.items()}
+    outs = [torch.full((6, 8 * 128), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+    call = lambda out: ops.shared_prefix_attention(c["qkv"], c["pages"], c["positions"], c["seq_starts"], c["table"], 300, out, 8, 2, 128, 64)  # noqa: E731
+    call(outs[0])
+    graphs = []
+    for out in outs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(out)
+            call(out)   # (the second waits for the first)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for out in outs:
+            out.fill_(7.0)
+        torch.cuda.synchronize()
+        for i in range(3):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay() if i < 2 else call(outs[2])
+        torch.cuda.synchronize()
+        for out in outs:
+            compare_attention(out, case, want, off)
+            assert torch.equal(out, outs[0])
 
 
 @pytest.mark.gpu
@@ -240,6 +380,7 @@ def test_attention_refuses():
     wrong = {
         "no CPU path": {}, "head sizes": dict(head_dim=60), "multiple of key/value heads": dict(kv_heads=3), "qkv must be": dict(qkv=torch.zeros(3, 255)),
         "out must be [rows": dict(out=torch.zeros(3, 255)), "of qkv's dtype": dict(out=torch.zeros(3, 256, dtype=torch.bfloat16)), "pages must be": dict(page_size=32),
+        "16-byte boundary": dict(pages=torch.zeros(4 * 2 * 16 * 64 + 1)[1:].view(4, 2, 1, 16, 64)),
         "a block table": dict(seq_starts=torch.zeros(4, dtype=torch.int32)), "positions [rows]": dict(positions=torch.zeros(4, dtype=torch.int32)),
         "shared must be a whole number from 0 to the 32 keys": dict(shared=33), "got -1": dict(shared=-1), "got True": dict(shared=True), "scale must be": dict(scale=0.0),
         "got nan": dict(scale=float("nan")), "are int32": dict(positions=torch.zeros(3, dtype=torch.int64)), "contiguous rows": dict(qkv=torch.zeros(6 * 64, 3).t()),

@@ -8,18 +8,18 @@
 // with M = max m_i, out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i (scores in units of log2).  Parts of the prefix are worked out
 // for all rows of the step at once, so that its keys and values are read once per 32 rows and not once per request; parts of an entry's own keys for its rows.
 //
-// A CTA owns one key/value head, 32 (row, head) pairs and a run of keys, which it copies to shared memory 32 at a time: in a score a lane owns a key, in a
-// weighted sum some of the value's channels.  All sums are 32-bit.
+// A CTA owns one key/value head, 32 (row, head) pairs and a run of keys, which it copies to shared memory 32 at a time, the next ones while it works on these.  Scores (32 x 32) and
+// weighted values (32 x head size) are register tiles of two pairs per thread: 32 multiply-adds for six 16-byte reads of shared memory, 64 for ten.  All sums are
+// 32-bit.  Bound by the multiply-adds where there are many rows, by the chain of a run's chunks where there are few (so runs are short there).
 #include "common.cuh"
+#include "mma_utils.cuh"
 #include "shared_memory_limit.cuh"
 
 namespace tlie {
 
 constexpr int kPairs = 32;         // (row, head) pairs of a CTA
-constexpr int kPairWarps = 4;
-constexpr int kPairsPerWarp = kPairs / kPairWarps;
-constexpr int kChunk = 32;         // keys in shared memory at a time: one per lane
-constexpr int kDimsPerLane = 8;    // up to 256
+constexpr int kPairThreads = 128;  // 16 times two pairs, 8 times four keys, or the value's channels in eight parts
+constexpr int kChunk = 32;         // keys in shared memory at a time
 constexpr float kToLog2 = 1.4426950408889634f;
 constexpr int kBadPage = 8;        // the bit of the device's error word
 
@@ -49,33 +49,39 @@ __device__ __forceinline__ int page_of(const SharedPrefixParams& p, const int* t
   return 0;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kPairWarps * 32) shared_prefix_generic_kernel(SharedPrefixParams p, int own_tiles) {
-  extern __shared__ float smem[];
-  const int D = p.head_dim, key_row = D + 4;   // four floats more: eight lanes that read 16 bytes of their keys' rows touch all banks
+__device__ __forceinline__ void dot4(float& acc, float4 a, float4 b) { acc = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, acc)))); }
+__device__ __forceinline__ void add4(float4& acc, float w, float4 v) {
+  acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
+}
+
+// MAX_DIM: 64, 128 or 256, the head size rounded up.
+template <typename T, int MAX_DIM>
+__global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(SharedPrefixParams p, int own_tiles) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int kQuads = MAX_DIM / 32;         // four channels each, of this thread's share of a value
+  const int D = p.head_dim, key_row = D + 4;   // four floats more: eight threads that read 16 bytes of their keys' rows touch all banks
   float* q_smem = smem;                        // [pairs][D]
-  float* k_smem = q_smem + kPairs * D;         // [keys][D + 4]
-  float* v_smem = k_smem + kChunk * key_row;   // [keys][D]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* w_smem = q_smem + kPairs * D;         // [pairs][keys + 4]
+  constexpr int kWeightRow = kChunk + 4;
+  float* chunks = w_smem + kPairs * kWeightRow;   // twice [keys][D + 4] of keys and [keys][D] of values
+  const int chunk_floats = kChunk * key_row + kChunk * D;
+  const int lane = threadIdx.x & 31, ty = threadIdx.x >> 3, tx = threadIdx.x & 7;
   const int kvh = blockIdx.y, group = p.q_heads / p.kv_heads;
+  grid_dependency_wait();
   const int first_row = max(0, p.seq_starts[0]), end_row = min(p.seq_starts[p.entries], p.rows);
   const bool of_prefix = (int)blockIdx.z < p.prefix_parts;
   const int part = blockIdx.z;
 
   // which pairs: consecutive ones of all rows, or of one entry's rows
-  int row0, pairs, entry = 0;
-  if (of_prefix) {
-    const long long all = (long long)(end_row - first_row) * group, at = (long long)blockIdx.x * kPairs;
-    if (at >= all) return;
-    row0 = first_row;
-    pairs = (int)min((long long)kPairs, all - at);
-  } else {
-    if ((int)blockIdx.x >= own_tiles) return;
-    row0 = 0;
-    pairs = 0;
-  }
+  int row0 = 0, pairs = 0, entry = 0;
   long long pair0 = (long long)blockIdx.x * kPairs;
-  if (!of_prefix) {   // the entry that this tile number falls to, counting every entry's tiles: 32 entries at a time
+  if (of_prefix) {
+    const long long all = (long long)(end_row - first_row) * group;
+    if (pair0 >= all) return;
+    row0 = first_row;
+    pairs = (int)min((long long)kPairs, all - pair0);
+  } else {   // the entry that this tile number falls to, counting every entry's tiles: 32 entries at a time
+    if ((int)blockIdx.x >= own_tiles) return;
     int tiles_before = 0;
     for (int e0 = 0; e0 < p.entries; e0 += 32) {
       const int e = e0 + lane;
@@ -112,164 +118,233 @@ __global__ void __launch_bounds__(kPairWarps * 32) shared_prefix_generic_kernel(
 
   const int* table = p.block_table + (size_t)entry * p.table_stride;
   const long long room = (long long)p.table_stride * p.page_size;
-  // keys a pair sees in this kind of part: below `limit`
-  auto limit_of = [&](int i) {
-    long long seen = (long long)p.positions[row_of(i)] + 1;
+  // keys a pair sees in this kind of part: below the result; lane i has pair i's
+  int limit = 0;
+  if (lane < pairs) {
+    long long seen = (long long)p.positions[row_of(lane)] + 1;
     if (seen > room) {
-      atomicOr(p.error_flag, kBadPage);
+      if (threadIdx.x < 32) atomicOr(p.error_flag, kBadPage);
       seen = room;
     }
-    return (int)(of_prefix ? min(seen, (long long)p.shared) : seen);
-  };
-  int last = 0;
-  for (int i = lane; i < pairs; i += 32) last = max(last, limit_of(i));
-  last = __reduce_max_sync(0xffffffffu, last);
+    limit = (int)max(0ll, of_prefix ? min(seen, (long long)p.shared) : seen);
+  }
+  const int last = __reduce_max_sync(0xffffffffu, limit);
+  const int limits[2] = {__shfl_sync(0xffffffffu, limit, 2 * ty), __shfl_sync(0xffffffffu, limit, 2 * ty + 1)};
+  const int lowest = __reduce_min_sync(0xffffffffu, lane < pairs ? limit : 0x7fffffff);
   const int from = of_prefix ? 0 : p.shared;
-  const int chunks = last > from ? (last - from + kChunk - 1) / kChunk : 0;
+  const int all_chunks = last > from ? (last - from + kChunk - 1) / kChunk : 0;
   const int parts_here = of_prefix ? p.prefix_parts : p.own_parts, which = of_prefix ? part : part - p.prefix_parts;
-  const int per_part = (chunks + parts_here - 1) / parts_here;
-  const int chunk_begin = which * per_part, chunk_end = min(chunks, chunk_begin + per_part);
+  const int chunk_begin = (int)((long long)all_chunks * which / parts_here), chunk_end = (int)((long long)all_chunks * (which + 1) / parts_here);
 
-  for (int i = threadIdx.x; i < kPairs * D; i += blockDim.x) {
+  const size_t plane = (size_t)p.kv_heads * p.page_size * D;
+  // The keys and values of a chunk: 16 bytes a copy.  Places past the last key become zeros.
+  auto fetch = [&](int chunk) {
+    constexpr int kEach = 16 / (int)sizeof(T);
+    float* k_smem = chunks + (chunk & 1) * chunk_floats;
+    float* v_smem = k_smem + kChunk * key_row;
+    const int pieces = D / kEach;
+    for (int i = threadIdx.x; i < kChunk * pieces; i += kPairThreads) {
+      const int j = i / pieces, d = (i - j * pieces) * kEach, key = from + chunk * kChunk + j;
+      const bool there = key < last;
+      const T* from_page = (const T*)p.pages;
+      if (there) from_page += (size_t)page_of(p, table, key / p.page_size) * 2 * plane + ((size_t)kvh * p.page_size + key % p.page_size) * D + d;
+      if constexpr (sizeof(T) == 4) {
+        cp_async_16(k_smem + j * key_row + d, from_page, there);
+        cp_async_16(v_smem + j * D + d, there ? from_page + plane : from_page, there);
+      } else {
+        uint4 k = make_uint4(0, 0, 0, 0), v = k;
+        if (there) k = *reinterpret_cast<const uint4*>(from_page), v = *reinterpret_cast<const uint4*>(from_page + plane);
+        const unsigned k_words[4] = {k.x, k.y, k.z, k.w}, v_words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          k_smem[j * key_row + d + 2 * w] = __uint_as_float(k_words[w] << 16), k_smem[j * key_row + d + 2 * w + 1] = __uint_as_float(k_words[w] & 0xffff0000u);
+          v_smem[j * D + d + 2 * w] = __uint_as_float(v_words[w] << 16), v_smem[j * D + d + 2 * w + 1] = __uint_as_float(v_words[w] & 0xffff0000u);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  if (chunk_begin < chunk_end) fetch(chunk_begin);
+  for (int i = threadIdx.x; i < kPairs * D; i += kPairThreads) {
     const int pair = i / D, d = i - pair * D;
     q_smem[i] = pair < pairs ? to_float(((const T*)p.q)[(size_t)row_of(pair) * p.q_row_stride + (size_t)head_of(pair) * D + d]) * p.scale * kToLog2 : 0.0f;
   }
-  int limit[kPairsPerWarp];
-  float top[kPairsPerWarp], sum[kPairsPerWarp], acc[kPairsPerWarp][kDimsPerLane];
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};   // of pairs 2 ty and 2 ty + 1, the same in their eight threads
+  float4 acc[2][kQuads];                                          // channels 4 (tx + 8 c)
 #pragma unroll
-  for (int r = 0; r < kPairsPerWarp; ++r) {
-    const int i = warp * kPairsPerWarp + r;
-    limit[r] = i < pairs ? limit_of(i) : 0;
-    top[r] = -INFINITY;
-    sum[r] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < kDimsPerLane; ++c) acc[r][c] = 0.0f;
-  }
-  const size_t plane = (size_t)p.kv_heads * p.page_size * D;
+  for (int c = 0; c < kQuads; ++c) acc[0][c] = acc[1][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int chunk = chunk_begin; chunk < chunk_end; ++chunk) {
-    const int key0 = from + chunk * kChunk, keys = min(kChunk, last - key0);
-    __syncthreads();
-    for (int j = warp; j < kChunk; j += kPairWarps) {
-      if (j < keys) {
-        const int key = key0 + j, page = page_of(p, table, key / p.page_size);
-        const T* k_row = (const T*)p.pages + (size_t)page * 2 * plane + ((size_t)kvh * p.page_size + key % p.page_size) * D;
-        for (int d = lane; d < D; d += 32) {
-          k_smem[j * key_row + d] = to_float(k_row[d]);
-          v_smem[j * D + d] = to_float(k_row[plane + d]);
-        }
-      } else {
-        for (int d = lane; d < D; d += 32) k_smem[j * key_row + d] = v_smem[j * D + d] = 0.0f;
-      }
+    if (chunk + 1 < chunk_end) {
+      fetch(chunk + 1);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
     }
     __syncthreads();
-    float score[kPairsPerWarp];
+    const float* k_smem = chunks + (chunk & 1) * chunk_floats;
+    const float* v_smem = k_smem + kChunk * key_row;
+    const int key0 = from + chunk * kChunk;
+    float score[2][4];   // pair 2 ty + r, key tx + 8 i
 #pragma unroll
-    for (int r = 0; r < kPairsPerWarp; ++r) score[r] = 0.0f;
+    for (int i = 0; i < 4; ++i) score[0][i] = score[1][i] = 0.0f;
+#pragma unroll 4
     for (int d = 0; d < D; d += 4) {
-      const float4 k4 = *reinterpret_cast<const float4*>(k_smem + lane * key_row + d);
+      const float4 q0 = *reinterpret_cast<const float4*>(q_smem + 2 * ty * D + d), q1 = *reinterpret_cast<const float4*>(q_smem + (2 * ty + 1) * D + d);
 #pragma unroll
-      for (int r = 0; r < kPairsPerWarp; ++r) {
-        const float4 q4 = *reinterpret_cast<const float4*>(q_smem + (warp * kPairsPerWarp + r) * D + d);
-        score[r] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, score[r]))));
+      for (int i = 0; i < 4; ++i) {
+        const float4 k = *reinterpret_cast<const float4*>(k_smem + (tx + 8 * i) * key_row + d);
+        dot4(score[0][i], q0, k);
+        dot4(score[1][i], q1, k);
       }
     }
 #pragma unroll
-    for (int r = 0; r < kPairsPerWarp; ++r) {
-      const bool seen = key0 + lane < limit[r];
-      const float s = seen ? score[r] : -INFINITY;
-      const float reference = fmaxf(top[r], warp_max(s));
-      const float base = reference == -INFINITY ? 0.0f : reference;
-      const float shrink = top[r] == -INFINITY ? 0.0f : exp2f(top[r] - base);
-      const float w = seen ? exp2f(s - base) : 0.0f;
+    for (int r = 0; r < 2; ++r) {
+      float here = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (key0 + tx + 8 * i >= limits[r]) score[r][i] = -INFINITY;
+        here = fmaxf(here, score[r][i]);
+      }
+#pragma unroll
+      for (int other = 1; other < 8; other <<= 1) here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, other));
+      const float reference = fmaxf(top[r], here), base = reference == -INFINITY ? 0.0f : reference;
+      const float shrink = exp2f(top[r] - base);
       top[r] = reference;
-      sum[r] = fmaf(sum[r], shrink, warp_sum(w));
+      float more = 0.0f;
 #pragma unroll
-      for (int c = 0; c < kDimsPerLane; ++c) acc[r][c] *= shrink;
-      score[r] = w;
-    }
-    // Only keys that a pair sees are added: what lies in another's later places (it may be no number) must not reach it through a weight of zero.
-#pragma unroll
-    for (int r = 0; r < kPairsPerWarp; ++r) {
-      const int seen = min(keys, limit[r] - key0);
-      for (int j = 0; j < seen; ++j) {
-        const float w = __shfl_sync(0xffffffffu, score[r], j);
-#pragma unroll
-        for (int c = 0; c < kDimsPerLane; ++c)
-          if (lane + 32 * c < D) acc[r][c] = fmaf(w, v_smem[j * D + lane + 32 * c], acc[r][c]);
+      for (int i = 0; i < 4; ++i) {
+        const float w = exp2f(score[r][i] - base);
+        w_smem[(2 * ty + r) * kWeightRow + tx + 8 * i] = w;
+        more += w;
       }
+#pragma unroll
+      for (int other = 1; other < 8; other <<= 1) more += __shfl_xor_sync(0xffffffffu, more, other);
+      sum[r] = fmaf(sum[r], shrink, more);
+#pragma unroll
+      for (int c = 0; c < kQuads; ++c) acc[r][c].x *= shrink, acc[r][c].y *= shrink, acc[r][c].z *= shrink, acc[r][c].w *= shrink;
     }
+    __syncwarp();   // (a pair's weights are its own eight threads')
+    const float* w0_row = w_smem + 2 * ty * kWeightRow;
+    const float* w1_row = w0_row + kWeightRow;
+    if (key0 + kChunk <= lowest) {
+#pragma unroll 2
+      for (int j = 0; j < kChunk; j += 4) {
+        const float4 w0 = *reinterpret_cast<const float4*>(w0_row + j), w1 = *reinterpret_cast<const float4*>(w1_row + j);
+#pragma unroll
+        for (int c = 0; c < kQuads; ++c) {
+          const int d = 4 * (tx + 8 * c);
+          if (d >= D) break;
+          const float4 v0 = *reinterpret_cast<const float4*>(v_smem + j * D + d), v1 = *reinterpret_cast<const float4*>(v_smem + (j + 1) * D + d);
+          const float4 v2 = *reinterpret_cast<const float4*>(v_smem + (j + 2) * D + d), v3 = *reinterpret_cast<const float4*>(v_smem + (j + 3) * D + d);
+          add4(acc[0][c], w0.x, v0), add4(acc[0][c], w0.y, v1), add4(acc[0][c], w0.z, v2), add4(acc[0][c], w0.w, v3);
+          add4(acc[1][c], w1.x, v0), add4(acc[1][c], w1.y, v1), add4(acc[1][c], w1.z, v2), add4(acc[1][c], w1.w, v3);
+        }
+      }
+    } else {
+      // Only keys that a pair sees are added: what lies in another's later places (it may be no number) must not reach it through a weight of zero.
+#pragma unroll 1
+      for (int j = 0; j < kChunk; ++j)
+#pragma unroll
+        for (int c = 0; c < kQuads; ++c) {
+          const int d = 4 * (tx + 8 * c);
+          if (d >= D) break;
+          const float4 v = *reinterpret_cast<const float4*>(v_smem + j * D + d);
+          if (key0 + j < limits[0]) add4(acc[0][c], w0_row[j], v);
+          if (key0 + j < limits[1]) add4(acc[1][c], w1_row[j], v);
+        }
+    }
+    __syncthreads();
   }
   const int parts = p.prefix_parts + p.own_parts;
 #pragma unroll
-  for (int r = 0; r < kPairsPerWarp; ++r) {
-    const int i = warp * kPairsPerWarp + r;
+  for (int r = 0; r < 2; ++r) {
+    const int i = 2 * ty + r;
     if (i >= pairs) break;
     const size_t at = ((size_t)row_of(i) * p.q_heads + head_of(i)) * parts + part;
-    if (lane == 0) p.part_ml[at] = make_float2(top[r], sum[r]);
+    if (tx == 0) p.part_ml[at] = make_float2(top[r], sum[r]);
 #pragma unroll
-    for (int c = 0; c < kDimsPerLane; ++c)
-      if (lane + 32 * c < D) p.part_o[at * D + lane + 32 * c] = acc[r][c];
+    for (int c = 0; c < kQuads; ++c)
+      if (4 * (tx + 8 * c) < D) *reinterpret_cast<float4*>(p.part_o + at * D + 4 * (tx + 8 * c)) = acc[r][c];
   }
 }
 
 // One warp per (row, head): the parts brought together.  A row that sees no key gives zeros.
 template <typename T>
 __global__ void shared_prefix_merge_kernel(SharedPrefixParams p) {
+  constexpr int kPerLane = 2, kDimsPerLane = 8;   // up to 64 parts, 256 channels
   const int lane = threadIdx.x & 31, parts = p.prefix_parts + p.own_parts, D = p.head_dim;
   const long long pair = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const long long row = pair / p.q_heads;
+  grid_dependency_wait();
   if (row < max(0, p.seq_starts[0]) || row >= min(p.rows, p.seq_starts[p.entries])) return;
-  const float2* ml = p.part_ml + pair * parts;
-  float top = -INFINITY;
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, ml[i].x);
-  float acc[kDimsPerLane] = {0.0f}, sum = 0.0f;
-  for (int i = 0; i < parts; ++i) {
-    const float2 here = ml[i];
-    const float factor = here.x == -INFINITY ? 0.0f : exp2f(here.x - top);
-    if (here.y == 0.0f) continue;
-    sum = fmaf(factor, here.y, sum);
+  float2 ml[kPerLane];
+  float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int c = 0; c < kDimsPerLane; ++c)
-      if (lane + 32 * c < D) acc[c] = fmaf(factor, p.part_o[((size_t)pair * parts + i) * D + lane + 32 * c], acc[c]);
+  for (int i = 0; i < kPerLane; ++i) {
+    ml[i] = lane + 32 * i < parts ? p.part_ml[pair * parts + lane + 32 * i] : make_float2(-INFINITY, 0.0f);
+    m = fmaxf(m, ml[i].x);
   }
+  m = warp_max(m);
 #pragma unroll
-  for (int c = 0; c < kDimsPerLane; ++c)
-    if (lane + 32 * c < D) ((T*)p.out)[(size_t)pair * D + lane + 32 * c] = from_float<T>(sum == 0.0f ? 0.0f : acc[c] / sum);
+  for (int i = 0; i < kPerLane; ++i) {
+    ml[i].x = ml[i].x == -INFINITY ? (ml[i].y == 0.0f ? 0.0f : 1.0f) : exp2f(ml[i].x - m);   // (a part of nothing but NaN keeps its NaN)
+    if (ml[i].x != 0.0f) l = fmaf(ml[i].x, ml[i].y, l);
+  }
+  l = warp_sum(l);
+  float acc[kDimsPerLane] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i)
+#pragma unroll 4
+    for (int c = 0; c < min(32, parts - 32 * i); ++c) {
+      const float factor = __shfl_sync(0xffffffffu, ml[i].x, c);
+      if (factor == 0.0f) continue;
+      const float* part = p.part_o + ((size_t)pair * parts + 32 * i + c) * D;
+#pragma unroll
+      for (int e = 0; e < kDimsPerLane; ++e)
+        if (lane + 32 * e < D) acc[e] = fmaf(factor, part[lane + 32 * e], acc[e]);
+    }
+#pragma unroll
+  for (int e = 0; e < kDimsPerLane; ++e)
+    if (lane + 32 * e < D) ((T*)p.out)[(size_t)pair * D + lane + 32 * e] = from_float<T>(l == 0.0f ? 0.0f : acc[e] / l);
 }
 
-template <typename T>
+template <typename T, int MAX_DIM>
 static int launch_generic(const SharedPrefixParams& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> devices{0};
-  const size_t smem = sizeof(float) * (size_t)(kPairs * p.head_dim + kChunk * (p.head_dim + 4) + kChunk * p.head_dim);
-  cudaError_t e = allow_shared_memory(shared_prefix_generic_kernel<T>, (int)(sizeof(float) * (kPairs * 256 + kChunk * 260 + kChunk * 256)), devices);
+  auto bytes = [](int dim) { return (int)sizeof(float) * (kPairs * dim + kPairs * (kChunk + 4) + 2 * (kChunk * (dim + 4) + kChunk * dim)); };
+  cudaError_t e = allow_shared_memory(shared_prefix_generic_kernel<T, MAX_DIM>, bytes(MAX_DIM), devices);
   if (e != cudaSuccess) return (int)e;
   const int group = p.q_heads / p.kv_heads;
   const long long tiles = ((long long)p.rows * group + kPairs - 1) / kPairs, own_tiles = tiles + p.entries;
   const long long pairs = (long long)p.rows * p.q_heads;
   if (own_tiles > 0x7fffffffLL || (pairs + 7) / 8 > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  shared_prefix_generic_kernel<T><<<dim3((unsigned)own_tiles, p.kv_heads, p.prefix_parts + p.own_parts), kPairWarps * 32, smem, stream>>>(p, (int)own_tiles);
-  e = cudaGetLastError();
+  e = launch_pdl(shared_prefix_generic_kernel<T, MAX_DIM>, dim3((unsigned)own_tiles, p.kv_heads, p.prefix_parts + p.own_parts), dim3(kPairThreads), (size_t)bytes(p.head_dim), stream, p,
+                 (int)own_tiles);
   if (e != cudaSuccess) return (int)e;
-  shared_prefix_merge_kernel<T><<<(unsigned)((pairs + 7) / 8), 256, 0, stream>>>(p);
-  return (int)cudaGetLastError();
+  return (int)launch_pdl(shared_prefix_merge_kernel<T>, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, stream, p);
+}
+template <typename T>
+static int launch_generic(const SharedPrefixParams& p, cudaStream_t stream) {
+  return p.head_dim <= 64 ? launch_generic<T, 64>(p, stream) : p.head_dim <= 128 ? launch_generic<T, 128>(p, stream) : launch_generic<T, 256>(p, stream);
 }
 
 }  // namespace tlie
 
 using namespace tlie;
 
-// q: rows [rows, q_row_stride] that start with the (rotated) query heads.  pages: one layer's pool [num_pages, 2, kv_heads, page_size, head_dim].  out: [rows,
+// q: rows [rows, q_row_stride] that start with the (rotated) query heads.  pages: one layer's pool [num_pages, 2, kv_heads, page_size, head_dim], 16-byte aligned.  out: [rows,
 // q_heads * head_dim]; rows outside [seq_starts[0], seq_starts[entries]) are left as they are.  scratch: rows * q_heads * (prefix_parts + own_parts) *
-// (head_dim + 2) floats, 8-byte aligned.
+// (head_dim + 2) floats, 16-byte aligned.
 TLIE_EXPORT int tlie_shared_prefix_generic(int dtype, const void* q, long long q_row_stride, const void* pages, int num_pages, const int* positions, const int* seq_starts,
                                            const int* block_table, int table_stride, void* out, float* scratch, int rows, int entries, int q_heads, int kv_heads,
                                            int head_dim, int page_size, int shared, float scale, int prefix_parts, int own_parts, int* error_flag, cudaStream_t stream) {
   if (rows <= 0 || entries <= 0) return 0;
-  if (head_dim <= 0 || head_dim > 256 || head_dim % 4 != 0 || kv_heads <= 0 || kv_heads > 65535 || q_heads % kv_heads != 0 || page_size <= 0 || num_pages <= 0 ||
-      prefix_parts < 0 || own_parts < 1 || prefix_parts + own_parts > 65535 || (prefix_parts == 0 && shared > 0) || error_flag == nullptr)
+  if (head_dim <= 0 || head_dim > 256 || head_dim % 16 != 0 || kv_heads <= 0 || kv_heads > 65535 || q_heads % kv_heads != 0 || page_size <= 0 || num_pages <= 0 ||
+      prefix_parts < 0 || own_parts < 1 || prefix_parts + own_parts > 64 || (prefix_parts == 0 && shared > 0) || error_flag == nullptr || ((uintptr_t)pages & 15) ||
+      ((uintptr_t)scratch & 15))
     return (int)cudaErrorInvalidValue;
   const size_t parts = (size_t)rows * q_heads * (prefix_parts + own_parts);
-  SharedPrefixParams p{q, q_row_stride, pages, num_pages, positions, seq_starts, block_table, table_stride, out, scratch + 2 * parts, (float2*)scratch,
+  SharedPrefixParams p{q, q_row_stride, pages, num_pages, positions, seq_starts, block_table, table_stride, out, scratch, (float2*)(scratch + parts * head_dim),
                        rows, entries, q_heads, kv_heads, head_dim, page_size, shared, scale, prefix_parts, own_parts, error_flag};
   return dtype == TLIE_F32 ? launch_generic<float>(p, stream) : launch_generic<__nv_bfloat16>(p, stream);
 }

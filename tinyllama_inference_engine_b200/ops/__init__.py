@@ -710,6 +710,8 @@ def _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared
         raise KernelError("shared_prefix_attention: positions, seq_starts and the block table are int32", code="invalid_dtype")
     if not all(t.is_contiguous() for t in (pages, positions, seq_starts, block_table, out)):
         raise KernelError("kernels take contiguous tensors")
+    if pages.data_ptr() % 16 != 0:
+        raise KernelError("shared_prefix_attention: pages must start on a 16-byte boundary", code="invalid_argument")
     _one_device("shared_prefix_attention", qkv=qkv, pages=pages, positions=positions, seq_starts=seq_starts, block_table=block_table, out=out)
     raise KernelError("shared_prefix_attention: the arguments do not fit each other", code="invalid_argument")
 
@@ -738,7 +740,7 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
             and 0 < head_dim <= 256 and head_dim % 16 == 0 and 0 < kv_heads <= q_heads and q_heads % kv_heads == 0 and width >= q_heads * head_dim
             and out.shape == (rows, q_heads * head_dim) and pages.shape[1:] == (2, kv_heads, page_size, head_dim) and pages.shape[0] > 0
             and positions.shape == (rows,) and seq_starts.shape == (entries + 1,) and type(shared) is int and 0 <= shared <= table_width * page_size
-            and 0.0 < scale < float("inf") and (qkv.stride(1) == 1 or rows == 0) and pages.is_contiguous() and out.is_contiguous()
+            and 0.0 < scale < float("inf") and (qkv.stride(1) == 1 or rows == 0) and pages.is_contiguous() and pages.data_ptr() % 16 == 0 and out.is_contiguous()
             and positions.is_contiguous() and seq_starts.is_contiguous() and block_table.is_contiguous()):
         _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
     if rows == 0 or entries == 0:
@@ -747,8 +749,8 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
         if fast.shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale):
             return
         tiles = -(-rows * (q_heads // kv_heads) // 32) * kv_heads
-        prefix_parts = 0 if shared == 0 else max(1, min(-(-4 * fast.sm_count() // tiles), -(-shared // 128), 64))
-        own_parts = max(1, min(2 * fast.sm_count() // (tiles + entries * kv_heads), -(-(block_table.shape[1] * page_size - shared) // 256), 16))
+        prefix_parts = 0 if shared == 0 else max(1, min(4 * fast.sm_count() // tiles, -(-shared // 32), 48))
+        own_parts = max(1, min(2 * fast.sm_count() // (tiles + entries * kv_heads), -(-(table_width * page_size - shared) // 64), 16))
         buffer = torch.empty(rows * q_heads * (prefix_parts + own_parts) * (head_dim + 2), dtype=torch.float32, device=device)
         _check(
             shared_prefix().tlie_shared_prefix_generic(
