@@ -56,12 +56,12 @@ __device__ __forceinline__ void add4(float4& acc, float w, float4 v) {
 
 // MAX_DIM: 64, 128 or 256, the head size rounded up.
 template <typename T, int MAX_DIM>
-__global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(SharedPrefixParams p, int own_tiles) {
+__global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(SharedPrefixParams p, int tiles_of_all) {
   extern __shared__ __align__(16) float smem[];
   constexpr int kQuads = MAX_DIM / 32;         // four channels each, of this thread's share of a value
-  const int D = p.head_dim, key_row = D + 4;   // four floats more: eight threads that read 16 bytes of their keys' rows touch all banks
-  float* q_smem = smem;                        // [pairs][D]
-  float* w_smem = q_smem + kPairs * D;         // [pairs][keys + 4]
+  const int D = p.head_dim, key_row = D + 4;   // four floats more: threads that read 16 bytes of eight keys' rows, or of every other of eight queries', touch different banks
+  float* q_smem = smem;                        // [pairs][D + 4]
+  float* w_smem = q_smem + kPairs * key_row;   // [pairs][keys + 4]
   constexpr int kWeightRow = kChunk + 4;
   float* chunks = w_smem + kPairs * kWeightRow;   // twice [keys][D + 4] of keys and [keys][D] of values
   const int chunk_floats = kChunk * key_row + kChunk * D;
@@ -69,19 +69,20 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
   const int kvh = blockIdx.y, group = p.q_heads / p.kv_heads;
   grid_dependency_wait();
   const int first_row = max(0, p.seq_starts[0]), end_row = min(p.seq_starts[p.entries], p.rows);
-  const bool of_prefix = (int)blockIdx.z < p.prefix_parts;
-  const int part = blockIdx.z;
+  // the prefix's parts, `tiles_of_all` CTAs each, then those of the entries' own keys with a CTA more per entry
+  const bool of_prefix = blockIdx.x < (unsigned)tiles_of_all * p.prefix_parts;
+  const unsigned number = of_prefix ? blockIdx.x : blockIdx.x - (unsigned)tiles_of_all * p.prefix_parts, tiles_here = of_prefix ? tiles_of_all : tiles_of_all + p.entries;
+  const int which = (int)(number / tiles_here), tile = (int)(number % tiles_here), part = of_prefix ? which : p.prefix_parts + which;
 
   // which pairs: consecutive ones of all rows, or of one entry's rows
   int row0 = 0, pairs = 0, entry = 0;
-  long long pair0 = (long long)blockIdx.x * kPairs;
+  long long pair0 = (long long)tile * kPairs;
   if (of_prefix) {
     const long long all = (long long)(end_row - first_row) * group;
     if (pair0 >= all) return;
     row0 = first_row;
     pairs = (int)min((long long)kPairs, all - pair0);
   } else {   // the entry that this tile number falls to, counting every entry's tiles: 32 entries at a time
-    if ((int)blockIdx.x >= own_tiles) return;
     int tiles_before = 0;
     for (int e0 = 0; e0 < p.entries; e0 += 32) {
       const int e = e0 + lane;
@@ -97,14 +98,14 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
         const int other = __shfl_up_sync(0xffffffffu, upto, offset);
         if (lane >= offset) upto += other;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, tiles_before + upto > (int)blockIdx.x);
+      const unsigned past = __ballot_sync(0xffffffffu, tiles_before + upto > tile);
       if (past != 0u) {
         const int at = __ffs(past) - 1;
         entry = e0 + at;
         const int before = tiles_before + __shfl_sync(0xffffffffu, upto - tiles, at);
         row0 = __shfl_sync(0xffffffffu, begin, at);
         const int rows_here = __shfl_sync(0xffffffffu, end, at) - row0;
-        pair0 = (long long)((int)blockIdx.x - before) * kPairs;
+        pair0 = (long long)(tile - before) * kPairs;
         pairs = (int)min((long long)kPairs, (long long)rows_here * group - pair0);
         break;
       }
@@ -112,16 +113,17 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
     }
     if (pairs <= 0) return;
   }
-  // pair i of the tile: row and head
-  auto row_of = [&](int i) { return row0 + (int)((pair0 + i) / group); };
-  auto head_of = [&](int i) { return kvh * group + (int)((pair0 + i) % group); };
+  // pair i of the tile: row and head, in lane i; `at` is the pair's place among all pairs of a row and a query head
+  const int before_first = (int)(pair0 % group) + lane;
+  const int row = row0 + (int)(pair0 / group) + before_first / group, head = kvh * group + before_first % group;
+  const long long at_lane = (long long)row * p.q_heads + head;
 
   const int* table = p.block_table + (size_t)entry * p.table_stride;
   const long long room = (long long)p.table_stride * p.page_size;
   // keys a pair sees in this kind of part: below the result; lane i has pair i's
   int limit = 0;
   if (lane < pairs) {
-    long long seen = (long long)p.positions[row_of(lane)] + 1;
+    long long seen = (long long)p.positions[row] + 1;
     if (seen > room) {
       if (threadIdx.x < 32) atomicOr(p.error_flag, kBadPage);
       seen = room;
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
   const int lowest = __reduce_min_sync(0xffffffffu, lane < pairs ? limit : 0x7fffffff);
   const int from = of_prefix ? 0 : p.shared;
   const int all_chunks = last > from ? (last - from + kChunk - 1) / kChunk : 0;
-  const int parts_here = of_prefix ? p.prefix_parts : p.own_parts, which = of_prefix ? part : part - p.prefix_parts;
+  const int parts_here = of_prefix ? p.prefix_parts : p.own_parts;
   const int chunk_begin = (int)((long long)all_chunks * which / parts_here), chunk_end = (int)((long long)all_chunks * (which + 1) / parts_here);
 
   const size_t plane = (size_t)p.kv_heads * p.page_size * D;
@@ -142,12 +144,13 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
     constexpr int kEach = 16 / (int)sizeof(T);
     float* k_smem = chunks + (chunk & 1) * chunk_floats;
     float* v_smem = k_smem + kChunk * key_row;
-    const int pieces = D / kEach;
-    for (int i = threadIdx.x; i < kChunk * pieces; i += kPairThreads) {
-      const int j = i / pieces, d = (i - j * pieces) * kEach, key = from + chunk * kChunk + j;
-      const bool there = key < last;
-      const T* from_page = (const T*)p.pages;
-      if (there) from_page += (size_t)page_of(p, table, key / p.page_size) * 2 * plane + ((size_t)kvh * p.page_size + key % p.page_size) * D + d;
+    const int j = threadIdx.x >> 2, key = from + chunk * kChunk + j;   // four threads a key
+    const bool there = key < last;
+    const T* token = (const T*)p.pages;
+    if (there) token += (size_t)page_of(p, table, key / p.page_size) * 2 * plane + ((size_t)kvh * p.page_size + key % p.page_size) * D;
+#pragma unroll 4
+    for (int d = (threadIdx.x & 3) * kEach; d < D; d += 4 * kEach) {
+      const T* from_page = there ? token + d : token;
       if constexpr (sizeof(T) == 4) {
         cp_async_16(k_smem + j * key_row + d, from_page, there);
         cp_async_16(v_smem + j * D + d, there ? from_page + plane : from_page, there);
@@ -165,9 +168,14 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
     cp_async_commit();
   };
   if (chunk_begin < chunk_end) fetch(chunk_begin);
-  for (int i = threadIdx.x; i < kPairs * D; i += kPairThreads) {
-    const int pair = i / D, d = i - pair * D;
-    q_smem[i] = pair < pairs ? to_float(((const T*)p.q)[(size_t)row_of(pair) * p.q_row_stride + (size_t)head_of(pair) * D + d]) * p.scale * kToLog2 : 0.0f;
+  const long long q_lane = (long long)row * p.q_row_stride + (long long)head * D;
+#pragma unroll
+  for (int i = 0; i < kPairs / 4; ++i) {   // a warp brings eight queries
+    const int pair = (threadIdx.x >> 5) * (kPairs / 4) + i;
+    const T* q = (const T*)p.q + __shfl_sync(0xffffffffu, q_lane, pair);
+#pragma unroll
+    for (int d = 0; d < MAX_DIM; d += 32)
+      if (d + lane < D) q_smem[pair * key_row + d + lane] = pair < pairs ? to_float(q[d + lane]) * p.scale * kToLog2 : 0.0f;
   }
   float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};   // of pairs 2 ty and 2 ty + 1, the same in their eight threads
   float4 acc[2][kQuads];                                          // channels 4 (tx + 8 c)
@@ -189,7 +197,7 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
     for (int i = 0; i < 4; ++i) score[0][i] = score[1][i] = 0.0f;
 #pragma unroll 4
     for (int d = 0; d < D; d += 4) {
-      const float4 q0 = *reinterpret_cast<const float4*>(q_smem + 2 * ty * D + d), q1 = *reinterpret_cast<const float4*>(q_smem + (2 * ty + 1) * D + d);
+      const float4 q0 = *reinterpret_cast<const float4*>(q_smem + 2 * ty * key_row + d), q1 = *reinterpret_cast<const float4*>(q_smem + (2 * ty + 1) * key_row + d);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float4 k = *reinterpret_cast<const float4*>(k_smem + (tx + 8 * i) * key_row + d);
@@ -259,8 +267,8 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int i = 2 * ty + r;
-    if (i >= pairs) break;
-    const size_t at = ((size_t)row_of(i) * p.q_heads + head_of(i)) * parts + part;
+    const size_t at = (size_t)__shfl_sync(0xffffffffu, at_lane, i) * parts + part;
+    if (i >= pairs) continue;
     if (tx == 0) p.part_ml[at] = make_float2(top[r], sum[r]);
 #pragma unroll
     for (int c = 0; c < kQuads; ++c)
@@ -268,60 +276,80 @@ __global__ void __launch_bounds__(kPairThreads) shared_prefix_generic_kernel(Sha
   }
 }
 
-// One warp per (row, head): the parts brought together.  A row that sees no key gives zeros.
+// One CTA per (row, head): the parts brought together.  A thread has four channels of every so many-th part, four parts' loads in flight; a row that sees no
+// key gives zeros.
+constexpr int kMergeThreads = 128;
 template <typename T>
-__global__ void shared_prefix_merge_kernel(SharedPrefixParams p) {
-  constexpr int kPerLane = 2, kDimsPerLane = 8;   // up to 64 parts, 256 channels
-  const int lane = threadIdx.x & 31, parts = p.prefix_parts + p.own_parts, D = p.head_dim;
-  const long long pair = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const long long row = pair / p.q_heads;
+__global__ void __launch_bounds__(kMergeThreads) shared_prefix_merge_kernel(SharedPrefixParams p) {
+  __shared__ float factors[64];                  // 64 parts at most
+  __shared__ float4 sums[kMergeThreads];
+  __shared__ float all;
+  const int parts = p.prefix_parts + p.own_parts, quads = p.head_dim / 4, slots = kMergeThreads / quads;
+  const int slot = threadIdx.x / quads, quad = threadIdx.x - slot * quads;
+  const long long pair = blockIdx.x, row = pair / p.q_heads;
   grid_dependency_wait();
   if (row < max(0, p.seq_starts[0]) || row >= min(p.rows, p.seq_starts[p.entries])) return;
-  float2 ml[kPerLane];
-  float m = -INFINITY, l = 0.0f;
+  const float4* part_o = reinterpret_cast<const float4*>(p.part_o) + pair * parts * quads + quad;
+  auto load = [&](int c) { return slot < slots && c < parts ? part_o[(size_t)c * quads] : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
+  float4 first[4];
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    ml[i] = lane + 32 * i < parts ? p.part_ml[pair * parts + lane + 32 * i] : make_float2(-INFINITY, 0.0f);
-    m = fmaxf(m, ml[i].x);
-  }
-  m = warp_max(m);
+  for (int i = 0; i < 4; ++i) first[i] = load(slot + i * slots);
+  if (threadIdx.x < 32) {
+    float2 ml[2];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    ml[i].x = ml[i].x == -INFINITY ? (ml[i].y == 0.0f ? 0.0f : 1.0f) : exp2f(ml[i].x - m);   // (a part of nothing but NaN keeps its NaN)
-    if (ml[i].x != 0.0f) l = fmaf(ml[i].x, ml[i].y, l);
-  }
-  l = warp_sum(l);
-  float acc[kDimsPerLane] = {0.0f};
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i)
-#pragma unroll 4
-    for (int c = 0; c < min(32, parts - 32 * i); ++c) {
-      const float factor = __shfl_sync(0xffffffffu, ml[i].x, c);
-      if (factor == 0.0f) continue;
-      const float* part = p.part_o + ((size_t)pair * parts + 32 * i + c) * D;
-#pragma unroll
-      for (int e = 0; e < kDimsPerLane; ++e)
-        if (lane + 32 * e < D) acc[e] = fmaf(factor, part[lane + 32 * e], acc[e]);
+    for (int i = 0; i < 2; ++i) {
+      const int c = threadIdx.x + 32 * i;
+      ml[i] = c < parts ? p.part_ml[pair * parts + c] : make_float2(-INFINITY, 0.0f);
+      m = fmaxf(m, ml[i].x);
     }
+    m = warp_max(m);
 #pragma unroll
-  for (int e = 0; e < kDimsPerLane; ++e)
-    if (lane + 32 * e < D) ((T*)p.out)[(size_t)pair * D + lane + 32 * e] = from_float<T>(l == 0.0f ? 0.0f : acc[e] / l);
+    for (int i = 0; i < 2; ++i) {
+      const float factor = ml[i].x == -INFINITY ? (ml[i].y == 0.0f ? 0.0f : 1.0f) : exp2f(ml[i].x - m);   // (a part of nothing but NaN keeps its NaN)
+      if (factor != 0.0f) l = fmaf(factor, ml[i].y, l);
+      factors[threadIdx.x + 32 * i] = factor;
+    }
+    l = warp_sum(l);
+    if (threadIdx.x == 0) all = l;
+  }
+  __syncthreads();
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (slot + i * slots < parts) add4(acc, factors[slot + i * slots], first[i]);
+  for (int c = slot + 4 * slots; c < parts; c += 4 * slots) {
+    float4 next[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) next[i] = load(c + i * slots);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i * slots < parts) add4(acc, factors[c + i * slots], next[i]);
+  }
+  sums[threadIdx.x] = acc;
+  __syncthreads();
+  if (threadIdx.x < quads) {
+    for (int i = 1; i < slots; ++i) add4(acc, 1.0f, sums[i * quads + threadIdx.x]);
+    T* out = (T*)p.out + (size_t)pair * p.head_dim + 4 * threadIdx.x;
+    const float l = all;
+    out[0] = from_float<T>(l == 0.0f ? 0.0f : acc.x / l), out[1] = from_float<T>(l == 0.0f ? 0.0f : acc.y / l);
+    out[2] = from_float<T>(l == 0.0f ? 0.0f : acc.z / l), out[3] = from_float<T>(l == 0.0f ? 0.0f : acc.w / l);
+  }
 }
 
 template <typename T, int MAX_DIM>
 static int launch_generic(const SharedPrefixParams& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> devices{0};
-  auto bytes = [](int dim) { return (int)sizeof(float) * (kPairs * dim + kPairs * (kChunk + 4) + 2 * (kChunk * (dim + 4) + kChunk * dim)); };
+  auto bytes = [](int dim) { return (int)sizeof(float) * (kPairs * (dim + 4) + kPairs * (kChunk + 4) + 2 * (kChunk * (dim + 4) + kChunk * dim)); };
   cudaError_t e = allow_shared_memory(shared_prefix_generic_kernel<T, MAX_DIM>, bytes(MAX_DIM), devices);
   if (e != cudaSuccess) return (int)e;
   const int group = p.q_heads / p.kv_heads;
-  const long long tiles = ((long long)p.rows * group + kPairs - 1) / kPairs, own_tiles = tiles + p.entries;
+  const long long tiles = ((long long)p.rows * group + kPairs - 1) / kPairs, ctas = tiles * p.prefix_parts + (tiles + p.entries) * p.own_parts;
   const long long pairs = (long long)p.rows * p.q_heads;
-  if (own_tiles > 0x7fffffffLL || (pairs + 7) / 8 > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  e = launch_pdl(shared_prefix_generic_kernel<T, MAX_DIM>, dim3((unsigned)own_tiles, p.kv_heads, p.prefix_parts + p.own_parts), dim3(kPairThreads), (size_t)bytes(p.head_dim), stream, p,
-                 (int)own_tiles);
+  if (ctas > 0x7fffffffLL || pairs > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  e = launch_pdl(shared_prefix_generic_kernel<T, MAX_DIM>, dim3((unsigned)ctas, p.kv_heads), dim3(kPairThreads), (size_t)bytes(p.head_dim), stream, p, (int)tiles);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(shared_prefix_merge_kernel<T>, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, stream, p);
+  return (int)launch_pdl(shared_prefix_merge_kernel<T>, dim3((unsigned)pairs), dim3(kMergeThreads), 0, stream, p);
 }
 template <typename T>
 static int launch_generic(const SharedPrefixParams& p, cudaStream_t stream) {

@@ -748,9 +748,7 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     with _on(device):
         if fast.shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale):
             return
-        tiles = -(-rows * (q_heads // kv_heads) // 32) * kv_heads
-        prefix_parts = 0 if shared == 0 else max(1, min(4 * fast.sm_count() // tiles, -(-shared // 32), 48))
-        own_parts = max(1, min(2 * fast.sm_count() // (tiles + entries * kv_heads), -(-(table_width * page_size - shared) // 64), 16))
+        prefix_parts, own_parts = fast.generic_prefix_parts(rows, entries, q_heads // kv_heads, kv_heads, head_dim, shared, table_width * page_size - shared)
         buffer = torch.empty(rows * q_heads * (prefix_parts + own_parts) * (head_dim + 2), dtype=torch.float32, device=device)
         _check(
             shared_prefix().tlie_shared_prefix_generic(

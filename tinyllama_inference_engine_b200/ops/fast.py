@@ -1240,6 +1240,20 @@ def prefix_tc_parts(rows: int, kv_heads: int, group: int, head_dim: int, shared:
 
 
 @functools.lru_cache(maxsize=4096)
+def generic_prefix_parts(rows: int, entries: int, group: int, kv_heads: int, head_dim: int, shared: int, own: int) -> tuple[int, int]:
+    """Runs of the shared keys and of an entry's own ones in the general kernel: the shortest that one CTA each still has room on the GPU at once, 32 keys at least.
+
+    (A CTA holds 45, 88 or 170 KB of shared memory for head sizes up to 64, 128 and 256.)"""
+    room = sm_count() * (4 if head_dim <= 64 else 2 if head_dim <= 128 else 1)
+    tiles, keys = -(-rows * group // 32), 32 * max(1, -(-shared // (48 * 32)), -(-own // (16 * 32)))
+    while True:
+        prefix_parts, own_parts = -(-shared // keys), max(1, -(-own // keys))
+        if kv_heads * (tiles * prefix_parts + max(tiles, entries) * own_parts) <= room or prefix_parts <= 1 and own_parts == 1:
+            return prefix_parts, own_parts
+        keys += 32 * max(1, keys // 256)
+
+
+@functools.lru_cache(maxsize=4096)
 def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_heads: int, head_dim: int, page_size: int, shared: int) -> tuple:
     """Which kernels a call of these sizes runs: (prefix, own, parts, CTAs per row and head, floats of scratch memory)."""
     group = q_heads // kv_heads
