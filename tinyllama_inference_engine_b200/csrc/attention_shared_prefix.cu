@@ -382,12 +382,15 @@ extern "C" int tlie_prefix_tc(int, const void*, long long, const void*, int, con
 extern "C" int tlie_prefix_rows(const void*, long long, const void*, int, const int*, const int*, const int*, int, void*, const float*, const float*, int, int, int, int, int, int, int, int,
                                 float, int, int*, cudaStream_t);
 
-// The bfloat16 kernels for head sizes 64 and 128 (each checks what it takes).  prefix: 0, every row reads the shared keys for itself; 1, the prefix's parts come
-// from the tensor cores, `parts` runs of them.  own: 0, a row at a time (`ctas` per row and head), 1, an entry's rows on the tensor cores.
-// scratch: rows * q_heads * parts * (head_dim + 2) floats, 16-byte aligned.
-TLIE_EXPORT int tlie_shared_prefix_bf16(int prefix, int own, int parts, int ctas, const void* q, long long q_row_stride, const void* pages, int num_pages, const int* positions,
-                                        const int* seq_starts, const int* block_table, int table_stride, void* out, float* scratch, int rows, int entries, int q_heads, int kv_heads,
-                                        int head_dim, int page_size, int shared, float scale, int* error_flag, cudaStream_t stream) {
+// The bfloat16 kernels for head sizes 64 and 128 (each checks what it takes).  sizes, 12 numbers: prefix (0, every row reads the shared keys for itself; 1, the prefix's
+// parts come from the tensor cores, `parts` runs of them), own (0, a row at a time, `ctas` per row and head; 1, an entry's rows on the tensor cores), parts, ctas, rows, entries, pages
+// of a table row, q_heads, kv_heads, head_dim, page_size, shared.  scratch: rows * q_heads * parts * (head_dim + 2) floats, 16-byte aligned.
+TLIE_EXPORT int tlie_shared_prefix_bf16(const int* sizes, const void* q, long long q_row_stride, const void* pages, int num_pages, const int* positions, const int* seq_starts,
+                                        const int* block_table, void* out, float* scratch, float scale, int* error_flag, cudaStream_t stream) {
+  if (sizes == nullptr) return (int)cudaErrorInvalidValue;
+  const int prefix = sizes[0], own = sizes[1], ctas = sizes[3], rows = sizes[4], entries = sizes[5], table_stride = sizes[6], q_heads = sizes[7], kv_heads = sizes[8];
+  const int head_dim = sizes[9], page_size = sizes[10], shared = sizes[11];
+  int parts = sizes[2];
   float *part_o = nullptr, *part_ml = nullptr;
   int first_key = 0, status = 0;
   if (prefix != 0) {

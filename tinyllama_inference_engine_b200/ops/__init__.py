@@ -11,6 +11,7 @@ tensor-core kernel covers the shape; the 32-bit path always uses the engine's ow
 from __future__ import annotations
 
 import ctypes
+import functools
 from contextlib import nullcontext
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
@@ -108,6 +109,9 @@ DEVICE_ERRORS = {1: "a bounded wait inside a tensor-core kernel gave up; the ste
 
 def error_flag(device: torch.device) -> torch.Tensor:
     """The device's error word (int32 [1]); kernels set bits in it, ``raise_for_error_word`` names and clears them."""
+    found = _error_flags.get(device)   # (a device that was asked for before; a name is made one below)
+    if found is not None:
+        return found
     device = torch.device(device)
     if device not in _error_flags:
         _error_flags[device] = torch.zeros(1, dtype=torch.int32, device=device)
@@ -680,9 +684,13 @@ def _one_device(what: str, **tensors) -> torch.device:
     return devices.pop()
 
 
+def _current_device() -> int:
+    return torch.cuda.current_device() if _device_index is None else _device_index()
+
+
 def _on(device: torch.device):
     """Launches inside go to this device, whichever is the current one."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return nullcontext() if device.index == _current_device() else torch.cuda.device(device)
 
 
 def _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale) -> None:
@@ -728,33 +736,35 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     the device's error word.  ``scale``: positive, ``head_dim ** -0.5`` by default.  32-bit or bfloat16, head sizes that are multiples of 16 up to 256.
 
     Called inside the capture of a CUDA graph, the graph keeps ``shared`` and the tensors' addresses; what the tensors hold may change from replay to replay."""
-    if qkv.dim() != 2 or block_table.dim() != 2:
-        _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
-    rows, width = qkv.shape
-    entries, table_width = block_table.shape
     scale = head_dim ** -0.5 if scale is None else float(scale)
-    device, dtype = qkv.device, qkv.dtype
-    if not (device.type == "cuda" and (dtype is torch.bfloat16 or dtype is torch.float32) and pages.dtype is dtype and out.dtype is dtype
+    index, dtype = qkv.get_device(), qkv.dtype   # (a tensor that is not on a CUDA device is on -1)
+    if index < 0 or qkv.dim() != 2 or block_table.dim() != 2 or pages.dim() != 5:
+        _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
+    (rows, width), (q_stride, q_step), (entries, table_width) = qkv.shape, qkv.stride(), block_table.shape
+    num_pages, two, page_heads, page_keys, page_dim = pages.shape
+    if not ((dtype is torch.bfloat16 or dtype is torch.float32) and pages.dtype is dtype and out.dtype is dtype
             and positions.dtype is torch.int32 and seq_starts.dtype is torch.int32 and block_table.dtype is torch.int32
-            and pages.device == device and out.device == device and positions.device == device and seq_starts.device == device and block_table.device == device
+            and index == pages.get_device() == out.get_device() == positions.get_device() == seq_starts.get_device() == block_table.get_device()
             and 0 < head_dim <= 256 and head_dim % 16 == 0 and 0 < kv_heads <= q_heads and q_heads % kv_heads == 0 and width >= q_heads * head_dim
-            and out.shape == (rows, q_heads * head_dim) and pages.shape[1:] == (2, kv_heads, page_size, head_dim) and pages.shape[0] > 0
+            and out.shape == (rows, q_heads * head_dim) and num_pages > 0 and two == 2 and page_heads == kv_heads and page_keys == page_size and page_dim == head_dim
             and positions.shape == (rows,) and seq_starts.shape == (entries + 1,) and type(shared) is int and 0 <= shared <= table_width * page_size
-            and 0.0 < scale < float("inf") and (qkv.stride(1) == 1 or rows == 0) and pages.is_contiguous() and pages.data_ptr() % 16 == 0 and out.is_contiguous()
+            and 0.0 < scale < float("inf") and (q_step == 1 or rows == 0) and pages.is_contiguous() and pages.data_ptr() % 16 == 0 and out.is_contiguous()
             and positions.is_contiguous() and seq_starts.is_contiguous() and block_table.is_contiguous()):
         _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
     if rows == 0 or entries == 0:
         return
-    with _on(device):
-        if fast.shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale):
-            return
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
+    if dtype is not torch.bfloat16 or not fast.shared_prefix_attention(qkv, q_stride, pages, num_pages, positions, seq_starts, block_table, rows, entries, table_width, shared, out,
+                                                                       q_heads, kv_heads, head_dim, page_size, scale):
         prefix_parts, own_parts = fast.generic_prefix_parts(rows, entries, q_heads // kv_heads, kv_heads, head_dim, shared, table_width * page_size - shared)
-        buffer = torch.empty(rows * q_heads * (prefix_parts + own_parts) * (head_dim + 2), dtype=torch.float32, device=device)
+        buffer = torch.empty(rows * q_heads * (prefix_parts + own_parts) * (head_dim + 2), dtype=torch.float32, device=qkv.device)
         _check(
             shared_prefix().tlie_shared_prefix_generic(
-                _code(qkv), c_void_p(qkv.data_ptr()), c_longlong(qkv.stride(0)), _ptr(pages), c_int(pages.shape[0]), _i32(positions, "positions"), _i32(seq_starts, "seq_starts"),
-                _i32(block_table, "block_table"), c_int(block_table.shape[1]), _ptr(out), _ptr(buffer), c_int(rows), c_int(entries), c_int(q_heads), c_int(kv_heads),
-                c_int(head_dim), c_int(page_size), c_int(shared), c_float(scale), c_int(prefix_parts), c_int(own_parts), _ptr(error_flag(device)), _stream(),
+                _code(qkv), c_void_p(qkv.data_ptr()), c_longlong(q_stride), _ptr(pages), c_int(num_pages), _i32(positions, "positions"), _i32(seq_starts, "seq_starts"),
+                _i32(block_table, "block_table"), c_int(table_width), _ptr(out), _ptr(buffer), c_int(rows), c_int(entries), c_int(q_heads), c_int(kv_heads),
+                c_int(head_dim), c_int(page_size), c_int(shared), c_float(scale), c_int(prefix_parts), c_int(own_parts), _ptr(error_flag(qkv.device)), _stream(),
             ),
             "shared_prefix_attention",
         )
@@ -1420,11 +1430,34 @@ def sample(logits, temperature, top_p, seeds, counters, out) -> None:
     )
 
 
+@functools.lru_cache(maxsize=None)
 def filtered_sampling():
-    return load_library("tlie_sample_filtered", SAMPLE_FILTERED_SOURCES)
+    lib = load_library("tlie_sample_filtered", SAMPLE_FILTERED_SOURCES)
+    lib.tlie_sample_filtered.argtypes = [c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    return lib
 
 
 SAMPLE_FILTERED_MAX_VOCAB = 1 << 19    # sums of that many weights of 2^44 and less fit 64 bits (csrc/sample_filtered.cu)
+
+
+def _refuse_sample_filtered(logits, temperature, top_k, top_p, min_p, uniforms, out, rows) -> None:
+    """What of a call of ``sample_filtered`` is wrong."""
+    given = {"logits": logits, "temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p, "uniforms": uniforms, "out": out}
+    if rows is not None:
+        given["rows"] = rows
+    if logits.dtype != torch.float32 or any(t.dtype != torch.float32 for t in (temperature, top_p, min_p, uniforms)):
+        raise KernelError("sampling takes 32-bit logits, temperatures, top_p, min_p and uniform numbers", code="invalid_dtype")
+    if any(t.dtype != torch.int32 for t in (top_k, out, top_k if rows is None else rows)):
+        raise KernelError("sample_filtered: top_k, out and rows are int32", code="invalid_dtype")
+    if logits.dim() != 2 or not 0 < logits.shape[1] <= SAMPLE_FILTERED_MAX_VOCAB or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KernelError(f"sample_filtered: logits must be [rows, 1 to {SAMPLE_FILTERED_MAX_VOCAB} tokens] with contiguous rows", code="invalid_shape")
+    each = (logits.shape[0],) if rows is None else tuple(rows.shape)
+    if len(each) != 1 or any(tuple(t.shape) != each for t in (temperature, top_k, top_p, min_p, uniforms)) or tuple(out.shape) != (logits.shape[0],):
+        raise KernelError("sample_filtered: one temperature, top_k, top_p, min_p and uniform number per row, and out [rows of the logits]", code="invalid_shape")
+    if not all(t.is_contiguous() for name, t in given.items() if name != "logits"):
+        raise KernelError("kernels take contiguous tensors")
+    _one_device("sample_filtered", **given)
+    raise KernelError("sample_filtered: the arguments do not fit each other", code="invalid_argument")
 
 
 def sample_filtered(logits, temperature, top_k, top_p, min_p, uniforms, out, rows=None) -> None:
@@ -1438,30 +1471,26 @@ def sample_filtered(logits, temperature, top_k, top_p, min_p, uniforms, out, row
 
     temperature, top_p, min_p and uniforms are 32-bit floats, top_k int32, one per row.  ``rows`` (int32): the r-th options are for row ``rows[r]`` of
     the logits and of ``out``, each named once; numbers outside the logits (-1, say) are passed over, and rows that nobody names keep what ``out`` holds."""
-    count = logits.shape[0] if rows is None else rows.shape[0]
-    given = {"logits": logits, "temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p, "uniforms": uniforms, "out": out}
-    if rows is not None:
-        given["rows"] = rows
-    vocab = logits.shape[1] if logits.dim() == 2 else 0
-    if logits.dtype != torch.float32 or any(t.dtype != torch.float32 for t in (temperature, top_p, min_p, uniforms)):
-        raise KernelError("sampling takes 32-bit logits, temperatures, top_p, min_p and uniform numbers", code="invalid_dtype")
-    if any(t.dtype != torch.int32 for t in (top_k, out, top_k if rows is None else rows)):
-        raise KernelError("sample_filtered: top_k, out and rows are int32", code="invalid_dtype")
-    if not 0 < vocab <= SAMPLE_FILTERED_MAX_VOCAB or (vocab > 1 and logits.stride(1) != 1):
-        raise KernelError(f"sample_filtered: logits must be [rows, 1 to {SAMPLE_FILTERED_MAX_VOCAB} tokens] with contiguous rows", code="invalid_shape")
-    if any(tuple(t.shape) != (count,) for t in (temperature, top_k, top_p, min_p, uniforms)) or tuple(out.shape) != (logits.shape[0],) or (rows is not None and rows.dim() != 1):
-        raise KernelError("sample_filtered: one temperature, top_k, top_p, min_p and uniform number per row, and out [rows of the logits]", code="invalid_shape")
-    device = _one_device("sample_filtered", **given)
-    if count == 0 or logits.shape[0] == 0:
+    index = logits.get_device()   # (a tensor that is not on a CUDA device is on -1)
+    if index < 0 or logits.dim() != 2 or out.dim() != 1 or (rows is not None and rows.dim() != 1):
+        _refuse_sample_filtered(logits, temperature, top_k, top_p, min_p, uniforms, out, rows)
+    (all_rows, vocab), (stride, step) = logits.shape, logits.stride()
+    each = (all_rows,) if rows is None else rows.shape
+    if not (logits.dtype is torch.float32 and temperature.dtype is torch.float32 and top_p.dtype is torch.float32 and min_p.dtype is torch.float32 and uniforms.dtype is torch.float32
+            and top_k.dtype is torch.int32 and out.dtype is torch.int32 and 0 < vocab <= SAMPLE_FILTERED_MAX_VOCAB and (step == 1 or vocab == 1) and out.shape == (all_rows,)
+            and temperature.shape == each and top_k.shape == each and top_p.shape == each and min_p.shape == each and uniforms.shape == each
+            and index == temperature.get_device() == top_k.get_device() == top_p.get_device() == min_p.get_device() == uniforms.get_device() == out.get_device()
+            and temperature.is_contiguous() and top_k.is_contiguous() and top_p.is_contiguous() and min_p.is_contiguous() and uniforms.is_contiguous() and out.is_contiguous()
+            and (rows is None or (rows.dtype is torch.int32 and rows.get_device() == index and rows.is_contiguous()))):
+        _refuse_sample_filtered(logits, temperature, top_k, top_p, min_p, uniforms, out, rows)
+    if each[0] == 0 or all_rows == 0:
         return
-    with _on(device):
-        _check(
-            filtered_sampling().tlie_sample_filtered(
-                c_void_p(logits.data_ptr()), c_longlong(logits.stride(0)), c_int(logits.shape[0]), c_int(vocab), _i32(rows, "rows"), c_int(count), _ptr(temperature),
-                _i32(top_k, "top_k"), _ptr(top_p), _ptr(min_p), _ptr(uniforms), _i32(out, "out"), _stream(),
-            ),
-            "sample_filtered",
-        )
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return sample_filtered(logits, temperature, top_k, top_p, min_p, uniforms, out, rows)
+    _check(filtered_sampling().tlie_sample_filtered(
+        logits.data_ptr(), stride, all_rows, vocab, None if rows is None else rows.data_ptr(), each[0], temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
+        uniforms.data_ptr(), out.data_ptr(), _stream()), "sample_filtered")
 
 
 def uniforms(seeds, counters, out) -> None:

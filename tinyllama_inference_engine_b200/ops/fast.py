@@ -1204,20 +1204,13 @@ use_prefix = None             # None: by the rule below; 0, 1: every row reads t
 use_own = None                # likewise 0, 1: a row at a time, the tensor cores
 
 
+@functools.lru_cache(maxsize=None)
 def shared_prefix_library():
     """The kernels of attention over a shared prefix; this launcher takes plain Python numbers."""
     lib = _ops().shared_prefix()
-    if not getattr(lib, "_tlie_typed", False):
-        p, i, n = c_void_p, c_int, c_longlong
-        lib.tlie_shared_prefix_bf16.argtypes = [i, i, i, i, p, n, p, i, p, p, p, i, p, p, i, i, i, i, i, i, i, c_float, p, p]
-        lib._tlie_typed = True
+    p, n = c_void_p, c_longlong
+    lib.tlie_shared_prefix_bf16.argtypes = [p, p, n, p, c_int, p, p, p, p, p, c_float, p, p]
     return lib
-
-
-def shared_prefix_takes(qkv, pages, out, page_size: int, head_dim: int, group: int) -> bool:
-    """Whether the bfloat16 kernels for head sizes 64 and 128 can read these tensors: 16 bytes at a time, pages of a multiple of 16 keys, copies by 32-bit rows of the pool."""
-    return (qkv.dtype == torch.bfloat16 and head_dim in SHARED_PREFIX_HEAD_DIMS and page_size % 16 == 0 and group <= PREFIX_TC_PAIRS and qkv.stride(0) % 8 == 0
-            and (qkv.data_ptr() | pages.data_ptr() | out.data_ptr()) % 16 == 0 and pages.numel() // head_dim < 0x7FFFFF00)
 
 
 def prefix_rows_ctas(rows: int, kv_heads: int, group: int, keys: int) -> int:
@@ -1254,15 +1247,20 @@ def generic_prefix_parts(rows: int, entries: int, group: int, kv_heads: int, hea
 
 
 @functools.lru_cache(maxsize=4096)
-def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_heads: int, head_dim: int, page_size: int, shared: int) -> tuple:
-    """Which kernels a call of these sizes runs: (prefix, own, parts, CTAs per row and head, floats of scratch memory)."""
+def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_heads: int, head_dim: int, page_size: int, shared: int) -> tuple | None:
+    """Which kernels a call of these sizes runs: (the launcher's numbers, which start with prefix, own, parts and CTAs per row and head; floats of scratch memory).
+
+    None: sizes that only the general kernel takes."""
     group = q_heads // kv_heads
+    if head_dim not in SHARED_PREFIX_HEAD_DIMS or page_size % 16 != 0 or group > PREFIX_TC_PAIRS:
+        return None
     prefix, own = use_prefix, use_own
     own_keys = width * page_size - shared
+    pieces = rows // (2 * (PREFIX_TC_PAIRS // group))   # of rows that are worked out together; a grid has room for 65,535
     if own is None:
-        own = 1 if rows > 2 * entries else 0
+        own = 1 if rows > 2 * entries and pieces + entries <= 65535 else 0
     parts = 0
-    if shared > 0 and prefix != 0:
+    if shared > 0 and prefix != 0 and pieces < 65535:
         tc_parts, once = prefix_tc_parts(rows, kv_heads, group, head_dim, shared)
         if prefix is None:
             if own:   # an entry's rows fill the row tiles that would share the prefix
@@ -1273,19 +1271,24 @@ def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_hea
     else:
         prefix = 0
     ctas = prefix_rows_ctas(rows, kv_heads, group, own_keys if prefix else width * page_size)
-    return prefix, own, parts, ctas, rows * q_heads * parts * (head_dim + 2)
+    return (c_int * 12)(prefix, own, parts, ctas, rows, entries, width, q_heads, kv_heads, head_dim, page_size, shared), rows * q_heads * parts * (head_dim + 2)
 
 
-def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared: int, out, q_heads: int, kv_heads: int, head_dim: int, page_size: int, scale: float) -> bool:
-    """bfloat16 attention over a shared prefix on the kernels made for it; False if they do not take the call."""
-    if not shared_prefix_takes(qkv, pages, out, page_size, head_dim, q_heads // kv_heads):
+def shared_prefix_attention(qkv, q_stride: int, pages, num_pages: int, positions, seq_starts, block_table, rows: int, entries: int, width: int, shared: int, out, q_heads: int, kv_heads: int,
+                            head_dim: int, page_size: int, scale: float) -> bool:
+    """bfloat16 attention over a shared prefix on the kernels made for it; False if they do not take the call.
+
+    They take head sizes 64 and 128, pages of a multiple of 16 keys, rows that are read 16 bytes at a time, and pools whose rows of keys and values a 32-bit number counts."""
+    q, out_at = qkv.data_ptr(), out.data_ptr()
+    if q_stride % 8 != 0 or (q | out_at) % 16 != 0 or num_pages * 2 * kv_heads * page_size >= 0x7FFFFF00:
         return False
+    plan = shared_prefix_plan(rows, entries, width, q_heads, kv_heads, head_dim, page_size, shared)
+    if plan is None:
+        return False
+    sizes, floats = plan
     ops = _ops()
-    rows, (entries, width), device = qkv.shape[0], block_table.shape, qkv.device
-    prefix, own, parts, ctas, floats = shared_prefix_plan(rows, entries, width, q_heads, kv_heads, head_dim, page_size, shared)
-    buffer = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+    buffer = torch.empty(floats, dtype=torch.float32, device=qkv.device) if floats else None
     ops._check(shared_prefix_library().tlie_shared_prefix_bf16(
-        prefix, own, parts, ctas, qkv.data_ptr(), qkv.stride(0), pages.data_ptr(), pages.shape[0], positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), width,
-        out.data_ptr(), buffer.data_ptr() if floats else None, rows, entries, q_heads, kv_heads, head_dim, page_size, shared, scale, ops.error_flag(device).data_ptr(),
-        ops._stream()), "shared_prefix_attention")
+        sizes, q, q_stride, pages.data_ptr(), num_pages, positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), out_at,
+        buffer.data_ptr() if floats else None, scale, ops.error_flag(qkv.device).data_ptr(), ops._stream()), "shared_prefix_attention")
     return True
