@@ -760,14 +760,10 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
                                                                        q_heads, kv_heads, head_dim, page_size, scale):
         prefix_parts, own_parts = fast.generic_prefix_parts(rows, entries, q_heads // kv_heads, kv_heads, head_dim, shared, table_width * page_size - shared)
         buffer = torch.empty(rows * q_heads * (prefix_parts + own_parts) * (head_dim + 2), dtype=torch.float32, device=qkv.device)
-        _check(
-            shared_prefix().tlie_shared_prefix_generic(
-                _code(qkv), c_void_p(qkv.data_ptr()), c_longlong(q_stride), _ptr(pages), c_int(num_pages), _i32(positions, "positions"), _i32(seq_starts, "seq_starts"),
-                _i32(block_table, "block_table"), c_int(table_width), _ptr(out), _ptr(buffer), c_int(rows), c_int(entries), c_int(q_heads), c_int(kv_heads),
-                c_int(head_dim), c_int(page_size), c_int(shared), c_float(scale), c_int(prefix_parts), c_int(own_parts), _ptr(error_flag(qkv.device)), _stream(),
-            ),
-            "shared_prefix_attention",
-        )
+        _check(fast.shared_prefix_library().tlie_shared_prefix_generic(
+            _F32 if dtype is torch.float32 else _BF16, qkv.data_ptr(), q_stride, pages.data_ptr(), num_pages, positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), table_width,
+            out.data_ptr(), buffer.data_ptr(), rows, entries, q_heads, kv_heads, head_dim, page_size, shared, scale, prefix_parts, own_parts, error_flag(qkv.device).data_ptr(), _stream(),
+        ), "shared_prefix_attention")
 
 
 # --- recurrences ---------------------------------------------------------------------------

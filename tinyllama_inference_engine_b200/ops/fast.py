@@ -1206,10 +1206,11 @@ use_own = None                # likewise 0, 1: a row at a time, the tensor cores
 
 @functools.lru_cache(maxsize=None)
 def shared_prefix_library():
-    """The kernels of attention over a shared prefix; this launcher takes plain Python numbers."""
+    """The kernels of attention over a shared prefix; the launchers take plain Python numbers."""
     lib = _ops().shared_prefix()
-    p, n = c_void_p, c_longlong
-    lib.tlie_shared_prefix_bf16.argtypes = [p, p, n, p, c_int, p, p, p, p, p, c_float, p, p]
+    p, n, i = c_void_p, c_longlong, c_int
+    lib.tlie_shared_prefix_generic.argtypes = [i, p, n, p, i, p, p, p, i, p, p, i, i, i, i, i, i, i, c_float, i, i, p, p]
+    lib.tlie_shared_prefix_bf16.argtypes = [p, p, n, p, i, p, p, p, p, p, c_float, p, p]
     return lib
 
 
