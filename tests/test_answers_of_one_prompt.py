@@ -167,6 +167,16 @@ def test_runs_of_the_prefix_and_ctas_of_a_row(ops, way, heads, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("way", [(0, 0, 0, 1), (1, 0, 5, 1), (0, 0, 0, 2)], ids=lambda w: "-".join(map(str, w)), indirect=True)
+@pytest.mark.parametrize("warps", [2, 4, 16])
+@pytest.mark.parametrize("heads", [(5, 5, 64), (12, 4, 128), (34, 2, 128)], ids=lambda h: f"{h[0]}-{h[1]}x{h[2]}")
+def test_warps_of_a_row(ops, way, warps, heads, monkeypatch):
+    monkeypatch.setattr(ops.fast, "prefix_rows_warps", lambda *_: (0.0, warps))
+    case = attention_case(16, torch.bfloat16, *heads, 32, 333, [(5, 1), (0, 1), (400, 3), (40, 0), (31, 30)], front=1, behind=1, wider=8)
+    compare_attention(call_attention(ops, case), case, *plain_attention(case))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
 @pytest.mark.parametrize("heads,page_size,wider", [((8, 2, 64), 24, 0), ((8, 2, 128), 64, 3), ((160, 1, 64), 16, 0), ((7, 7, 176), 1, 0), ((4, 2, 240), 40, 0)])
 def test_sizes_of_the_general_kernel(ops, dtype, heads, page_size, wider):

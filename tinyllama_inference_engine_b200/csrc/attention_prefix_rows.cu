@@ -14,14 +14,15 @@
 
 #include "common.cuh"
 #include "mma_utils.cuh"
+#include "shared_memory_limit.cuh"
 
 namespace tlie {
 
-constexpr int kRowWarps = 8;
+constexpr int kRowWarps = 16;   // at most
 constexpr int kRowHeads = 8;       // query heads of a CTA: the columns of a product
 constexpr int kRowKeys = 16;       // keys of a tile: the rows of a product
 constexpr int kMostParts = 64;     // of the keys below first_key
-constexpr int kMostSources = 8 + kMostParts;   // (a CTA's warps, or a cluster's CTAs, and the parts)
+constexpr int kMostSources = kRowWarps + kMostParts;   // (a CTA's warps, or a cluster's CTAs, and the parts)
 constexpr float kToLog2 = 1.4426950408889634f;
 constexpr int kBadPage = 8;        // the bit of the device's error word
 
@@ -64,17 +65,17 @@ __device__ __forceinline__ unsigned transpose_8x8(unsigned two) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kRowWarps * 32, 2) prefix_rows_kernel(PrefixRowsParams p, bool waits_late) {
+__global__ void __launch_bounds__(kRowWarps * 32, 1) prefix_rows_kernel(PrefixRowsParams p, bool waits_late) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const int ctas = cluster.num_blocks(), rank = cluster.block_rank(), warps = blockDim.x >> 5;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row = blockIdx.x / ctas;
   const int group = p.q_heads / p.kv_heads, chunks = (group + kRowHeads - 1) / kRowHeads;
   const int kvh = blockIdx.y / chunks, head_in_group = (blockIdx.y - kvh * chunks) * kRowHeads;
   const int heads = min(kRowHeads, group - head_in_group), head0 = kvh * group + head_in_group;
   constexpr int kOutRow = D + 4;
-  __shared__ __align__(16) float merge_o[kRowWarps][kRowHeads][kOutRow];
+  extern __shared__ __align__(16) float merge_o[];   // [warp][head][kOutRow]
   __shared__ float2 merge_ml[kRowWarps][kRowHeads];
   __shared__ float factor_of[kRowHeads][kMostSources];
 
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) prefix_rows_kernel(PrefixRo
   if (!waits_late) grid_dependency_wait();
 
   // A step of one row per entry is asked for as such, all of it in one trip to memory; where the guess is wrong the entry is looked for.
-  const int warp_in_row = rank * kRowWarps + warp, step = ctas * kRowWarps;
+  const int warp_in_row = rank * warps + warp, step = ctas * warps;
   int tile = p.first_key / kRowKeys + warp_in_row;
   int entry = min(row, p.entries - 1);
   auto table_page = [&](const int* table, int tile) {
@@ -198,9 +199,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) prefix_rows_kernel(PrefixRo
 #pragma unroll
     for (int other = 4; other < 32; other <<= 1) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], other);
     if (g == 0) merge_ml[warp][2 * t + h] = make_float2(top[h], sum[h]);
+    if (2 * t + h >= heads) continue;
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
-      float* to = &merge_o[warp][2 * t + h][b * 64 + g * 8];
+      float* to = merge_o + (warp * heads + 2 * t + h) * kOutRow + b * 64 + g * 8;
       *reinterpret_cast<float4*>(to) = make_float4(o[b * 4][h], o[b * 4][h + 2], o[b * 4 + 1][h], o[b * 4 + 1][h + 2]);
       *reinterpret_cast<float4*>(to + 4) = make_float4(o[b * 4 + 2][h], o[b * 4 + 2][h + 2], o[b * 4 + 3][h], o[b * 4 + 3][h + 2]);
     }
@@ -221,49 +223,48 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) prefix_rows_kernel(PrefixRo
     return make_float2(m, warp_sum(l));
   };
   if (ctas > 1) {   // this CTA's part into the place of its first warp's, for the cluster
-    if (warp < heads) {
+    for (int h = warp; h < heads; h += warps) {
       float2 ml[kPerLane];
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) ml[i] = lane + 32 * i < kRowWarps ? merge_ml[lane + 32 * i][warp] : make_float2(-INFINITY, 0.0f);
+      for (int i = 0; i < kPerLane; ++i) ml[i] = lane + 32 * i < warps ? merge_ml[lane + 32 * i][h] : make_float2(-INFINITY, 0.0f);
       const float2 together = weigh(ml);
-      if (lane < kRowWarps) factor_of[warp][lane] = ml[0].x;
+      if (lane < warps) factor_of[h][lane] = ml[0].x;
       __syncwarp();
-      if (lane == 0) merge_ml[0][warp] = together;
+      if (lane == 0) merge_ml[0][h] = together;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * (D / 4); i += kRowWarps * 32) {
+    for (int i = threadIdx.x; i < heads * (D / 4); i += blockDim.x) {
       const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) {
+      for (int w = 0; w < warps; ++w) {
         const float f = factor_of[h][w];
         if (f == 0.0f) continue;
-        const float4 part = *reinterpret_cast<const float4*>(&merge_o[w][h][d]);
+        const float4 part = *reinterpret_cast<const float4*>(merge_o + (w * heads + h) * kOutRow + d);
         acc.x = fmaf(f, part.x, acc.x), acc.y = fmaf(f, part.y, acc.y), acc.z = fmaf(f, part.z, acc.z), acc.w = fmaf(f, part.w, acc.w);
       }
-      *reinterpret_cast<float4*>(&merge_o[0][h][d]) = acc;
+      *reinterpret_cast<float4*>(merge_o + h * kOutRow + d) = acc;
     }
     cluster.sync();
   }
   if (waits_late) grid_dependency_wait();
 
   // the cluster's CTAs' parts (or this CTA's warps') and those of the keys below first_key
-  const int own_sources = ctas > 1 ? ctas : kRowWarps, sources = own_sources + p.parts;
-  if (warp < heads && entry >= 0) {
-    const size_t pair = (size_t)row * p.q_heads + head0 + warp;
+  const int own_sources = ctas > 1 ? ctas : warps, sources = own_sources + p.parts;
+  for (int h = warp; h < heads && entry >= 0; h += warps) {
+    const size_t pair = (size_t)row * p.q_heads + head0 + h;
     float2 ml[kPerLane];
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const int source = lane + 32 * i;
       ml[i] = make_float2(-INFINITY, 0.0f);
-      if (source < own_sources) ml[i] = ctas > 1 ? *cluster.map_shared_rank(&merge_ml[0][warp], source) : merge_ml[source][warp];
+      if (source < own_sources) ml[i] = ctas > 1 ? *cluster.map_shared_rank(&merge_ml[0][h], source) : merge_ml[source][h];
       else if (source < sources) ml[i] = __ldcg(&p.part_ml[pair * p.parts + source - own_sources]);
     }
     const float l = weigh(ml).y;
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i)
-      if (lane + 32 * i < sources) factor_of[warp][lane + 32 * i] = ml[i].x == 0.0f ? 0.0f : ml[i].x * inverse;
+      if (lane + 32 * i < sources) factor_of[h][lane + 32 * i] = ml[i].x == 0.0f ? 0.0f : ml[i].x * inverse;
   }
   __syncthreads();
   // every CTA of the cluster finishes its share of the output; a part that counts for nothing is not read (it may never have been written)
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) prefix_rows_kernel(PrefixRo
 #pragma unroll 4
       for (int c = 0; c < own_sources; ++c) {
         const float f = factor[c];
-        const float* from = ctas > 1 ? cluster.map_shared_rank(&merge_o[0][h][d], c) : &merge_o[c][h][d];
+        const float* from = ctas > 1 ? cluster.map_shared_rank(merge_o + h * kOutRow + d, c) : merge_o + (c * heads + h) * kOutRow + d;
         add(f, f != 0.0f ? *reinterpret_cast<const float4*>(from) : nothing);
       }
       *reinterpret_cast<uint2*>(p.out + pair * D + d) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
@@ -293,11 +294,15 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) prefix_rows_kernel(PrefixRo
 }
 
 template <int D>
-static int launch_rows(const PrefixRowsParams& p, int ctas, bool waits_late, cudaStream_t stream) {
+static int launch_rows(const PrefixRowsParams& p, int ctas, int warps, bool waits_late, cudaStream_t stream) {
+  static std::atomic<unsigned long long> devices{0};
+  const cudaError_t e = allow_shared_memory(prefix_rows_kernel<D>, (int)sizeof(float) * kRowWarps * kRowHeads * (D + 4), devices);
+  if (e != cudaSuccess) return (int)e;
   const int group = p.q_heads / p.kv_heads, chunks = (group + kRowHeads - 1) / kRowHeads;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)p.rows * ctas, p.kv_heads * chunks);
-  config.blockDim = dim3(kRowWarps * 32);
+  config.blockDim = dim3(warps * 32);
+  config.dynamicSmemBytes = sizeof(float) * warps * (group < kRowHeads ? group : kRowHeads) * (D + 4);
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
@@ -315,18 +320,18 @@ static int launch_rows(const PrefixRowsParams& p, int ctas, bool waits_late, cud
 using namespace tlie;
 
 // q: rows [rows, q_row_stride] that start with the (rotated) query heads.  pages: one layer's pool [num_pages, 2, kv_heads, page_size, head_dim].  out: [rows,
-// q_heads * head_dim]; rows outside [seq_starts[0], seq_starts[entries]) are left as they are.  ctas: 1, 2, 4 or 8 per (row, head).  parts: for every (row, query
+// q_heads * head_dim]; rows outside [seq_starts[0], seq_starts[entries]) are left as they are.  ctas: 1, 2, 4 or 8 per (row, head), of 1 to 16 warps.  parts: for every (row, query
 // head), of the keys below first_key (0 if first_key is): 32-bit numbers [rows, q_heads, parts, 2] and then [rows, q_heads, parts, head_dim], 16-byte aligned
 // from first to last.  With parts the kernel in front in the stream must be the one that writes them.
 TLIE_EXPORT int tlie_prefix_rows(const void* q, long long q_row_stride, const void* pages, int num_pages, const int* positions, const int* seq_starts, const int* block_table,
                                  int table_stride, void* out, const float* part_ml, const float* part_o, int parts, int rows, int entries, int q_heads, int kv_heads,
-                                 int head_dim, int page_size, int first_key, float scale, int ctas, int* error_flag, cudaStream_t stream) {
+                                 int head_dim, int page_size, int first_key, float scale, int ctas, int warps, int* error_flag, cudaStream_t stream) {
   if (rows <= 0 || entries <= 0) return 0;
   if (kv_heads <= 0 || q_heads % kv_heads != 0 || page_size <= 0 || page_size % 16 != 0 || num_pages <= 0 || q_row_stride % 8 != 0 || ((uintptr_t)q & 15) || ((uintptr_t)pages & 15) ||
-      ((uintptr_t)out & 7) || ((uintptr_t)part_o & 15) || ((uintptr_t)part_ml & 7) || parts < 0 || parts > kMostParts || (ctas != 1 && ctas != 2 && ctas != 4 && ctas != 8) || (long long)rows * ctas > 0x7fffffffLL ||
+      ((uintptr_t)out & 7) || ((uintptr_t)part_o & 15) || ((uintptr_t)part_ml & 7) || parts < 0 || parts > kMostParts || (ctas != 1 && ctas != 2 && ctas != 4 && ctas != 8) || warps < 1 || warps > kRowWarps || (long long)rows * ctas > 0x7fffffffLL ||
       (long long)kv_heads * ((q_heads / kv_heads + kRowHeads - 1) / kRowHeads) > 65535 || error_flag == nullptr || (head_dim != 64 && head_dim != 128))
     return (int)cudaErrorInvalidValue;
   PrefixRowsParams p{(const __nv_bfloat16*)q, q_row_stride, (const __nv_bfloat16*)pages, num_pages, positions, seq_starts, block_table, table_stride, (__nv_bfloat16*)out,
                      part_o, (const float2*)part_ml, parts, rows, entries, q_heads, kv_heads, page_size, first_key, scale, error_flag};
-  return head_dim == 64 ? launch_rows<64>(p, ctas, parts > 0, stream) : launch_rows<128>(p, ctas, parts > 0, stream);
+  return head_dim == 64 ? launch_rows<64>(p, ctas, warps, parts > 0, stream) : launch_rows<128>(p, ctas, warps, parts > 0, stream);
 }

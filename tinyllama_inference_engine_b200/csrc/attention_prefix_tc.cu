@@ -1,9 +1,9 @@
 // Paged grouped-query attention for batches whose requests share their first cached keys, on the 5th-generation tensor cores (bfloat16, head size 64 or 128,
-// pages of a multiple of 16 keys).  Two builds of one kernel:
-//   * of the prefix (OWN false): all rows of the step against the keys below `shared`, a run of which a CTA takes; it leaves (m, l, o) per (row, query head): the
+// pages of a multiple of 16 keys).  Three builds of one kernel:
+//   * of the prefix: all rows of the step against the keys below `shared`, a run of which a CTA takes; it leaves (m, l, o) per (row, query head): the
 //     largest score (a reference near it), the sum of weights and the weighted sum of values;
-//   * of an entry's own keys (OWN true): an entry's rows against its keys first_key <= j <= p, brought together with the parts of the prefix where there are any,
-//     to the finished output.  With first_key = 0 it is the whole attention of portions of many rows.
+//   * of an entry's own keys (OWN): an entry's rows against its keys first_key <= j <= p, to the finished output, brought together with the parts of the prefix
+//     (JOINS); without them first_key is 0, and this is the whole attention of portions of many rows.
 //
 // The query heads of a group meet the same keys: a row tile is 128 (row, head of the group) pairs, 128 / group rows of the step.  A CTA has two such tiles and a
 // ring of key and value tiles for both, so that keys and values come from L2 once per 256 pairs.  One CTA fills an SM.
@@ -152,6 +152,10 @@ struct PrefixTCParams {
 template <int D>
 constexpr int kKeysOf = D <= 64 ? 128 : 80;   // keys of a key tile
 
+// Parts of the prefix that a CTA of own keys brings together: their factors lie in Q's place, behind 16 columns of a row tile's output.
+template <int D>
+constexpr int kOwnParts = (D * 2 - 64) / 4 < 32 ? (D * 2 - 64) / 4 : 32;
+
 template <int D>
 struct SmemPrefix {
   static constexpr int kKeys = kKeysOf<D>, kStages = D <= 64 ? 4 : 3;
@@ -170,7 +174,7 @@ struct SmemPrefix {
   int abort_flag;
 };
 
-template <int D, bool OWN>
+template <int D, bool OWN, bool JOINS>
 __global__ void __launch_bounds__(kThreadsTC, 1)
     prefix_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const PrefixTCParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -216,10 +220,9 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tmem = sm.tmem_base;
-  // Nothing of global memory is touched before the kernel in front has completed.  With OWN and parts that one is the prefix's, which lets this one start when all
+  // Nothing of global memory is touched before the kernel in front has completed.  With JOINS that one is the prefix's, which lets this one start when all
   // its CTAs are past this very wait: then what came before it is complete, and only its parts have to be waited for, at the end.
-  const bool waits_late = OWN && p.parts > 0;
-  if (!waits_late) grid_dependency_wait();
+  if (!JOINS) grid_dependency_wait();
   if (!OWN) grid_launch_dependents();
 
   // which rows: token0, and up to 2 * tile_tokens rows from there
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
       if (lane == 0 && j >= 0) mbar_arrive(&sm.s_read[u]);   // (the load was warp-wide: every lane has its scores)
       if (masked) {
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i) sc[i] = key0 + i < limit && (!OWN || key0 + i >= p.first_key) ? sc[i] : -INFINITY;
+        for (int i = 0; i < kKeys; ++i) sc[i] = key0 + i < limit && (!JOINS || key0 + i >= p.first_key) ? sc[i] : -INFINITY;
       }
       float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
@@ -477,7 +480,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
         // Values of keys that none of the CTA's rows sees (never written, perhaps) become zeros: 0 * (whatever is there) must stay 0.  Of keys that some rows see, what is
         // not finite is taken out and noted.
         const bool some_see = lowest < min(key0 + kKeys, last);
-        const int none_from = max(0, min(kKeys, last - key0)), none_to = OWN ? max(0, min(kKeys, p.first_key - key0)) : 0;
+        const int none_from = max(0, min(kKeys, last - key0)), none_to = JOINS ? max(0, min(kKeys, p.first_key - key0)) : 0;
         if (none_from < kKeys || none_to > 0 || some_see) {
           if (ok) ok = warp_wait(&sm.v_full[at.stage], at.phase, abort_flag);
           uint8_t* v_tile = reinterpret_cast<uint8_t*>(sm.v[at.stage]);
@@ -531,32 +534,47 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
       }
     };
     // Tiles that every row sees all of, then the others: what the masks take stays out of the loop that counts (with it inside, every tile took a fifth longer).
-    const int all_seen = OWN && p.first_key % kKeys != 0 ? 0 : max(0, min(mine, lowest / kKeys - kt_begin));
+    const int all_seen = JOINS && p.first_key % kKeys != 0 ? 0 : max(0, min(mine, lowest / kKeys - kt_begin));
     int j = -1;
     for (; mine > 0 && j < all_seen; ++j) take_tile(j, std::false_type{});
     for (; mine > 0 && j < mine; ++j) take_tile(j, std::true_type{});
     if (ok && mine > 0) ok = warp_wait(&sm.pv_done[u], (mine - 1) & 1, abort_flag);
-    if (waits_late) grid_dependency_wait();   // the prefix's parts
+    if (JOINS) grid_dependency_wait();   // the prefix's parts
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       const size_t at_pair = (size_t)token * p.q_heads + head;
       const bool any_bad = *(volatile int*)&sm.any_bad != 0;
       float top = reference, total = row_sum, factor = 1.0f;
-      if (OWN && mine_valid) {
-        for (int i = 0; i < p.parts; ++i) top = fmaxf(top, __ldcg(&p.part_ml[at_pair * p.parts + i]).x);
+      float4* staged = reinterpret_cast<float4*>(sm.q[u]) + sub * 32 * 4;
+      float* factors = reinterpret_cast<float*>(sm.q[u]) + kPairsTC * 16 + sub * 32 * kOwnParts<D>;   // [part][the warp's row]
+      if (JOINS) {
+        const float2* parts_ml = p.part_ml + at_pair * p.parts;
+#pragma unroll 2
+        for (int i = 0; i < p.parts; ++i) top = fmaxf(top, mine_valid ? __ldcg(parts_ml + i).x : -INFINITY);
         factor = reference == -INFINITY ? (row_sum == 0.0f ? 0.0f : 1.0f) : exp2f(reference - top);   // (a part of nothing but NaN keeps its NaN)
         total = row_sum * factor;
+#pragma unroll 2
         for (int i = 0; i < p.parts; ++i) {
-          const float2 ml = __ldcg(&p.part_ml[at_pair * p.parts + i]);
+          const float2 ml = mine_valid ? __ldcg(parts_ml + i) : make_float2(-INFINITY, 0.0f);
           const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : exp2f(ml.x - top);
           if (f != 0.0f) total = fmaf(f, ml.y, total);
+          factors[i * 32 + lane] = f;
         }
-      } else if (mine_valid) {
+      } else if (!OWN && mine_valid) {
         p.part_ml[at_pair * p.parts + blockIdx.x] = make_float2(reference, row_sum);
       }
       const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
       // A thread has its row, memory wants lines: 16 columns of the warp's 32 rows go through shared memory (Q's place: its products are done), piece i of row r at i ^ (r / 2 % 4).
-      float4* staged = reinterpret_cast<float4*>(sm.q[u]) + sub * 32 * 4;
+      // Row r = 8 i + lane / 4, piece lane % 4, is then a lane's i-th, of the prefix's parts too.  (Without parts a thread writes its own row: 32 bytes at a time, and less code to fetch.)
+      const int quarter = lane & 3;
+      size_t pair_at[4];
+      bool there[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int other = sub * 32 + 8 * i + (lane >> 2);
+        there[i] = other < tile_rows * group;
+        pair_at[i] = (size_t)(token0 + u * tile_tokens + other / group) * p.q_heads + kvh * group + other % group;
+      }
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {   // (the load is warp-wide: every lane takes part)
         uint32_t raw[16];
@@ -577,39 +595,50 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
             else if (minus) o[i] -= INFINITY;
           }
         }
+        if (!OWN && mine <= 0) continue;
         if (OWN) {
-          if (!mine_valid) continue;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = factor == 0.0f ? 0.0f : o[i] * factor;
-          for (int s = 0; s < p.parts; ++s) {
-            const float2 ml = __ldcg(&p.part_ml[at_pair * p.parts + s]);
-            const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : exp2f(ml.x - top);
-            if (f == 0.0f) continue;
-            const float4* part = reinterpret_cast<const float4*>(p.part_o + (at_pair * p.parts + s) * D + c);
+          for (int i = 0; i < 16; ++i) o[i] = JOINS && factor == 0.0f ? 0.0f : o[i] * factor;
+          if (!JOINS) {
+            uint4* to = reinterpret_cast<uint4*>(p.out + at_pair * D + c);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (mine_valid)
+                to[i] = make_uint4(pack_bf16(o[8 * i] * inverse, o[8 * i + 1] * inverse), pack_bf16(o[8 * i + 2] * inverse, o[8 * i + 3] * inverse),
+                                   pack_bf16(o[8 * i + 4] * inverse, o[8 * i + 5] * inverse), pack_bf16(o[8 * i + 6] * inverse, o[8 * i + 7] * inverse));
+            continue;
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) staged[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        __syncwarp();
+        float4 sums[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2);
+          sums[i] = staged[r * 4 + (quarter ^ ((r >> 1) & 3))];
+          if (!OWN && there[i]) reinterpret_cast<float4*>(p.part_o + (pair_at[i] * p.parts + blockIdx.x) * D + c)[quarter] = sums[i];
+        }
+        if (OWN) {
+#pragma unroll 2
+          for (int part = 0; part < p.parts; ++part) {
+            float4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = there[i] ? __ldcg(reinterpret_cast<const float4*>(p.part_o + (pair_at[i] * p.parts + part) * D + c) + quarter) : sums[i];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float4 v = __ldcg(part + i);
-              o[4 * i] = fmaf(f, v.x, o[4 * i]), o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]), o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]), o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
+              const float f = factors[part * 32 + 8 * i + (lane >> 2)];
+              if (f != 0.0f)   // (a part without keys was not written)
+                sums[i].x = fmaf(f, v[i].x, sums[i].x), sums[i].y = fmaf(f, v[i].y, sums[i].y), sums[i].z = fmaf(f, v[i].z, sums[i].z), sums[i].w = fmaf(f, v[i].w, sums[i].w);
             }
           }
-          uint4* to = reinterpret_cast<uint4*>(p.out + at_pair * D + c);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            to[i] = make_uint4(pack_bf16(o[8 * i] * inverse, o[8 * i + 1] * inverse), pack_bf16(o[8 * i + 2] * inverse, o[8 * i + 3] * inverse),
-                               pack_bf16(o[8 * i + 4] * inverse, o[8 * i + 5] * inverse), pack_bf16(o[8 * i + 6] * inverse, o[8 * i + 7] * inverse));
-        } else if (mine > 0) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) staged[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          __syncwarp();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = 8 * i + (lane >> 2), other = sub * 32 + r;
-            if (other < tile_rows * group) {
-              const size_t other_pair = (size_t)(token0 + u * tile_tokens + other / group) * p.q_heads + kvh * group + other % group;
-              reinterpret_cast<float4*>(p.part_o + (other_pair * p.parts + blockIdx.x) * D + c)[lane & 3] = staged[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
-            }
+            const float by = __shfl_sync(0xffffffffu, inverse, 8 * i + (lane >> 2));
+            if (there[i])
+              reinterpret_cast<uint2*>(p.out + pair_at[i] * D + c)[quarter] = make_uint2(pack_bf16(sums[i].x * by, sums[i].y * by), pack_bf16(sums[i].z * by, sums[i].w * by));
           }
-          __syncwarp();
         }
       }
     }
@@ -631,22 +660,22 @@ static bool make_q_map(CUtensorMap* map, const void* q, int rows, int q_heads, i
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, bool OWN>
+template <int D, bool OWN, bool JOINS>
 static int launch_tc(const CUtensorMap& map_q, const CUtensorMap& map_kv, const PrefixTCParams& p, dim3 grid, cudaStream_t stream) {
   static std::atomic<unsigned long long> devices{0};
   static std::atomic<int> registers{0};
   const int smem = (int)sizeof(SmemPrefix<D>) + 1024;
   static_assert(sizeof(SmemPrefix<D>) + 1024 <= 232448, "shared memory of a CTA");
-  cudaError_t e = allow_shared_memory(prefix_tc_kernel<D, OWN>, smem, devices);
+  cudaError_t e = allow_shared_memory(prefix_tc_kernel<D, OWN, JOINS>, smem, devices);
   if (e != cudaSuccess) return (int)e;
   if (registers.load(std::memory_order_relaxed) == 0) {   // the warps' shares are handed out of what the launch holds: less than that would wait for good
     cudaFuncAttributes found;
-    e = cudaFuncGetAttributes(&found, prefix_tc_kernel<D, OWN>);
+    e = cudaFuncGetAttributes(&found, prefix_tc_kernel<D, OWN, JOINS>);
     if (e != cudaSuccess) return (int)e;
     registers.store(found.numRegs, std::memory_order_relaxed);
   }
   if (registers.load(std::memory_order_relaxed) < kLaunchRegs) return (int)cudaErrorLaunchOutOfResources;
-  return (int)launch_pdl(prefix_tc_kernel<D, OWN>, grid, dim3(kThreadsTC), (size_t)smem, stream, map_q, map_kv, p);
+  return (int)launch_pdl(prefix_tc_kernel<D, OWN, JOINS>, grid, dim3(kThreadsTC), (size_t)smem, stream, map_q, map_kv, p);
 }
 
 }  // namespace tlie
@@ -661,6 +690,7 @@ TLIE_EXPORT int tlie_prefix_tc(int own, const void* q, long long q_row_stride, c
                                const int* block_table, int table_stride, void* out, float* part_ml, float* part_o, int parts, int rows, int entries, int q_heads, int kv_heads,
                                int head_dim, int page_size, int shared, int first_key, float scale, int* error_flag, cudaStream_t stream) {
   if (rows <= 0 || entries <= 0) return 0;
+  if (own && (parts > (head_dim == 64 ? kOwnParts<64> : kOwnParts<128>) || (parts > 0) != (first_key > 0))) return (int)cudaErrorInvalidValue;
   if (kv_heads <= 0 || q_heads % kv_heads != 0 || q_heads / kv_heads > kPairsTC || kv_heads > 65535 || page_size <= 0 || page_size % 16 != 0 || num_pages <= 0 || q_row_stride % 8 != 0 ||
       (head_dim != 64 && head_dim != 128) || error_flag == nullptr || ((uintptr_t)q & 15) || ((uintptr_t)pages & 15) || ((uintptr_t)out & 15) || ((uintptr_t)part_o & 15) ||
       ((uintptr_t)part_ml & 7) || (!own && (parts < 1 || shared < 1)))
@@ -681,9 +711,10 @@ TLIE_EXPORT int tlie_prefix_tc(int own, const void* q, long long q_row_stride, c
     const long long items = (long long)rows / (2 * tile_tokens) + entries;   // every entry may leave one piece that is not full
     if (items > 65535) return (int)cudaErrorInvalidValue;
     const dim3 grid(kv_heads, (unsigned)items);
-    return head_dim == 64 ? launch_tc<64, true>(map_q, map_kv, p, grid, stream) : launch_tc<128, true>(map_q, map_kv, p, grid, stream);
+    if (parts > 0) return head_dim == 64 ? launch_tc<64, true, true>(map_q, map_kv, p, grid, stream) : launch_tc<128, true, true>(map_q, map_kv, p, grid, stream);
+    return head_dim == 64 ? launch_tc<64, true, false>(map_q, map_kv, p, grid, stream) : launch_tc<128, true, false>(map_q, map_kv, p, grid, stream);
   }
   if (pieces > 65535) return (int)cudaErrorInvalidValue;
   const dim3 grid(parts, kv_heads, pieces);
-  return head_dim == 64 ? launch_tc<64, false>(map_q, map_kv, p, grid, stream) : launch_tc<128, false>(map_q, map_kv, p, grid, stream);
+  return head_dim == 64 ? launch_tc<64, false, false>(map_q, map_kv, p, grid, stream) : launch_tc<128, false, false>(map_q, map_kv, p, grid, stream);
 }

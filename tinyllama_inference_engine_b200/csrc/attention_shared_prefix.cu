@@ -380,11 +380,11 @@ TLIE_EXPORT int tlie_shared_prefix_generic(int dtype, const void* q, long long q
 extern "C" int tlie_prefix_tc(int, const void*, long long, const void*, int, const int*, const int*, const int*, int, void*, float*, float*, int, int, int, int, int, int, int, int, int, float,
                               int*, cudaStream_t);
 extern "C" int tlie_prefix_rows(const void*, long long, const void*, int, const int*, const int*, const int*, int, void*, const float*, const float*, int, int, int, int, int, int, int, int,
-                                float, int, int*, cudaStream_t);
+                                float, int, int, int*, cudaStream_t);
 
-// The bfloat16 kernels for head sizes 64 and 128 (each checks what it takes).  sizes, 12 numbers: prefix (0, every row reads the shared keys for itself; 1, the prefix's
+// The bfloat16 kernels for head sizes 64 and 128 (each checks what it takes).  sizes, 13 numbers: prefix (0, every row reads the shared keys for itself; 1, the prefix's
 // parts come from the tensor cores, `parts` runs of them), own (0, a row at a time, `ctas` per row and head; 1, an entry's rows on the tensor cores), parts, ctas, rows, entries, pages
-// of a table row, q_heads, kv_heads, head_dim, page_size, shared.  scratch: rows * q_heads * parts * (head_dim + 2) floats, 16-byte aligned.
+// of a table row, q_heads, kv_heads, head_dim, page_size, shared, warps of those CTAs.  scratch: rows * q_heads * parts * (head_dim + 2) floats, 16-byte aligned.
 TLIE_EXPORT int tlie_shared_prefix_bf16(const int* sizes, const void* q, long long q_row_stride, const void* pages, int num_pages, const int* positions, const int* seq_starts,
                                         const int* block_table, void* out, float* scratch, float scale, int* error_flag, cudaStream_t stream) {
   if (sizes == nullptr) return (int)cudaErrorInvalidValue;
@@ -405,7 +405,7 @@ TLIE_EXPORT int tlie_shared_prefix_bf16(const int* sizes, const void* q, long lo
     parts = 0;
   }
   return own == 0 ? tlie_prefix_rows(q, q_row_stride, pages, num_pages, positions, seq_starts, block_table, table_stride, out, part_ml, part_o, parts, rows, entries, q_heads, kv_heads,
-                                     head_dim, page_size, first_key, scale, ctas, error_flag, stream)
+                                     head_dim, page_size, first_key, scale, ctas, sizes[12], error_flag, stream)
                   : tlie_prefix_tc(1, q, q_row_stride, pages, num_pages, positions, seq_starts, block_table, table_stride, out, part_ml, part_o, parts, rows, entries, q_heads, kv_heads,
                                    head_dim, page_size, shared, first_key, scale, error_flag, stream);
 }

@@ -1223,14 +1223,39 @@ def prefix_rows_ctas(rows: int, kv_heads: int, group: int, keys: int) -> int:
     return ctas
 
 
-def prefix_tc_parts(rows: int, kv_heads: int, group: int, head_dim: int, shared: int) -> tuple[int, float]:
-    """Runs that the prefix's key tiles are cut into, and microseconds: what takes the longest SM's share of them and the parts' way through memory the least time.
+def prefix_rows_warps(pairs: int, ctas: int, keys: int) -> tuple[float, int]:
+    """Microseconds beside the reading, and warps of a CTA: 2, 4 or 8 where it alone has its row and head, 8 where a cluster has, 16 if there are few and long ones.
 
-    A key tile takes 1.1 us, an item's own start and end some 8, the parts are written and read again at some 4 TB/s."""
-    tiles = -(-shared // PREFIX_TC_KEYS[head_dim])
+    An SM holds 16 warps.  A CTA's start and end take it 1.7 us and 0.2 us a warp, and the last CTA's tiles of 16 keys follow one another, 0.85 us each.  (us, heads of 128: 131 rows, 32 heads
+    and 24 keys each, 2: 33, 4: 44, 8: 73; 48 rows, 32 heads, 825 keys, 2: 111, 4: 100, 8: 105; 48 rows, 8 heads, 1,100 keys, 2: 90, 4: 59, 8: 54; with the prefix's kernel in front.  With
+    one warp nothing was faster.  One row, 8 heads, 24,000 keys, 64 CTAs: 8: 38, 16: 30; two rows, 18,320 keys, 128 CTAs: 8: 40, 16: 46; 32 CTAs of 25 keys: 8: 5.1, 16: 5.7.)"""
+    if ctas > 1 or pairs * 2 <= sm_count():
+        return 0.0, 16 if pairs * ctas * 2 <= sm_count() and keys > 512 * ctas else 8
+    return min((pairs / sm_count() / 16 * (1.7 * warps + 0.2 * warps * warps) + 0.85 * keys / 16 / warps, warps) for warps in (2, 4, 8))
+
+
+def prefix_rows_us(rows: int, kv_heads: int, group: int, head_dim: int, keys: int) -> float:
+    """Microseconds of the kernel that works a row at a time: keys and values at some 9 TB/s from L2 and 4 GB/s per warp of 16 on an SM, or its CTAs' own starts and ends."""
+    pairs, ctas = rows * kv_heads * -(-group // 8), prefix_rows_ctas(rows, kv_heads, group, keys)
+    us, warps = prefix_rows_warps(pairs, ctas, keys)
+    return 4 + max(pairs * keys * head_dim * 4 / 9e6, -(-pairs * ctas * warps // (16 * sm_count())) * keys / ctas / warps * head_dim / 1e3, us)
+
+
+def prefix_tc_us(items: int, head_dim: int, keys: int, parts: int = 0) -> float:
+    """Microseconds of the tensor-core kernel for so many items (256 pairs of row and head at most) of so many keys each: 13 ns a key and 4 us an item, one item per SM at a time.
+
+    Where parts of the prefix are brought in, an item starts when they are there and takes 16 us and one a part."""
+    tile = PREFIX_TC_KEYS[head_dim]
+    return -(-items // sm_count()) * (-(-keys // tile) * tile * 0.0131 + (16 + parts if parts else 4)) + 4
+
+
+def prefix_tc_parts(rows: int, kv_heads: int, group: int, head_dim: int, shared: int) -> tuple[int, float]:
+    """Runs that the prefix's key tiles are cut into, and microseconds: what takes the longest SM's share of them and the parts' way through memory (written and read again at some 4 TB/s) the least time."""
+    tile = PREFIX_TC_KEYS[head_dim]
+    tiles = -(-shared // tile)
     items = -(-rows // (2 * (PREFIX_TC_PAIRS // group))) * kv_heads
     part = rows * kv_heads * group * head_dim * 8 / 4e6
-    return min(((-(-items * parts // sm_count()) * (-(-tiles // parts) * 1.1 + 3) + parts * part + 5, parts) for parts in range(1, min(tiles, PREFIX_MOST_PARTS) + 1)))[::-1]
+    return min(((prefix_tc_us(items * parts, head_dim, -(-tiles // parts) * tile) + parts * part, parts) for parts in range(1, min(tiles, PREFIX_MOST_PARTS) + 1)))[::-1]
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1251,28 +1276,28 @@ def generic_prefix_parts(rows: int, entries: int, group: int, kv_heads: int, hea
 def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_heads: int, head_dim: int, page_size: int, shared: int) -> tuple | None:
     """Which kernels a call of these sizes runs: (the launcher's numbers, which start with prefix, own, parts and CTAs per row and head; floats of scratch memory).
 
-    None: sizes that only the general kernel takes."""
+    None: sizes that only the general kernel takes.  Of the four ways (the shared keys once for all rows or by every row for itself; the rest a row at a time or an entry's rows
+    together) the one that the measured rates above say is fastest."""
     group = q_heads // kv_heads
     if head_dim not in SHARED_PREFIX_HEAD_DIMS or page_size % 16 != 0 or group > PREFIX_TC_PAIRS:
         return None
-    prefix, own = use_prefix, use_own
-    own_keys = width * page_size - shared
+    keys = width * page_size
     pieces = rows // (2 * (PREFIX_TC_PAIRS // group))   # of rows that are worked out together; a grid has room for 65,535
-    if own is None:
-        own = 1 if rows > 2 * entries and pieces + entries <= 65535 else 0
-    parts = 0
-    if shared > 0 and prefix != 0 and pieces < 65535:
-        tc_parts, once = prefix_tc_parts(rows, kv_heads, group, head_dim, shared)
-        if prefix is None:
-            if own:   # an entry's rows fill the row tiles that would share the prefix
-                prefix = 0 if rows * group >= 2 * PREFIX_TC_PAIRS * entries else 1
-            else:     # every row reads the prefix for itself, from L2 at some 7 TB/s
-                prefix = 0 if rows * kv_heads * -(-group // 8) * shared * head_dim * 4 / 7e6 < once else 1
-        parts = tc_parts if prefix else 0
-    else:
-        prefix = 0
-    ctas = prefix_rows_ctas(rows, kv_heads, group, own_keys if prefix else width * page_size)
-    return (c_int * 12)(prefix, own, parts, ctas, rows, entries, width, q_heads, kv_heads, head_dim, page_size, shared), rows * q_heads * parts * (head_dim + 2)
+    items = min(rows, pieces + entries) * kv_heads
+    parts, once = prefix_tc_parts(rows, kv_heads, group, head_dim, shared) if shared > 0 and pieces < 65535 else (0, 0.0)
+    ways = []
+    for prefix in (0, 1):
+        for own in (0, 1):
+            if prefix and parts == 0 or own and pieces + entries > 65535 or use_prefix not in (None, prefix) and parts > 0 or use_own not in (None, own):
+                continue
+            left, brought = (keys - shared, min(parts, head_dim // 4)) if prefix else (keys, 0)
+            ways.append(((once if prefix else 0.0) + (prefix_tc_us(items, head_dim, left, brought) if own else prefix_rows_us(rows, kv_heads, group, head_dim, left)), prefix, own))
+    _, prefix, own = min(ways)
+    parts = 0 if not prefix else min(parts, head_dim // 4) if own else parts
+    left = keys - shared if prefix else keys
+    ctas = prefix_rows_ctas(rows, kv_heads, group, left)
+    warps = prefix_rows_warps(rows * kv_heads * -(-group // 8), ctas, left)[1]
+    return (c_int * 13)(prefix, own, parts, ctas, rows, entries, width, q_heads, kv_heads, head_dim, page_size, shared, warps), rows * q_heads * parts * (head_dim + 2)
 
 
 def shared_prefix_attention(qkv, q_stride: int, pages, num_pages: int, positions, seq_starts, block_table, rows: int, entries: int, width: int, shared: int, out, q_heads: int, kv_heads: int,
