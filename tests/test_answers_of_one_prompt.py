@@ -390,6 +390,7 @@ def test_attention_refuses():
     wrong = {
         "no CPU path": {}, "head sizes": dict(head_dim=60), "multiple of key/value heads": dict(kv_heads=3), "qkv must be": dict(qkv=torch.zeros(3, 255)),
         "out must be [rows": dict(out=torch.zeros(3, 255)), "of qkv's dtype": dict(out=torch.zeros(3, 256, dtype=torch.bfloat16)), "pages must be": dict(page_size=32),
+        "fewer than 2^31 keys": dict(block_table=torch.zeros(1, dtype=torch.int32).expand(2, 1 << 27)),
         "16-byte boundary": dict(pages=torch.zeros(4 * 2 * 16 * 64 + 1)[1:].view(4, 2, 1, 16, 64)),
         "a block table": dict(seq_starts=torch.zeros(4, dtype=torch.int32)), "positions [rows]": dict(positions=torch.zeros(4, dtype=torch.int32)),
         "shared must be a whole number from 0 to the 32 keys": dict(shared=33), "got -1": dict(shared=-1), "got True": dict(shared=True), "scale must be": dict(scale=0.0),

@@ -10,6 +10,10 @@
 // from global memory straight to the registers that the products read, 16 bytes a load, nothing in shared memory: which of a head's dims a product's k index, or a row of
 // its output, stands for is free, as long as the query agrees, so the four lanes of a key read 64 consecutive bytes of it, and the eight lanes of a value 128.  A
 // warp has a whole tile, 4 KB at head size 64 and 8 KB at 128, on its way at once.
+//
+// CTAs of few warps where there are many: a CTA's start and end (the chain from the table to its first key, its parts' joining) cost an SM more than the keys of a short request, and
+// 16 warps are on an SM either way (128 registers a thread).  48 rows, 32 heads of 128, 612 keys each on average, behind 2,192 shared ones: 481 MB in 84 us beside the prefix's 17, 0.88 of the
+// measured copy rate.  131 rows, 32 heads, 24 keys: 33 us with the prefix's 17 (8 warps: 73).  64 rows, 4 key/value heads of 64 for 8 query heads each, 870 keys: 11.9 us, 4.8 TB/s from L2; one row behind 305: 5 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -18,7 +22,7 @@
 
 namespace tlie {
 
-constexpr int kRowWarps = 16;   // at most
+constexpr int kRowWarps = 16;      // at most
 constexpr int kRowHeads = 8;       // query heads of a CTA: the columns of a product
 constexpr int kRowKeys = 16;       // keys of a tile: the rows of a product
 constexpr int kMostParts = 64;     // of the keys below first_key

