@@ -381,6 +381,22 @@ def test_attention_in_graphs_and_on_other_streams(ops, dtype):
     compare_attention(held[0][1], case, *plain_attention(case))
 
 
+def test_a_wait_of_the_prefix_kernel_that_gives_up_is_reported():
+    """As in the other kernels with bounded waits: nobody reports by itself, all waits lie in front of the closing report, and tensor memory is given back behind it."""
+    import re
+    from pathlib import Path
+
+    from tinyllama_inference_engine_b200 import ops
+
+    source = (Path(ops.__file__).parent.parent / "csrc" / "attention_prefix_tc.cu").read_text()
+    assert "if (*gave_up" not in source
+    kernels = [part for part in re.split(r"(?=__global__ )", source)[1:] if "warp_wait(" in part]
+    assert len(kernels) == 1
+    for kernel in kernels:
+        end = kernel.index("close_and_report(gave_up,")
+        assert "_wait(&" not in kernel[end:] and kernel.index("tcgen05.dealloc", end) > end
+
+
 def test_attention_refuses():
     from tinyllama_inference_engine_b200 import ops
     from tinyllama_inference_engine_b200.errors import KernelError

@@ -117,9 +117,9 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // A whole warp waits: what follows is warp-wide, so the lanes go on or give up together.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
   if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up)) != 0;
 }
 
 // Non-zero where one of two bfloat16 numbers is infinite or NaN (an exponent of ones carries into the sign's place).
@@ -174,7 +174,7 @@ struct SmemPrefix {
   // them.  p_full: its weights are there; pv_done: its weighted values are added.
   uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], s_read[2], p_full[2], pv_done[2], exps_done[2][4];
   uint32_t tmem_base;
-  int abort_flag;
+  int gave_up;
 };
 
 template <int D, bool OWN, bool JOINS>
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
   using Smem = SmemPrefix<D>;
   constexpr int kStages = Smem::kStages, kKeys = Smem::kKeys, kHalves = D / kBoxDims;
   Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  volatile int* abort_flag = &sm.abort_flag;
+  volatile int* gave_up = &sm.gave_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = OWN ? blockIdx.x : blockIdx.y;
   const int group = p.q_heads / p.kv_heads, tile_tokens = kPairsTC / group;
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
       sm.lowest[u] = kNoKey;
       sm.last[u] = 0;
     }
-    sm.abort_flag = sm.any_bad = 0;
+    sm.gave_up = sm.any_bad = 0;
     sm.entry = sm.token0 = sm.tokens = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     bool ok = true;
     int rows = n > 0 ? look_up(0) : 0;
     for (int j = 0; j < n && ok; ++j, ring.advance()) {
-      ok = warp_wait(&empty[ring.stage], ring.phase ^ 1, abort_flag);
+      ok = warp_wait(&empty[ring.stage], ring.phase ^ 1, gave_up);
       if (!ok) break;
       const uint32_t to = tiles + ring.stage * (kKeys * D * 2), bar = smem_u32(&full[ring.stage]);
       if (leader) mbar_expect_tx(bar, kKeys * D * 2);
@@ -359,10 +359,10 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     const uint32_t q_low = umma_desc_low(smem_u32(sm.q[u])), k_low = umma_desc_low(smem_u32(sm.k)), to = tmem + kScoreCol0 + u * kKeys;
     const bool leader = elect_one();
     RingPosition<kStages> ring;
-    bool ok = mine == 0 || warp_wait(&sm.q_full, 0, abort_flag);
+    bool ok = mine == 0 || warp_wait(&sm.q_full, 0, gave_up);
     for (int j = 0; j < mine && ok; ++j, ring.advance()) {
-      ok = warp_wait(&sm.k_full[ring.stage], ring.phase, abort_flag);
-      if (ok && j > 0) ok = warp_wait(&sm.s_read[u], (j - 1) & 1, abort_flag);
+      ok = warp_wait(&sm.k_full[ring.stage], ring.phase, gave_up);
+      if (ok && j > 0) ok = warp_wait(&sm.s_read[u], (j - 1) & 1, gave_up);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       const uint32_t k_tile = k_low + ring.stage * ((kKeys * D * 2) >> 4);
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
       }
     }
     for (int j = mine; j < n && ok; ++j, ring.advance()) {   // none of this tile's rows sees these keys
-      ok = warp_wait(&sm.k_full[ring.stage], ring.phase, abort_flag);
+      ok = warp_wait(&sm.k_full[ring.stage], ring.phase, gave_up);
       if (ok && leader) mbar_arrive(&sm.k_empty[ring.stage]);
     }
   } else if (warp == 4) {
@@ -388,12 +388,12 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     RingPosition<kStages> ring;
     bool ok = true;
     for (int j = 0; j < n && ok; ++j, ring.advance()) {
-      ok = warp_wait(&sm.v_full[ring.stage], ring.phase, abort_flag);
+      ok = warp_wait(&sm.v_full[ring.stage], ring.phase, gave_up);
       const uint32_t v_tile = v_low + ring.stage * ((kKeys * D * 2) >> 4);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (!ok || j >= (u == 0 ? n0 : n1)) continue;
-        ok = warp_wait(&sm.p_full[u], j & 1, abort_flag);
+        ok = warp_wait(&sm.p_full[u], j & 1, gave_up);
         if (!ok) continue;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         if (leader) {
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     auto take_tile = [&](int j, auto some_masked) {
       constexpr bool masked = decltype(some_masked)::value;
       const int key0 = (kt_begin + max(j, 0)) * kKeys;
-      if (j >= 0 && ok) ok = warp_wait(&sm.s_full[u], j & 1, abort_flag);
+      if (j >= 0 && ok) ok = warp_wait(&sm.s_full[u], j & 1, gave_up);
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       float sc[kKeys];
       {
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
       const bool grown = scaled_max > reference + kLazyRescale;
       if (__builtin_expect(__any_sync(0xffffffffu, grown), 0)) {
         if (j > 0) {
-          if (ok) ok = warp_wait(&sm.pv_done[u], (j - 1) & 1, abort_flag);   // the product that last added to the output
+          if (ok) ok = warp_wait(&sm.pv_done[u], (j - 1) & 1, gave_up);   // the product that last added to the output
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           const float alpha = grown ? exp2f(reference - scaled_max) : 1.0f;
 #pragma unroll 1
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
         const bool some_see = lowest < min(key0 + kKeys, last);
         const int none_from = max(0, min(kKeys, last - key0)), none_to = JOINS ? max(0, min(kKeys, p.first_key - key0)) : 0;
         if (none_from < kKeys || none_to > 0 || some_see) {
-          if (ok) ok = warp_wait(&sm.v_full[at.stage], at.phase, abort_flag);
+          if (ok) ok = warp_wait(&sm.v_full[at.stage], at.phase, gave_up);
           uint8_t* v_tile = reinterpret_cast<uint8_t*>(sm.v[at.stage]);
           for (int r = pair >> 3; r < kKeys; r += kPairsTC / 8) {   // 8 threads a row of 128 bytes, whatever the swizzle
             if (r < none_to || r >= none_from) {
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
       }
       // The warps of the two row tiles that share a scheduler take turns: one's exponentials, which the exponential unit sets the pace of, run under the other's loads, maxima and
       // stores.  Left alone they fall into step and wait for the unit together, then leave it idle together (2,750 cycles a tile).
-      if (ok && (u == 0 ? j > 0 && j <= n1 : j >= 0 && j < n0)) ok = warp_wait(&sm.exps_done[u ^ 1][sub], (u == 0 ? j - 1 : j) & 1, abort_flag);
+      if (ok && (u == 0 ? j > 0 && j <= n1 : j >= 0 && j < n0)) ok = warp_wait(&sm.exps_done[u ^ 1][sub], (u == 0 ? j - 1 : j) & 1, gave_up);
       const Pair scale2 = pair_of(sl2, sl2), minus_base2 = pair_of(-base, -base);
       Pair sums = pair_of(0.0f, 0.0f);
       uint32_t packed[kKeys / 2];
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
         packed[i] = pack_bf16(p0, p1);   // a weight keeps 8 bits where it meets its value, as in the other bfloat16 attention kernels; the sum has all of it
       }
       if (lane == 0 && j >= 0) mbar_arrive(&sm.exps_done[u][sub]);
-      if (j > 0 && ok) ok = warp_wait(&sm.pv_done[u], (j - 1) & 1, abort_flag);   // the weights before have been read
+      if (j > 0 && ok) ok = warp_wait(&sm.pv_done[u], (j - 1) & 1, gave_up);   // the weights before have been read
 #pragma unroll
       for (int c = 0; c < kKeys / 2; c += 4) tmem_store_4(tmem_p + c, packed + c);
       asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     int j = -1;
     for (; mine > 0 && j < all_seen; ++j) take_tile(j, std::false_type{});
     for (; mine > 0 && j < mine; ++j) take_tile(j, std::true_type{});
-    if (ok && mine > 0) ok = warp_wait(&sm.pv_done[u], (mine - 1) & 1, abort_flag);
+    if (ok && mine > 0) ok = warp_wait(&sm.pv_done[u], (mine - 1) & 1, gave_up);
     if (JOINS) grid_dependency_wait();   // the prefix's parts
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   }
-  close_and_report(abort_flag, p.error_flag);
+  close_and_report(gave_up, p.error_flag);
   if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols));
 }
 
