@@ -240,10 +240,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) prefix_rows_kernel(PrefixRo
     for (int i = threadIdx.x; i < heads * (D / 4); i += blockDim.x) {
       const int h = i / (D / 4), d = (i - h * (D / 4)) * 4;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
       for (int w = 0; w < warps; ++w) {
         const float f = factor_of[h][w];
-        if (f == 0.0f) continue;
-        const float4 part = *reinterpret_cast<const float4*>(merge_o + (w * heads + h) * kOutRow + d);
+        float4 part = *reinterpret_cast<const float4*>(merge_o + (w * heads + h) * kOutRow + d);
+        if (f == 0.0f) part = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // (what counts for nothing may be no number)
         acc.x = fmaf(f, part.x, acc.x), acc.y = fmaf(f, part.y, acc.y), acc.z = fmaf(f, part.z, acc.z), acc.w = fmaf(f, part.w, acc.w);
       }
       *reinterpret_cast<float4*>(merge_o + h * kOutRow + d) = acc;
