@@ -740,17 +740,18 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     Called inside the capture of a CUDA graph, the graph keeps ``shared`` and the tensors' addresses; what the tensors hold may change from replay to replay."""
     scale = head_dim ** -0.5 if scale is None else float(scale)
     index, dtype = qkv.get_device(), qkv.dtype   # (a tensor that is not on a CUDA device is on -1)
-    if index < 0 or qkv.dim() != 2 or block_table.dim() != 2 or pages.dim() != 5:
+    try:
+        (rows, width), (q_stride, q_step), (entries, table_width), (num_pages, two, page_heads, page_keys, page_dim) = qkv.shape, qkv.stride(), block_table.shape, pages.shape
+    except ValueError:   # another number of axes
         _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
-    (rows, width), (q_stride, q_step), (entries, table_width) = qkv.shape, qkv.stride(), block_table.shape
-    num_pages, two, page_heads, page_keys, page_dim = pages.shape
-    if not ((dtype is torch.bfloat16 or dtype is torch.float32) and pages.dtype is dtype and out.dtype is dtype
+    pages_at = pages.data_ptr()
+    if not (index >= 0 and (dtype is torch.bfloat16 or dtype is torch.float32) and pages.dtype is dtype and out.dtype is dtype
             and positions.dtype is torch.int32 and seq_starts.dtype is torch.int32 and block_table.dtype is torch.int32
             and index == pages.get_device() == out.get_device() == positions.get_device() == seq_starts.get_device() == block_table.get_device()
             and 0 < head_dim <= 256 and head_dim % 16 == 0 and 0 < kv_heads <= q_heads and q_heads % kv_heads == 0 and width >= q_heads * head_dim
             and out.shape == (rows, q_heads * head_dim) and num_pages > 0 and two == 2 and page_heads == kv_heads and page_keys == page_size and page_dim == head_dim
             and positions.shape == (rows,) and seq_starts.shape == (entries + 1,) and type(shared) is int and 0 <= shared <= table_width * page_size < 1 << 31
-            and 0.0 < scale < float("inf") and (q_step == 1 or rows == 0) and pages.is_contiguous() and pages.data_ptr() % 16 == 0 and out.is_contiguous()
+            and 0.0 < scale < float("inf") and (q_step == 1 or rows == 0) and pages.is_contiguous() and pages_at % 16 == 0 and out.is_contiguous()
             and positions.is_contiguous() and seq_starts.is_contiguous() and block_table.is_contiguous()):
         _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
     if rows == 0 or entries == 0:
@@ -758,14 +759,23 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     if index != _current_device():
         with torch.cuda.device(index):
             return shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
-    if dtype is not torch.bfloat16 or not fast.shared_prefix_attention(qkv, q_stride, pages, num_pages, positions, seq_starts, block_table, rows, entries, table_width, shared, out,
-                                                                       q_heads, kv_heads, head_dim, page_size, scale):
+    q_at, out_at, lib = qkv.data_ptr(), out.data_ptr(), fast.shared_prefix_library()
+    plan = None
+    # (the bfloat16 kernels read and write rows 16 bytes at a time and count the pool's rows of keys and values in 31 bits)
+    if dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_at | out_at) % 16 == 0 and num_pages * 2 * kv_heads * page_size < 0x7FFFFF00:
+        plan = fast.shared_prefix_plan(rows, entries, table_width, q_heads, kv_heads, head_dim, page_size, shared)
+    if plan is not None:
+        sizes, floats = plan
+        scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device) if floats else None
+        status = lib.tlie_shared_prefix_bf16(sizes, q_at, q_stride, pages_at, num_pages, positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), out_at,
+                                             scratch.data_ptr() if floats else None, scale, error_flag(qkv.device).data_ptr(), _stream())
+    else:
         prefix_parts, own_parts = fast.generic_prefix_parts(rows, entries, q_heads // kv_heads, kv_heads, head_dim, shared, table_width * page_size - shared)
-        buffer = torch.empty(rows * q_heads * (prefix_parts + own_parts) * (head_dim + 2), dtype=torch.float32, device=qkv.device)
-        _check(fast.shared_prefix_library().tlie_shared_prefix_generic(
-            _F32 if dtype is torch.float32 else _BF16, qkv.data_ptr(), q_stride, pages.data_ptr(), num_pages, positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), table_width,
-            out.data_ptr(), buffer.data_ptr(), rows, entries, q_heads, kv_heads, head_dim, page_size, shared, scale, prefix_parts, own_parts, error_flag(qkv.device).data_ptr(), _stream(),
-        ), "shared_prefix_attention")
+        scratch = torch.empty(rows * q_heads * (prefix_parts + own_parts) * (head_dim + 2), dtype=torch.float32, device=qkv.device)
+        status = lib.tlie_shared_prefix_generic(
+            _F32 if dtype is torch.float32 else _BF16, q_at, q_stride, pages_at, num_pages, positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), table_width, out_at, scratch.data_ptr(),
+            rows, entries, q_heads, kv_heads, head_dim, page_size, shared, scale, prefix_parts, own_parts, error_flag(qkv.device).data_ptr(), _stream())
+    _check(status, "shared_prefix_attention")
 
 
 # --- recurrences ---------------------------------------------------------------------------

@@ -1274,9 +1274,9 @@ def generic_prefix_parts(rows: int, entries: int, group: int, kv_heads: int, hea
 
 @functools.lru_cache(maxsize=4096)
 def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_heads: int, head_dim: int, page_size: int, shared: int) -> tuple | None:
-    """Which kernels a call of these sizes runs: (the launcher's numbers, which start with prefix, own, parts and CTAs per row and head; floats of scratch memory).
+    """Which bfloat16 kernels a call of these sizes runs: (the launcher's numbers, which start with prefix, own, parts and CTAs per row and head; floats of scratch memory).
 
-    None: sizes that only the general kernel takes.  Of the four ways (the shared keys once for all rows or by every row for itself; the rest a row at a time or an entry's rows
+    None: sizes that only the general kernel takes (these take head sizes 64 and 128 and pages of a multiple of 16 keys).  Of the four ways (the shared keys once for all rows or by every row for itself; the rest a row at a time or an entry's rows
     together) the one that the measured rates above say is fastest."""
     group = q_heads // kv_heads
     if head_dim not in SHARED_PREFIX_HEAD_DIMS or page_size % 16 != 0 or group > PREFIX_TC_PAIRS:
@@ -1298,23 +1298,3 @@ def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_hea
     ctas = prefix_rows_ctas(rows, kv_heads, group, left)
     warps = prefix_rows_warps(rows * kv_heads * -(-group // 8), ctas, left)[1]
     return (c_int * 13)(prefix, own, parts, ctas, rows, entries, width, q_heads, kv_heads, head_dim, page_size, shared, warps), rows * q_heads * parts * (head_dim + 2)
-
-
-def shared_prefix_attention(qkv, q_stride: int, pages, num_pages: int, positions, seq_starts, block_table, rows: int, entries: int, width: int, shared: int, out, q_heads: int, kv_heads: int,
-                            head_dim: int, page_size: int, scale: float) -> bool:
-    """bfloat16 attention over a shared prefix on the kernels made for it; False if they do not take the call.
-
-    They take head sizes 64 and 128, pages of a multiple of 16 keys, rows that are read 16 bytes at a time, and pools whose rows of keys and values a 32-bit number counts."""
-    q, out_at = qkv.data_ptr(), out.data_ptr()
-    if q_stride % 8 != 0 or (q | out_at) % 16 != 0 or num_pages * 2 * kv_heads * page_size >= 0x7FFFFF00:
-        return False
-    plan = shared_prefix_plan(rows, entries, width, q_heads, kv_heads, head_dim, page_size, shared)
-    if plan is None:
-        return False
-    sizes, floats = plan
-    ops = _ops()
-    buffer = torch.empty(floats, dtype=torch.float32, device=qkv.device) if floats else None
-    ops._check(shared_prefix_library().tlie_shared_prefix_bf16(
-        sizes, q, q_stride, pages.data_ptr(), num_pages, positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), out_at,
-        buffer.data_ptr() if floats else None, scale, ops.error_flag(qkv.device).data_ptr(), ops._stream()), "shared_prefix_attention")
-    return True
