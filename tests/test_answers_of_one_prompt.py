@@ -506,6 +506,26 @@ def test_equal_weights_are_counted_to_the_token(ops):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40, 200])
+@pytest.mark.parametrize("vocab", [2000, 32000, 128256])
+def test_a_border_on_a_whole_number_of_equal_weights(ops, vocab, rows):
+    """Some tokens weigh 1 and all others nothing: top_p of them ends exactly at a token, which what they weigh about cannot tell."""
+    g = torch.Generator().manual_seed(vocab + rows)
+    number = [int(n) for n in torch.randint(2, 180, (rows,), generator=g)]
+    logits = torch.full((rows, vocab), -1e4)
+    ids = [torch.randperm(vocab, generator=g)[:n].sort().values for n in number]
+    for row, where in enumerate(ids):
+        logits[row, where] = 3.0
+    top_p = [float(np.float32(p)) for p in (0.5, 0.25, 0.75, 0.125, 0.9, 0.3)]
+    u = torch.rand(rows, generator=g).tolist()
+    want = []
+    for row in range(rows):
+        kept = max(1, math.ceil(top_p[row % 6] * number[row]))
+        want.append(int(ids[row][int(float(np.float32(u[row])) * kept)]))
+    assert call_choice(ops, logits, [0.8] * rows, [0] * rows, [top_p[row % 6] for row in range(rows)], [0.0] * rows, u) == want
+
+
+@pytest.mark.gpu
 def test_logits_that_are_no_numbers(ops):
     inf, nan = float("inf"), float("nan")
     row = torch.tensor([nan, -inf, 1.0, nan, 2.0, -inf, 2.0, 0.0])

@@ -67,10 +67,11 @@ struct Border {
 
 // A row belongs to a cluster of CTAs, consecutive tokens to each, which read them once for the maximum and again, from the caches, for what follows; that is mostly done by the first CTA on a short
 // list of the order's first tokens.  As many threads' maxima as are asked for bound the list from below (so many tokens at least are not below the least of them), and the highest
-// of the CTAs' bounds holds for all.  With top_k so many tokens are asked for and all others are out of it; with top_p alone some hundred, and the exact weight of all
-// tokens tells whether they suffice; min_p alone says itself which tokens it leaves.  One row is bound by the chain of its steps and the fetching of their code (32,000 tokens, top-k 40 and
-// top-p: 10.7 us); many with top-k by reading (256 rows of 128,256 tokens: 41.6 us, 3.2 TB/s; reading ahead through shared memory took 44); with top-p alone by the 21 instructions of a token's exact
-// weight and by the slowest CTA of a cluster (64 rows of 128,256: 35.5 us, of which the weights some 10).
+// of the CTAs' bounds holds for all.  With top_k so many tokens are asked for and all others are out of it; with top_p alone some hundred, and what all tokens weigh, to some 2^-19 of it, tells whether
+// they suffice and where the border lies; only if it would lie elsewhere for another total in between are all weights worked out exactly (with exact weights at once, 21 instructions a token,
+// 64 rows of 128,256 took 35.5 us).  min_p alone says itself which tokens it leaves.  One row is bound by the chain of its steps (32,000 tokens, top-k 40 and top-p: 10.7 us, top-p alone: 15.3);
+// many by reading (256 rows of 128,256 with top-k 50: 41.5 us, 3.2 TB/s; reading ahead through shared memory took 44) and, with top-p alone, by the second pass and the slowest CTA of a
+// cluster (64 rows of 128,256: 26.1 us).
 //
 // Where the list does not do (top_k beyond it, flat rows), a border is found from a histogram over 2,048 runs of logits, 1/64 wide, below the largest, of numbers or
 // of exact weights, and from the tokens of the run that it falls in, which the first CTA sorts.  Where those are too many (equal logits, or very close ones) the run is
@@ -211,29 +212,53 @@ class RowFilter {
         const unsigned long long token = sh.early[threadIdx.x];
         if ((int)threadIdx.x < listed && (unsigned)(token >> 32) >= bounds.x) sh.list[atomicAdd(&sh.listed, 1)] = token;
         __syncthreads();
-        return choose_from_list(top_k, top_p, 0ull, u);
+        return choose_from_list(top_k, top_p, 0ull, 0ull, u);
       }
     }
     const bool by_floor = !by_number && !by_weight && floor_weight > 0ull;
     if (by_floor) bound = m + temperature * (logf(min_p) * 1.0001f - 0.001f);   // (a little low: the list is longer than what stays of it)
     if (bound > -INFINITY) {
-      unsigned long long mine = 0ull, total = 0ull;
-      list_from(bound, by_weight && !by_number, mine);
-      if (by_weight && !by_number) {
-        block_prefix(mine, sh.scan, mine);
-        all = gather(mine, 0ull);
-        for (int c = 0; c < ctas; ++c) total += all[c];
+      const bool nucleus = by_weight && !by_number;
+      unsigned long long mine = 0ull, least = 0ull, most = 0ull;
+      float spread = 0.0f;
+      list_from(bound, nucleus, mine, spread);
+      if (nucleus) {   // between what two numbers the weight of all tokens lies
+        mine = warp_sum_u64(mine);
+        unsigned long long spread_of_all = warp_sum_u64((unsigned long long)(spread * 1048576.0f));
+        if (lane == 0) sh.scan[warp] = mine, sh.exchange[0][warp] = spread_of_all;
+        __syncthreads();
+        mine = spread_of_all = 0ull;
+        for (int w = 0; w < kFilterWarps; ++w) mine += sh.scan[w], spread_of_all += sh.exchange[0][w];
+        all = gather(mine, spread_of_all);
+        unsigned long long about = 0ull, far = 0ull;
+        for (int c = 0; c < ctas; ++c) about += all[c], far += all[8 + c];
+        const unsigned long long off = (unsigned long long)((double)about * 1e-6 + ((double)far / 1048576.0 + 0.01) * (1.5e-7 * (double)(1ull << kWeightBits))) + 1ull;
+        least = about - min(about, off), most = about + off;
       } else {
         sync();
       }
       if (*at_first(&sh.listed) <= kListed) {
-        if (by_number || by_floor) return rank == 0 ? choose_from_list(by_number ? top_k : kListed, top_p, 0ull, u) : 0;
-        if (rank == 0) {
-          const int token = choose_from_list(kListed, top_p, total, u);
-          if (threadIdx.x == 0) sh.chosen = token;
+        if (by_number || by_floor) return rank == 0 ? choose_from_list(by_number ? top_k : kListed, top_p, 0ull, 0ull, u) : 0;
+#pragma unroll 1
+        for (int exact = m < INFINITY ? 0 : 1; exact < 2; ++exact) {
+          if (exact) {
+            mine = 0ull;
+            for_tokens([&](float l, int) { mine += weight(l); });
+            block_prefix(mine, sh.scan, mine);
+            all = gather(mine, 0ull);
+            least = 0ull;
+            for (int c = 0; c < ctas; ++c) least += all[c];
+            most = least;
+          }
+          if (rank == 0) {
+            const int token = choose_from_list(kListed, top_p, least, most, u);
+            if (threadIdx.x == 0) sh.chosen = token;
+          }
+          sync();
+          const int token = *at_first(&sh.chosen);
+          if (token >= 0) return token;
+          if (token == kListTooShort) break;
         }
-        sync();
-        if (*at_first(&sh.chosen) >= 0) return sh.chosen;
       }
       sync();   // (all have read the list's length before the next search clears it)
     }
@@ -249,7 +274,7 @@ class RowFilter {
   }
 
  private:
-  static constexpr int kGuess = 192;
+  static constexpr int kGuess = 192, kListTooShort = -1, kUnsure = -2;
   FilterShared& sh;
   cooperative_groups::cluster_group cluster;
   const int vocab, ctas, rank, lane, warp, first_id, count;
@@ -411,47 +436,52 @@ class RowFilter {
     return id;
   }
 
-  // Lists the tokens that are not below the bound; with `weights` the weight of all tokens, this thread's share of it.
-  __device__ __forceinline__ void list_from(float bound, bool weights, unsigned long long& mine) {
-    const float nan = __int_as_float(0x7fffffff);
+  // Lists the tokens that are not below the bound; with `weights` about what all tokens weigh in units of 2^-44, this thread's share of it, and the sum of their weights times their distances
+  // y = log2 of the weight from the largest.  An eighth of the exact weights' instructions: l - m, the scale and the product are off by 2^-24 each, so a weight by 1.25e-7 |y|, the exponential by
+  // 2^-22, the sum of 16 by 6 * 2^-24, what is left of exact weights below 2^-44 and of |y| above 64 by 2^-25 together: 1.5e-7 |y| and 1e-6 hold all that.  Whether
+  // top_p's border lies on the same token for all totals in between is seen when the list is in order; if not, exact weights tell.
+  __device__ __forceinline__ void list_from(float bound, bool weights, unsigned long long& mine, float& spread) {
+    const float nan = __int_as_float(0x7fffffff), slope = (float)scale.c;
     constexpr int kFlight = 4;
+    auto about = [&](float l) {   // (NaN counts for 2^-64)
+      const float y = fmaxf((l - m) * slope, -64.0f), w = exp2_approx(y);
+      spread = fmaf(w, -y, spread);
+      return w;
+    };
     for (int q0 = threadIdx.x; q0 - (int)threadIdx.x < quads; q0 += kFlight * kFilterThreads) {
       float4 v[kFlight];
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) v[u] = q0 + u * kFilterThreads < quads ? quad(q0 + u * kFilterThreads) : make_float4(nan, nan, nan, nan);
-      if (!weights) {
+      if (weights) {
+        float sum = 0.0f;
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u) put_quad(v[u], bound, q0 + u * kFilterThreads, at_first(&sh.listed), at_first(sh.list));
-        continue;
+        for (int u = 0; u < kFlight; ++u) sum += (about(v[u].x) + about(v[u].y)) + (about(v[u].z) + about(v[u].w));
+        mine += (unsigned long long)(sum * (float)(1ull << kWeightBits));
       }
-#pragma unroll 1
-      for (int u = 0; u < kFlight; ++u) {
-        mine += (weight(v[0].x) + weight(v[0].y)) + (weight(v[0].z) + weight(v[0].w));
-        put_quad(v[0], bound, q0 + u * kFilterThreads, at_first(&sh.listed), at_first(sh.list));
 #pragma unroll
-        for (int other = 0; other + 1 < kFlight; ++other) v[other] = v[other + 1];
-      }
+      for (int u = 0; u < kFlight; ++u) put_quad(v[u], bound, q0 + u * kFilterThreads, at_first(&sh.listed), at_first(sh.list));
     }
     const int i = edge_token();
     const float l = i >= 0 ? tokens[i] : nan;
-    if (weights) mine += weight(l);
+    if (weights) mine += (unsigned long long)(about(l) * (float)(1ull << kWeightBits));
     put(l >= bound, l, first_id + i);
   }
 
-  // The row's token if its first top_k tokens (or all that min_p leaves, or, where `total` is the weight of all tokens, all that top_p leaves) are on the list; by the first CTA.  -1: the
-  // list's weight does not reach top_p of `total`.
-  __device__ __forceinline__ int choose_from_list(int top_k, float top_p, unsigned long long total, float u) {
+  // The row's token if its first top_k tokens (or all that min_p leaves, or, where the weight of all tokens lies between `least` and `most`, all that top_p leaves) are on the list; by the
+  // first CTA.  Where the list's weight does not reach top_p of all tokens' kListTooShort, where it depends on what they weigh exactly kUnsure.
+  __device__ __forceinline__ int choose_from_list(int top_k, float top_p, unsigned long long least, unsigned long long most, float u) {
     const int number = min(top_k, sh.listed), mine = threadIdx.x;
     const unsigned long long token = sort_falling(sh.list[mine], sh.listed, sh.exchange);
     const unsigned long long w = mine < number ? weight(key_logit((unsigned)(token >> 32))) : 0ull;
     unsigned long long all, of_kept;
     const unsigned long long before = block_prefix(w, sh.scan, all);
-    const unsigned long long of = total != 0ull ? total : all;
-    const unsigned long long wanted = top_p < 1.0f ? max(1ull, min(of, (unsigned long long)ceil((double)top_p * (double)of))) : ~0ull;
-    if (total != 0ull && all < wanted) return -1;
+    if (most == 0ull) least = most = all;
+    else if (all < wanted_of(top_p, least)) return kListTooShort;
+    else if (all < wanted_of(top_p, most)) return kUnsure;
     // kept: in front of which top_p has not been reached, heavy enough; the first always
-    const bool kept = mine == 0 || (mine < number && before < wanted && w >= floor_weight);
-    const int many = __syncthreads_count(kept);
+    const bool heavy = mine < number && w >= floor_weight;
+    const int many = __syncthreads_count(mine == 0 || (heavy && before < wanted_of(top_p, least)));
+    if (least != most && __syncthreads_count(mine == 0 || (heavy && before < wanted_of(top_p, most))) != many) return kUnsure;
     // in order of ids (the lower one's complement is the larger), the weight behind the id
     const unsigned long long by_id = sort_falling(((unsigned long long)((unsigned)token & (kFilterMaxVocab - 1)) << (kWeightBits + 1)) | w, many, sh.exchange);
     const unsigned long long kept_weight = mine < many ? by_id & ((2ull << kWeightBits) - 1ull) : 0ull;
@@ -459,6 +489,10 @@ class RowFilter {
     if (target >= start && target < start + kept_weight) sh.found_id = (int)(~(unsigned)(by_id >> (kWeightBits + 1)) & (kFilterMaxVocab - 1));
     __syncthreads();
     return sh.found_id;
+  }
+  // What top_p of a total comes to.
+  __device__ static unsigned long long wanted_of(float top_p, unsigned long long total) {
+    return top_p < 1.0f ? max(1ull, min(total, (unsigned long long)ceil((double)top_p * (double)total))) : ~0ull;
   }
   __device__ static unsigned long long target_of(float u, unsigned long long total) {
     const unsigned long long target = u > 0.0f ? (unsigned long long)((double)fminf(u, 1.0f) * (double)total) : 0ull;
