@@ -526,6 +526,35 @@ def test_a_border_on_a_whole_number_of_equal_weights(ops, vocab, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40, 200])
+@pytest.mark.parametrize("vocab", [2000, 32000, 128256])
+def test_a_number_that_falls_where_a_token_ends(ops, vocab, rows):
+    """Without top-k, top-p and min-p, over equal weights: the number is where one token ends and the next begins, or just in front of it."""
+    g = torch.Generator().manual_seed(vocab + rows)
+    number = [2 ** int(n) for n in torch.randint(1, 11, (rows,), generator=g)]
+    logits = torch.full((rows, vocab), -float("inf"))
+    ids = [torch.randperm(vocab, generator=g)[:n].sort().values for n in number]
+    place = [int(torch.randint(1, n, (1,), generator=g)) for n in number]
+    for row, where in enumerate(ids):
+        logits[row, where] = -2.0
+    for before in (False, True):
+        u = [float(np.nextafter(np.float32(k / n), np.float32(0))) if before else k / n for k, n in zip(place, number)]
+        want = [int(where[k - before]) for where, k in zip(ids, place)]
+        assert call_choice(ops, logits, [1.3] * rows, [0] * rows, [1.0] * rows, [0.0] * rows, u) == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1, 5, 2000, 32003, 128256])
+def test_the_first_of_equal_largest_tokens(ops, vocab):
+    g = torch.Generator().manual_seed(vocab)
+    for rows in (1, 30, 200):
+        logits = torch.randn(rows, vocab + 3, generator=g).round()[:, 1 : vocab + 1]   # (rows that do not start on 16 bytes)
+        want = [int((row == row.max()).nonzero()[0]) for row in logits]
+        assert call_choice(ops, logits, [0.0] * rows, [0] * rows, [1.0] * rows, [0.0] * rows, [0.5] * rows) == want
+        assert call_choice(ops, logits, [1.0] * rows, [1] * rows, [1.0] * rows, [0.0] * rows, [0.5] * rows) == want
+
+
+@pytest.mark.gpu
 def test_logits_that_are_no_numbers(ops):
     inf, nan = float("inf"), float("nan")
     row = torch.tensor([nan, -inf, 1.0, nan, 2.0, -inf, 2.0, 0.0])

@@ -18,6 +18,7 @@ namespace tlie {
 constexpr int kFilterThreads = 512, kFilterWarps = kFilterThreads / 32;
 constexpr int kBinBits = 11, kBins = 1 << kBinBits, kBinsEach = kBins / kFilterThreads;
 constexpr int kListed = kFilterThreads;    // tokens of the list, one per thread
+constexpr int kEarly = 3 * kFilterThreads; // ... and of those that may come on it, while a row is read
 constexpr int kFilterMaxVocab = 1 << 19;   // (so many weights of 2^44 and less: sums fit 64 bits, a token's id and weight one number)
 constexpr int kWeightBits = 44;
 
@@ -83,7 +84,7 @@ struct FilterShared {
     };
     unsigned long long list[kListed];
   };
-  unsigned long long exchange[2][kFilterThreads], early[kListed];
+  unsigned long long exchange[2][kFilterThreads], early[kEarly];
   unsigned long long scan[kFilterWarps];
   unsigned long long gather[2][2][8];   // two numbers per CTA
   unsigned long long above;       // the first CTA's are the cluster's, as are:
@@ -208,11 +209,18 @@ class RowFilter {
       __syncthreads();
       if (threadIdx.x == 0) sh.listed = 0;
       __syncthreads();
-      if (listed >= top_k && listed <= kListed) {
-        const unsigned long long token = sh.early[threadIdx.x];
-        if ((int)threadIdx.x < listed && (unsigned)(token >> 32) >= bounds.x) sh.list[atomicAdd(&sh.listed, 1)] = token;
+      if (listed >= top_k && listed <= kEarly) {
+        for (int i = threadIdx.x; i < listed; i += kFilterThreads) {
+          const unsigned long long token = sh.early[i];
+          if ((unsigned)(token >> 32) < bounds.x) continue;
+          const int at = atomicAdd(&sh.listed, 1);
+          if (at < kListed) sh.list[at] = token;
+        }
         __syncthreads();
-        return choose_from_list(top_k, top_p, 0ull, 0ull, u);
+        if (sh.listed <= kListed) return choose_from_list(top_k, top_p, 0ull, 0ull, u);
+        __syncthreads();
+        if (threadIdx.x == 0) sh.listed = 0;
+        __syncthreads();
       }
     }
     const bool by_floor = !by_number && !by_weight && floor_weight > 0ull;
@@ -224,16 +232,16 @@ class RowFilter {
       list_from(bound, nucleus, mine, spread);
       if (nucleus) {   // between what two numbers the weight of all tokens lies
         mine = warp_sum_u64(mine);
-        unsigned long long spread_of_all = warp_sum_u64((unsigned long long)(spread * 1048576.0f));
+        unsigned long long spread_of_all = warp_sum_u64(spread_in_units(spread));
         if (lane == 0) sh.scan[warp] = mine, sh.exchange[0][warp] = spread_of_all;
         __syncthreads();
         mine = spread_of_all = 0ull;
         for (int w = 0; w < kFilterWarps; ++w) mine += sh.scan[w], spread_of_all += sh.exchange[0][w];
         all = gather(mine, spread_of_all);
-        unsigned long long about = 0ull, far = 0ull;
-        for (int c = 0; c < ctas; ++c) about += all[c], far += all[8 + c];
-        const unsigned long long off = (unsigned long long)((double)about * 1e-6 + ((double)far / 1048576.0 + 0.01) * (1.5e-7 * (double)(1ull << kWeightBits))) + 1ull;
-        least = about - min(about, off), most = about + off;
+        unsigned long long total = 0ull, far = 0ull;
+        for (int c = 0; c < ctas; ++c) total += all[c], far += all[8 + c];
+        const unsigned long long off = off_at_most(total, far);
+        least = total - min(total, off), most = total + off;
       } else {
         sync();
       }
@@ -261,6 +269,12 @@ class RowFilter {
         }
       }
       sync();   // (all have read the list's length before the next search clears it)
+    }
+    if (!by_number && !by_weight && floor_weight == 0ull) {   // all tokens
+      const int token = m < INFINITY ? draw_from_all<false>(u) : -1;
+      if (token >= 0) return token;
+      sync();   // (all have read it)
+      return draw_from_all<true>(u);
     }
     Border kept = {0u, vocab};
 #pragma unroll 1
@@ -302,22 +316,22 @@ class RowFilter {
   __device__ static int bin_below(float top, float l) { return l == top ? 0 : (int)fminf((top - l) * 64.0f, (float)(kBins - 1)); }
 
   // Puts a token on a list if `wanted`; a warp's threads come together.  The list may be too short: its length says so.
-  __device__ __forceinline__ void put_into(bool wanted, float l, int id, int* listed, unsigned long long* list) {
+  __device__ __forceinline__ void put_into(bool wanted, float l, int id, int* listed, unsigned long long* list, int room = kListed) {
     const unsigned who = __ballot_sync(0xffffffffu, wanted);
     if (who == 0u) return;
     int at = 0;
     if (lane == 0) at = atomicAdd(listed, __popc(who));
     at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-    if (wanted && at < kListed) list[at] = ((unsigned long long)logit_key(l) << 32) | (unsigned)~id;
+    if (wanted && at < room) list[at] = ((unsigned long long)logit_key(l) << 32) | (unsigned)~id;
   }
   // ... on the first CTA's.
   __device__ __forceinline__ void put(bool wanted, float l, int id) { put_into(wanted, l, id, at_first(&sh.listed), at_first(sh.list)); }
   // Those of four tokens that are not below a bound.
-  __device__ __forceinline__ void put_quad(float4 v, float bound, int q, int* listed, unsigned long long* list) {
+  __device__ __forceinline__ void put_quad(float4 v, float bound, int q, int* listed, unsigned long long* list, int room = kListed) {
     if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) return;
 #pragma unroll 1
     for (int e = 0; e < 4; ++e) {
-      put_into(v.x >= bound, v.x, first_id + head + 4 * q + e, listed, list);
+      put_into(v.x >= bound, v.x, first_id + head + 4 * q + e, listed, list, room);
       v.x = v.y, v.y = v.z, v.z = v.w;
     }
   }
@@ -329,7 +343,7 @@ class RowFilter {
   __device__ __forceinline__ float4 quad(int q) const { return reinterpret_cast<const float4*>(tokens + head)[q]; }
 
   // This thread's largest token (NaN is none).  With `asked` (and one CTA) tokens go on the list as they come, those that are not below a bound that so many tokens before are not
-  // below; the bound is taken anew when twice as many tokens have been seen.
+  // below; the bound is taken anew when four times as many tokens have been seen.
   __device__ __forceinline__ void load(int asked) {
     const float nan = __int_as_float(0x7fffffff);
     thread_max = nan;
@@ -345,18 +359,18 @@ class RowFilter {
       if (asked == 0) continue;
       const int seen = q0 - (int)threadIdx.x + kFlight * kFilterThreads;
       if (seen >= next_bound) {   // (the same for all threads)
-        next_bound = 2 * seen;
+        next_bound = 4 * seen;
         const float largest = block_max(thread_max);
         bound = largest > -INFINITY ? key_logit(least_of_maxima(largest, asked, asked).x) : INFINITY;   // (INFINITY: whole runs of tokens without one above -infinity)
         __syncthreads();
       }
 #pragma unroll
-      for (int u = 0; u < kFlight; ++u) put_quad(v[u], bound, q0 + u * kFilterThreads, &sh.listed, sh.early);
+      for (int u = 0; u < kFlight; ++u) put_quad(v[u], bound, q0 + u * kFilterThreads, &sh.listed, sh.early, kEarly);
     }
     const int i = edge_token();
     const float l = i >= 0 ? tokens[i] : nan;
     thread_max = fmaxf(thread_max, l);
-    if (asked != 0) put_into(l >= bound, l, first_id + i, &sh.listed, sh.early);
+    if (asked != 0) put_into(l >= bound, l, first_id + i, &sh.listed, sh.early, kEarly);
   }
   // NaN if all are.
   __device__ __forceinline__ float block_max(float v) {
@@ -420,12 +434,22 @@ class RowFilter {
   }
   // The first token of the order.
   __device__ __forceinline__ int first_of_order() {
-    int id = 0x7fffffff;
-    for (int i = threadIdx.x; i < count; i += kFilterThreads)
-      if (tokens[i] == m) {
-        id = first_id + i;
-        break;
+    constexpr int kNone = 0x7fffffff, kFlight = 4;
+    int id = kNone;
+    if (thread_max == m) {   // (who has read such a token looks where it stands)
+      for (int q0 = threadIdx.x; q0 < quads && id == kNone; q0 += kFlight * kFilterThreads) {
+        float4 v[kFlight];
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f) v[f] = quad(min(q0 + f * kFilterThreads, quads - 1));
+#pragma unroll
+        for (int f = kFlight - 1; f >= 0; --f) {
+          const int at = first_id + head + 4 * min(q0 + f * kFilterThreads, quads - 1);
+          id = v[f].x == m ? at : v[f].y == m ? at + 1 : v[f].z == m ? at + 2 : v[f].w == m ? at + 3 : id;
+        }
       }
+      const int i = edge_token();
+      if (i >= 0 && tokens[i] == m) id = min(id, first_id + i);
+    }
     id = __reduce_min_sync(0xffffffffu, id);
     if (threadIdx.x == 0) sh.found_id = 0x7fffffff;
     __syncthreads();
@@ -436,34 +460,42 @@ class RowFilter {
     return id;
   }
 
-  // Lists the tokens that are not below the bound; with `weights` about what all tokens weigh in units of 2^-44, this thread's share of it, and the sum of their weights times their distances
-  // y = log2 of the weight from the largest.  An eighth of the exact weights' instructions: l - m, the scale and the product are off by 2^-24 each, so a weight by 1.25e-7 |y|, the exponential by
-  // 2^-22, the sum of 16 by 6 * 2^-24, what is left of exact weights below 2^-44 and of |y| above 64 by 2^-25 together: 1.5e-7 |y| and 1e-6 hold all that.  Whether
-  // top_p's border lies on the same token for all totals in between is seen when the list is in order; if not, exact weights tell.
+  // About what a token weighs, of the largest one's weight, and its share of the sum of weights times their distances y = log2 of the weight from the largest.  An eighth of the exact weight's
+  // instructions: l - m, the scale and the product are off by 2^-24 each, so a weight by 1.25e-7 |y|, the exponential by 2^-22, a sum of 16 in pairs by 4 * 2^-24, what is left of exact weights below
+  // 2^-44 and of |y| above 64 by 2^-25 each, exact weights themselves by 1.5e-7: 1.5e-7 |y| and 8e-7 hold all that.  (NaN counts for 2^-64.)
+  __device__ __forceinline__ float about(float l, float slope, float& spread) const {
+    const float y = fmaxf((l - m) * slope, -64.0f), w = exp2_approx(y);
+    spread = fmaf(w, -y, spread);
+    return w;
+  }
+  __device__ __forceinline__ float about(float4 v, float slope, float& spread) const {
+    return (about(v.x, slope, spread) + about(v.y, slope, spread)) + (about(v.z, slope, spread) + about(v.w, slope, spread));
+  }
+  __device__ static unsigned long long in_units(float w) { return (unsigned long long)(w * (float)(1ull << kWeightBits)); }
+  __device__ static unsigned long long spread_in_units(float spread) { return (unsigned long long)(spread * 1048576.0f); }
+  // How far what tokens weigh about, in units of 2^-44, is off what they weigh at most.
+  __device__ static unsigned long long off_at_most(unsigned long long about, unsigned long long spread) {
+    return (unsigned long long)((double)about * 8e-7 + ((double)spread / 1048576.0 + 0.01) * (1.5e-7 * (double)(1ull << kWeightBits))) + 1ull;
+  }
+  // Lists the tokens that are not below the bound; with `weights` about what all tokens weigh, this thread's share of it.  Whether top_p's border lies on the same token for all totals in between
+  // is seen when the list is in order; if not, exact weights tell.
   __device__ __forceinline__ void list_from(float bound, bool weights, unsigned long long& mine, float& spread) {
     const float nan = __int_as_float(0x7fffffff), slope = (float)scale.c;
     constexpr int kFlight = 4;
-    auto about = [&](float l) {   // (NaN counts for 2^-64)
-      const float y = fmaxf((l - m) * slope, -64.0f), w = exp2_approx(y);
-      spread = fmaf(w, -y, spread);
-      return w;
-    };
     for (int q0 = threadIdx.x; q0 - (int)threadIdx.x < quads; q0 += kFlight * kFilterThreads) {
       float4 v[kFlight];
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) v[u] = q0 + u * kFilterThreads < quads ? quad(q0 + u * kFilterThreads) : make_float4(nan, nan, nan, nan);
       if (weights) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u) sum += (about(v[u].x) + about(v[u].y)) + (about(v[u].z) + about(v[u].w));
-        mine += (unsigned long long)(sum * (float)(1ull << kWeightBits));
+        static_assert(kFlight == 4, "sums of 16");
+        mine += in_units((about(v[0], slope, spread) + about(v[1], slope, spread)) + (about(v[2], slope, spread) + about(v[3], slope, spread)));
       }
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) put_quad(v[u], bound, q0 + u * kFilterThreads, at_first(&sh.listed), at_first(sh.list));
     }
     const int i = edge_token();
     const float l = i >= 0 ? tokens[i] : nan;
-    if (weights) mine += (unsigned long long)(about(l) * (float)(1ull << kWeightBits));
+    if (weights) mine += in_units(about(l, slope, spread));
     put(l >= bound, l, first_id + i);
   }
 
@@ -643,6 +675,70 @@ class RowFilter {
     }
     sync();
     return Border{key, *at_first(&sh.found_id)};
+  }
+  // The token that the number falls on among all of them, in order of ids: from exact weights, or from what they weigh about, and -1 then if it lies too near another token for that.
+  template <bool EXACT>
+  __device__ __forceinline__ int draw_from_all(float u) {
+    const float slope = (float)scale.c, nan = __int_as_float(0x7fffffff);
+    float spread = 0.0f;
+    auto of_token = [&](float l) { return EXACT ? weight(l) : in_units(about(l, slope, spread)); };
+    const int segment = (quads + kFilterWarps - 1) / kFilterWarps, begin = min(quads, warp * segment), end = min(quads, begin + segment);   // as below
+    unsigned long long mine = 0ull;
+    constexpr int kFlight = 4;
+    for (int q0 = begin + lane; q0 < end; q0 += 32 * kFlight) {
+      float4 v[kFlight];
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) v[f] = q0 + 32 * f < end ? quad(q0 + 32 * f) : make_float4(nan, nan, nan, nan);
+      static_assert(kFlight == 4, "sums of 16");
+      if constexpr (EXACT) {
+#pragma unroll 1
+        for (int f = 0; f < kFlight; ++f) {
+          mine += (weight(v[0].x) + weight(v[0].y)) + (weight(v[0].z) + weight(v[0].w));
+#pragma unroll
+          for (int other = 0; other + 1 < kFlight; ++other) v[other] = v[other + 1];
+        }
+      } else {
+        mine += in_units((about(v[0], slope, spread) + about(v[1], slope, spread)) + (about(v[2], slope, spread) + about(v[3], slope, spread)));
+      }
+    }
+    const int first = warp == 0 ? 0 : head + 4 * begin, last = warp == kFilterWarps - 1 ? count : head + 4 * end;   // this warp's tokens
+    if (warp == 0 && lane < head) mine += of_token(tokens[lane]);
+    if (warp == kFilterWarps - 1 && head + 4 * quads + lane < count) mine += of_token(tokens[head + 4 * quads + lane]);
+    mine = warp_sum_u64(mine);
+    unsigned long long far = warp_sum_u64(spread_in_units(spread));
+    if (lane == 0) sh.exchange[0][warp] = far;
+    if (threadIdx.x == 0) sh.found_id = -1;
+    unsigned long long all, before = block_prefix(lane == 0 ? mine : 0ull, sh.scan, all);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    far = 0ull;
+    for (int w = 0; w < kFilterWarps; ++w) far += sh.exchange[0][w];
+    const unsigned long long* of_cta = gather(all, far);
+    unsigned long long total = 0ull, start = 0ull;
+    far = 0ull;
+    for (int c = 0; c < ctas; ++c) {
+      if (c < rank) start += of_cta[c];
+      total += of_cta[c], far += of_cta[8 + c];
+    }
+    // The number's place is off by so much at most, and so is where a token begins or ends (every token in front of it counts once).
+    const unsigned long long target = target_of(u, total), off = EXACT ? 0ull : 2ull * off_at_most(total, far) + 8ull;
+    if (target >= start && target < start + all) {
+      if (lane == 0 && target >= start + before && target < start + before + mine) sh.last_run[0] = first, sh.last_run[1] = last, sh.above = start + before;
+      __syncthreads();
+      const int from = sh.last_run[0], to = sh.last_run[1], each = (to - from + kFilterThreads - 1) / kFilterThreads;
+      const int a = min(to, from + (int)threadIdx.x * each), b = min(to, a + each);
+      unsigned long long part = 0ull, sum;
+      for (int i = a; i < b; ++i) part += of_token(tokens[i]);
+      unsigned long long running = sh.above + block_prefix(part, sh.scan, sum);
+      if (target >= running && target < running + part) {
+        for (int i = a; i < b; ++i) {
+          const unsigned long long w = of_token(tokens[i]);
+          if (target >= running + off && target + off < running + w) *at_first(&sh.found_id) = first_id + i;   // (a token at most)
+          running += w;
+        }
+      }
+    }
+    sync();
+    return *at_first(&sh.found_id);
   }
   // The token that the number falls on among the kept ones, in order of ids.
   __device__ __forceinline__ int draw(const Border& kept, float u) {
