@@ -71,12 +71,12 @@ struct Border {
 // of the CTAs' bounds holds for all.  With top_k so many tokens are asked for and all others are out of it; with top_p alone some hundred, and what all tokens weigh, to some 2^-19 of it, tells whether
 // they suffice and where the border lies; only if it would lie elsewhere for another total in between are all weights worked out exactly (with exact weights at once, 21 instructions a token,
 // 64 rows of 128,256 took 35.5 us).  min_p alone says itself which tokens it leaves.  One row is bound by the chain of its steps (32,000 tokens, top-k 40 and top-p: 10.7 us, top-p alone: 15.3);
-// many by reading (256 rows of 128,256 with top-k 50: 41.5 us, 3.2 TB/s; reading ahead through shared memory took 44) and, with top-p alone, by the second pass and the slowest CTA of a
+// many by reading (256 rows of 128,256 with top-k 50: 39.7 us, 3.3 TB/s; reading ahead through shared memory took 2 more) and, with top-p alone, by the second pass and the slowest CTA of a
 // cluster (64 rows of 128,256: 26.1 us).
 //
 // Where the list does not do (top_k beyond it, flat rows), a border is found from a histogram over 2,048 runs of logits, 1/64 wide, below the largest, of numbers or
 // of exact weights, and from the tokens of the run that it falls in, which the first CTA sorts.  Where those are too many (equal logits, or very close ones) the run is
-// cut by the bits of the logits, and equal ones by id.  (One row of 32,000 with top-k 450: 48 us; 64 rows of 128,256 at a temperature of 3 with top-p alone: 134 us.)
+// cut by the bits of the logits, and equal ones by id.  (One row of 32,000 with top-k 450: 48 us; 160 rows of 128,256 with top-k 400: 433, with 300, on the list: 71; 64 rows at a temperature of 3 with top-p alone: 134.)
 struct FilterShared {
   union {                         // (one is done with before the other begins)
     struct {
@@ -343,7 +343,7 @@ class RowFilter {
   __device__ __forceinline__ float4 quad(int q) const { return reinterpret_cast<const float4*>(tokens + head)[q]; }
 
   // This thread's largest token (NaN is none).  With `asked` (and one CTA) tokens go on the list as they come, those that are not below a bound that so many tokens before are not
-  // below; the bound is taken anew when four times as many tokens have been seen.
+  // below; the bound is taken anew when four times (two, where many are asked for) as many tokens have been seen.
   __device__ __forceinline__ void load(int asked) {
     const float nan = __int_as_float(0x7fffffff);
     thread_max = nan;
@@ -359,7 +359,7 @@ class RowFilter {
       if (asked == 0) continue;
       const int seen = q0 - (int)threadIdx.x + kFlight * kFilterThreads;
       if (seen >= next_bound) {   // (the same for all threads)
-        next_bound = 4 * seen;
+        next_bound = (asked <= 200 ? 4 : 2) * seen;   // (what comes in between has to find room; 256 rows of 128,256, top-k 50: 39.8 us, 41.6 by twos; 160 rows, top-k 300: 103, 71 by twos)
         const float largest = block_max(thread_max);
         bound = largest > -INFINITY ? key_logit(least_of_maxima(largest, asked, asked).x) : INFINITY;   // (INFINITY: whole runs of tokens without one above -infinity)
         __syncthreads();
