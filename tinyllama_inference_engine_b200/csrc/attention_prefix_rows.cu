@@ -16,6 +16,8 @@
 // measured copy rate.  131 rows, 32 heads, 24 keys: 33 us with the prefix's 17 (8 warps: 73).  64 rows, 4 key/value heads of 64 for 8 query heads each, 870 keys: 11.9 us, 4.8 TB/s from L2; one row behind 305: 5 us.
 #include <cooperative_groups.h>
 
+#include <cstdlib>
+
 #include "common.cuh"
 #include "mma_utils.cuh"
 #include "shared_memory_limit.cuh"
@@ -316,7 +318,11 @@ static int launch_rows(const PrefixRowsParams& p, int ctas, int warps, bool wait
   attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
-  config.numAttrs = 2;
+  static const bool pdl = [] {
+    const char* v = std::getenv("TLIE_PDL");
+    return !(v && v[0] == '0');
+  }();
+  config.numAttrs = pdl ? 2 : 1;
   return (int)cudaLaunchKernelEx(&config, prefix_rows_kernel<D>, p, waits_late);
 }
 

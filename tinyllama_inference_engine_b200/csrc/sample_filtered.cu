@@ -11,6 +11,8 @@
 // it: with sums in 32-bit floats the border of top-p, and the token that a number falls on, would be off by a token in one draw of some hundred over a flat row.
 #include <cooperative_groups.h>
 
+#include <cstdlib>
+
 #include "common.cuh"
 
 namespace tlie {
@@ -856,7 +858,11 @@ TLIE_EXPORT int tlie_sample_filtered(const float* logits, long long row_stride, 
   attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
-  config.numAttrs = 2;
+  static const bool pdl = [] {
+    const char* v = std::getenv("TLIE_PDL");
+    return !(v && v[0] == '0');
+  }();
+  config.numAttrs = pdl ? 2 : 1;
   return (int)cudaLaunchKernelEx(&config, sample_filtered_kernel, logits, row_stride, all_rows, vocab, slice, rows, temperature, top_k, top_p, min_p, uniforms, out);
 }
 
