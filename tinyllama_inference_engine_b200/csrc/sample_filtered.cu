@@ -361,9 +361,11 @@ class RowFilter {
       if (asked == 0) continue;
       const int seen = q0 - (int)threadIdx.x + kFlight * kFilterThreads;
       if (seen >= next_bound) {   // (the same for all threads)
-        next_bound = (asked <= 200 ? 4 : 2) * seen;   // (what comes in between has to find room; 256 rows of 128,256, top-k 50: 39.8 us, 41.6 by twos; 160 rows, top-k 300: 103, 71 by twos)
         const float largest = block_max(thread_max);
-        bound = largest > -INFINITY ? key_logit(least_of_maxima(largest, asked, asked).x) : INFINITY;   // (INFINITY: whole runs of tokens without one above -infinity)
+        if (largest > -INFINITY) {   // (while no token is, there is nothing to list and the next batch asks again: a bound has to stand before the first of them is tested)
+          bound = key_logit(least_of_maxima(largest, asked, asked).x);
+          next_bound = (asked <= 200 ? 4 : 2) * seen;   // (what comes in between has to find room; 256 rows of 128,256, top-k 50: 39.8 us, 41.6 by twos; 160 rows, top-k 300: 103, 71 by twos)
+        }
         __syncthreads();
       }
 #pragma unroll
