@@ -542,6 +542,9 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
     for (; mine > 0 && j < all_seen; ++j) take_tile(j, std::false_type{});
     for (; mine > 0 && j < mine; ++j) take_tile(j, std::true_type{});
     if (ok && mine > 0) ok = warp_wait(&sm.pv_done[u], (mine - 1) & 1, gave_up);
+    // Where only the other row tile has keys (a portion that begins inside the prefix), this one's queries are copied too, and nothing above has waited for them: they land
+    // before anything else is put in their place.
+    if (JOINS && mine == 0 && n > 0) ok = warp_wait(&sm.q_full, 0, gave_up);
     if (JOINS) grid_dependency_wait();   // the prefix's parts
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -567,7 +570,8 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
         p.part_ml[at_pair * p.parts + blockIdx.x] = make_float2(reference, row_sum);
       }
       const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-      // A thread has its row, memory wants lines: 16 columns of the warp's 32 rows go through shared memory (Q's place: its products are done), piece i of row r at i ^ (r / 2 % 4).
+      // A thread has its row, memory wants lines: 16 columns of the warp's 32 rows go through shared memory (Q's place: it has landed and its products are done, or it was never
+      // copied), piece i of row r at i ^ (r / 2 % 4).
       // Row r = 8 i + lane / 4, piece lane % 4, is then a lane's i-th, of the prefix's parts too.  (Without parts a thread writes its own row: 32 bytes at a time, and less code to fetch.)
       const int quarter = lane & 3;
       size_t pair_at[4];
