@@ -776,6 +776,9 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
             _F32 if dtype is torch.float32 else _BF16, q_at, q_stride, pages_at, num_pages, positions.data_ptr(), seq_starts.data_ptr(), block_table.data_ptr(), table_width, out_at, scratch.data_ptr(),
             rows, entries, q_heads, kv_heads, head_dim, page_size, shared, scale, prefix_parts, own_parts, error_flag(qkv.device).data_ptr(), _stream())
     _check(status, "shared_prefix_attention")
+    if plan is None or plan[1]:
+        global launch_count
+        launch_count += 1   # two kernels: one that leaves parts, one that brings them together
 
 
 # --- recurrences ---------------------------------------------------------------------------
