@@ -26,3 +26,25 @@ def test_kernels_of_the_general_way_are_counted(ops, dtype, dim):  # noqa: F811
     empty = {**case, "qkv": case["qkv"][:0], "positions": case["positions"][:0], "seq_starts": case["seq_starts"] * 0}
     call_attention(ops, empty)
     assert ops.launch_count - before == 2
+
+
+def test_a_plan_is_for_the_switches_it_is_asked_with():
+    from tinyllama_inference_engine_b200.ops import fast
+
+    sizes = (8, 8, 12, 32, 8, 128, 64, 500)
+    for prefix in (0, 1):
+        for own in (0, 1):
+            for _ in range(2):
+                assert list(fast.shared_prefix_plan(*sizes, prefix, own)[0])[:2] == [prefix, own]
+    assert list(fast.shared_prefix_plan(*sizes, None, None)[0]) == list(fast.shared_prefix_plan(*sizes)[0])
+
+
+@pytest.mark.gpu
+def test_a_switch_holds_for_sizes_seen_before(ops, monkeypatch):  # noqa: F811
+    case = attention_case(33, torch.bfloat16, 8, 2, 64, 16, 100, [(20, 1), (6, 1)])
+    for prefix, own, kernels in ((0, 0, 1), (1, 1, 2), (0, 1, 1), (1, 0, 2), (0, 0, 1)):
+        monkeypatch.setattr(ops.fast, "use_prefix", prefix)
+        monkeypatch.setattr(ops.fast, "use_own", own)
+        before = ops.launch_count
+        call_attention(ops, case)
+        assert ops.launch_count - before == kernels, (prefix, own)

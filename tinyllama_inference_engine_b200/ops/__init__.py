@@ -763,7 +763,7 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     plan = None
     # (the bfloat16 kernels read and write rows 16 bytes at a time and count the pool's rows of keys and values in 31 bits)
     if dtype is torch.bfloat16 and q_stride % 8 == 0 and (q_at | out_at) % 16 == 0 and num_pages * 2 * kv_heads * page_size < 0x7FFFFF00:
-        plan = fast.shared_prefix_plan(rows, entries, table_width, q_heads, kv_heads, head_dim, page_size, shared)
+        plan = fast.shared_prefix_plan(rows, entries, table_width, q_heads, kv_heads, head_dim, page_size, shared, fast.use_prefix, fast.use_own)
     if plan is not None:
         sizes, floats = plan
         scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device) if floats else None

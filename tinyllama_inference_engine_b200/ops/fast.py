@@ -1273,11 +1273,12 @@ def generic_prefix_parts(rows: int, entries: int, group: int, kv_heads: int, hea
 
 
 @functools.lru_cache(maxsize=4096)
-def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_heads: int, head_dim: int, page_size: int, shared: int) -> tuple | None:
+def shared_prefix_plan(rows: int, entries: int, width: int, q_heads: int, kv_heads: int, head_dim: int, page_size: int, shared: int, use_prefix: int | None = None,
+                       use_own: int | None = None) -> tuple | None:
     """Which bfloat16 kernels a call of these sizes runs: (the launcher's numbers, which start with prefix, own, parts and CTAs per row and head; floats of scratch memory).
 
     None: sizes that only the general kernel takes (these take head sizes 64 and 128 and pages of a multiple of 16 keys).  Of the four ways (the shared keys once for all rows or by every row for itself; the rest a row at a time or an entry's rows
-    together) the one that the measured rates above say is fastest."""
+    together) the one that the measured rates above say is fastest; ``use_prefix`` and ``use_own`` (the switches above, which a call hands over) leave fewer of them."""
     group = q_heads // kv_heads
     if head_dim not in SHARED_PREFIX_HEAD_DIMS or page_size % 16 != 0 or group > PREFIX_TC_PAIRS:
         return None
