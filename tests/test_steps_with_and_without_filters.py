@@ -1,0 +1,35 @@
+"""Decode sessions that go from requests with top-k or min-p to requests without and back."""
+from __future__ import annotations
+
+import pytest
+
+import plain_llama
+from test_filtered_generation import _prompts
+from tinyllama_inference_engine_b200 import EngineConfig
+from tinyllama_inference_engine_b200.engine.api import Engine
+from tinyllama_inference_engine_b200.engine.request import SamplingParams
+
+
+@pytest.mark.gpu
+def test_a_session_counts_the_kernels_of_the_steps_it_runs(model_folders):
+    config, _ = plain_llama.load_model(model_folders["b"])
+    prompts = _prompts(config["vocab_size"])[:4]
+    kinds = {"plain": SamplingParams(max_tokens=8, temperature=0.9), "filtered": SamplingParams(max_tokens=8, temperature=0.9, top_k=5)}
+
+    def engine():
+        return Engine(model_folders["b"], EngineConfig(dtype="bfloat16", page_size=16, max_cache_tokens=512, max_requests=4, max_batch_tokens=64))
+
+    def counts(e):
+        session = e._sessions[4]
+        return session.kernels_per_step, session.library_calls_per_step
+
+    alone = {}
+    for kind, params in kinds.items():
+        e = engine()
+        e.generate(prompts, params)
+        alone[kind] = counts(e)
+    assert alone["filtered"][0] == alone["plain"][0] + 2   # the numbers and the choice
+    e = engine()
+    for kind in ("plain", "filtered", "plain", "plain", "filtered", "plain"):
+        e.generate(prompts, kinds[kind])
+        assert counts(e) == alone[kind], kind

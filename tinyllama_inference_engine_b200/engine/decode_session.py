@@ -72,7 +72,7 @@ class DecodeSession:
         self.min_p = torch.zeros(count, dtype=torch.float32, device=device)
         self.uniforms = torch.zeros(count, dtype=torch.float32, device=device)
         self.filtered = False              # whether a loaded request has such options: a step of such requests is a graph of its own
-        self._other: tuple = (0, None, None)   # (steps run kernel by kernel, graph, logits) of the kind of step that ``filtered`` does not say
+        self._other: tuple = (0, None, None, 0, 0)   # (steps run kernel by kernel, graph, logits, kernels and library products of a step) of the kind of step that ``filtered`` does not say
         self.positions = [0] * count      # host mirror: position of the token each request runs next
         self.use_graph = use_graph
         self._fresh = True
@@ -125,7 +125,9 @@ class DecodeSession:
                 self.min_p.copy_(torch.tensor([p.min_p for p in params], dtype=torch.float32))
             if filtered != self.filtered:
                 self.filtered = filtered
-                self._other, (self._eager_steps, self.graph, self.logits) = (self._eager_steps, self.graph, self.logits), self._other
+                mine = (self._eager_steps, self.graph, self.logits, self.kernels_per_step, self.library_calls_per_step)
+                self._eager_steps, self.graph, self.logits, self.kernels_per_step, self.library_calls_per_step = self._other
+                self._other = mine
 
     def _reserve_and_fill_tables(self) -> bool:
         """Pages for this step's positions; returns whether any block-table row changed."""
