@@ -1,13 +1,15 @@
-"""Decode sessions that go from requests with top-k or min-p to requests without and back."""
+"""Decode sessions that go from requests with top-k or min-p to requests without and back, and models whose vocabulary is too long for such requests."""
 from __future__ import annotations
 
 import pytest
 
 import plain_llama
+import plain_ops
 from test_filtered_generation import _prompts
 from tinyllama_inference_engine_b200 import EngineConfig
 from tinyllama_inference_engine_b200.engine.api import Engine
 from tinyllama_inference_engine_b200.engine.request import SamplingParams
+from tinyllama_inference_engine_b200.errors import EngineError
 
 
 @pytest.mark.gpu
@@ -33,3 +35,20 @@ def test_a_session_counts_the_kernels_of_the_steps_it_runs(model_folders):
     for kind in ("plain", "filtered", "plain", "plain", "filtered", "plain"):
         e.generate(prompts, kinds[kind])
         assert counts(e) == alone[kind], kind
+
+
+def test_filters_are_refused_where_the_vocabulary_is_too_long(model_folders, monkeypatch):
+    """ops.sample_filtered takes vocabularies up to a limit: beyond it a request that needs it is refused when it is added, not in the middle of a step."""
+    from tinyllama_inference_engine_b200 import ops
+
+    plain_ops.install(monkeypatch)
+    config, _ = plain_llama.load_model(model_folders["a"])
+    engine = Engine(model_folders["a"], EngineConfig(dtype="float32", page_size=16, max_cache_tokens=512, max_requests=6, max_batch_tokens=32, device="cpu"))
+    monkeypatch.setattr(ops, "SAMPLE_FILTERED_MAX_VOCAB", config["vocab_size"] - 1)
+    for options in (dict(top_k=5), dict(min_p=0.1)):
+        with pytest.raises(EngineError, match=f"{config['vocab_size']} tokens"):
+            engine.add_request([1, 2, 3], SamplingParams(temperature=0.7, **options))
+        engine.add_request([1, 2, 3], SamplingParams(**options))   # (greedy: these options say nothing)
+    assert len(engine.requests) == 2
+    monkeypatch.setattr(ops, "SAMPLE_FILTERED_MAX_VOCAB", config["vocab_size"])
+    engine.add_request([1, 2, 3], SamplingParams(temperature=0.7, top_k=5))

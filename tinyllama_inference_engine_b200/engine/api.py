@@ -12,6 +12,7 @@ import time
 from dataclasses import dataclass, field
 from pathlib import Path
 
+from .. import ops
 from ..config import EngineConfig
 from ..errors import EngineError
 from ..sampling import Sampler
@@ -70,6 +71,8 @@ class Engine:
         for token in prompt:
             if not 0 <= token < vocab:
                 raise EngineError(f"input token {token} is outside the model vocabulary", code="out_of_bounds")
+        if params.filtered and vocab > ops.SAMPLE_FILTERED_MAX_VOCAB:
+            raise EngineError(f"top_k and min_p are for vocabularies of at most {ops.SAMPLE_FILTERED_MAX_VOCAB} tokens, this model has {vocab} tokens")
         request = Request(request_id, prompt, params)
         self.scheduler.add(request)
         self.requests[request_id] = request
