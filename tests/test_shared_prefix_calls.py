@@ -48,3 +48,16 @@ def test_a_switch_holds_for_sizes_seen_before(ops, monkeypatch):  # noqa: F811
         before = ops.launch_count
         call_attention(ops, case)
         assert ops.launch_count - before == kernels, (prefix, own)
+
+
+def test_tables_near_2_to_31_keys_are_refused():
+    """The kernels count keys in 32-bit numbers and look up to 2,048 keys ahead of a request's last one."""
+    from tinyllama_inference_engine_b200 import ops as plain
+    from tinyllama_inference_engine_b200.errors import KernelError
+
+    good = dict(qkv=torch.zeros(3, 4 * 64), pages=torch.zeros(4, 2, 1, 16, 64), positions=torch.zeros(3, dtype=torch.int32), seq_starts=torch.zeros(3, dtype=torch.int32), shared=16,
+                out=torch.zeros(3, 4 * 64), q_heads=4, kv_heads=1, head_dim=64, page_size=16)
+    one = torch.zeros(1, dtype=torch.int32)
+    for width, message in (((1 << 27) - 1, "fewer than 2^31 keys"), ((1 << 27) - 256, "fewer than 2^31 keys"), ((1 << 27) - 257, "contiguous")):   # (the last is let past: what it lacks is something else)
+        with pytest.raises(KernelError, match=message.replace("^", r"\^")):
+            plain.shared_prefix_attention(block_table=one.expand(2, width), **good)

@@ -693,6 +693,10 @@ def _on(device: torch.device):
     return nullcontext() if device.index == _current_device() else torch.cuda.device(device)
 
 
+# The kernels count keys in 32-bit numbers and look up to 2,048 keys (eight CTAs of 16 warps, 16 keys each) ahead of a request's last one.
+SHARED_PREFIX_KEYS_END = (1 << 31) - 4096
+
+
 def _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale) -> None:
     """What of a call of ``shared_prefix_attention`` is wrong."""
     if head_dim % 16 != 0 or not 0 < head_dim <= 256:
@@ -708,8 +712,8 @@ def _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared
         raise KernelError("shared_prefix_attention: pages must be [pages, 2, kv heads, page size, head size] of qkv's dtype", code="invalid_shape")
     if block_table.dim() != 2 or tuple(seq_starts.shape) != (entries + 1,) or tuple(positions.shape) != (rows,):
         raise KernelError("shared_prefix_attention: a block table [entries, pages], seq_starts [entries + 1] and positions [rows]", code="invalid_shape")
-    if block_table.shape[1] * page_size >= 1 << 31:
-        raise KernelError("shared_prefix_attention: a block-table row reaches fewer than 2^31 keys", code="invalid_shape")
+    if block_table.shape[1] * page_size >= SHARED_PREFIX_KEYS_END:
+        raise KernelError("shared_prefix_attention: a block-table row reaches at least 4,096 keys fewer than 2^31 keys", code="invalid_shape")
     if isinstance(shared, bool) or not isinstance(shared, int) or not 0 <= shared <= block_table.shape[1] * page_size:
         raise KernelError(f"shared_prefix_attention: shared must be a whole number from 0 to the {block_table.shape[1] * page_size} keys that a block-table row reaches, got {shared!r}",
                           code="invalid_argument")
@@ -736,6 +740,7 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     keys may lie in the rest of that page or of its copy.  An entry brings any number of rows, none included.  Rows in front of ``seq_starts[0]`` and behind ``seq_starts[-1]`` are left as they
     were; a row that sees no key (a negative position) becomes zero.  Positions that the block table does not reach and pages outside the pool are reported in
     the device's error word.  ``scale``: positive, ``head_dim ** -0.5`` by default.  32-bit or bfloat16, head sizes that are multiples of 16 up to 256.
+    Block-table rows that reach 2^31 - 4,096 keys or more are refused.
 
     Called inside the capture of a CUDA graph, the graph keeps ``shared`` and the tensors' addresses; what the tensors hold may change from replay to replay."""
     scale = head_dim ** -0.5 if scale is None else float(scale)
@@ -750,7 +755,7 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
             and index == pages.get_device() == out.get_device() == positions.get_device() == seq_starts.get_device() == block_table.get_device()
             and 0 < head_dim <= 256 and head_dim % 16 == 0 and 0 < kv_heads <= q_heads and q_heads % kv_heads == 0 and width >= q_heads * head_dim
             and out.shape == (rows, q_heads * head_dim) and num_pages > 0 and two == 2 and page_heads == kv_heads and page_keys == page_size and page_dim == head_dim
-            and positions.shape == (rows,) and seq_starts.shape == (entries + 1,) and type(shared) is int and 0 <= shared <= table_width * page_size < 1 << 31
+            and positions.shape == (rows,) and seq_starts.shape == (entries + 1,) and type(shared) is int and 0 <= shared <= table_width * page_size < SHARED_PREFIX_KEYS_END
             and 0.0 < scale < float("inf") and (q_step == 1 or rows == 0) and pages.is_contiguous() and pages_at % 16 == 0 and out.is_contiguous()
             and positions.is_contiguous() and seq_starts.is_contiguous() and block_table.is_contiguous()):
         _refuse_shared_prefix(qkv, pages, positions, seq_starts, block_table, shared, out, q_heads, kv_heads, head_dim, page_size, scale)
