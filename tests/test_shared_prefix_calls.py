@@ -61,3 +61,36 @@ def test_tables_near_2_to_31_keys_are_refused():
     for width, message in (((1 << 27) - 1, "fewer than 2^31 keys"), ((1 << 27) - 256, "fewer than 2^31 keys"), ((1 << 27) - 257, "contiguous")):   # (the last is let past: what it lacks is something else)
         with pytest.raises(KernelError, match=message.replace("^", r"\^")):
             plain.shared_prefix_attention(block_table=one.expand(2, width), **good)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+def test_an_error_word_made_inside_a_capture_keeps_what_it_holds(ops, dtype, monkeypatch):  # noqa: F811
+    """The first call of a process may be a captured one: the device's error word is no part of that graph, whose replays leave what other work has reported."""
+    from tinyllama_inference_engine_b200.errors import KernelError
+
+    case = attention_case(34, dtype, 8, 2, 64, 16, 40, [(20, 1), (6, 1)], poison=False)
+    c = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in case.items()}
+    out = torch.zeros(2, 512, dtype=dtype, device="cuda")
+    device = torch.device("cuda:0")
+    call_attention(ops, case)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(ops, "_error_flags", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.shared_prefix_attention(c["qkv"], c["pages"], c["positions"], c["seq_starts"], c["table"], c["shared"], out, 8, 2, 64, 16)
+    ops.check_device_errors(device)   # nothing has run
+    ops.error_flag(device).fill_(4)
+    graph.replay()
+    with pytest.raises(KernelError, match="learned position vectors"):
+        ops.check_device_errors(device)
+    graph.replay()
+    ops.check_device_errors(device)
+    c["table"][0, 1] = 1 << 30
+    for _ in range(2):   # what a replay reports is not lost to the next one
+        graph.replay()
+    c["table"].copy_(case["table"])
+    graph.replay()
+    with pytest.raises(KernelError, match="outside the pool"):
+        ops.check_device_errors(device)
+    assert torch.equal(out, call_attention(ops, case))

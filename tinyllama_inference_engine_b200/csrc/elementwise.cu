@@ -557,3 +557,18 @@ TLIE_EXPORT int tlie_activation(int dtype, int kind, const void* in, void* out, 
     activation_kernel<__nv_bfloat16><<<grid_for(count, 256), 256, 0, stream>>>((const __nv_bfloat16*)in, (__nv_bfloat16*)out, kind, a, b, (size_t)count);
   return (int)cudaGetLastError();
 }
+
+// New memory on the current device with zeros in it, there when this returns: no part of what the calling thread captures.
+TLIE_EXPORT int tlie_zeros_now(void** memory, long long bytes) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // (this thread's: what follows has nothing to do with a capture)
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return (int)e;
+  cudaStream_t stream = nullptr;
+  e = cudaMalloc(memory, (size_t)bytes);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(*memory, 0, (size_t)bytes, stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (stream != nullptr) cudaStreamDestroy(stream);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  return (int)e;
+}

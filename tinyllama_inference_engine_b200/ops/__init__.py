@@ -114,8 +114,28 @@ def error_flag(device: torch.device) -> torch.Tensor:
         return found
     device = torch.device(device)
     if device not in _error_flags:
-        _error_flags[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        _error_flags[device] = _new_error_flag(device)
     return _error_flags[device]
+
+
+def _new_error_flag(device: torch.device) -> torch.Tensor:
+    if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+        return torch.zeros(1, dtype=torch.int32, device=device)
+    # Inside the capture of a graph: the word must be no part of it.  Replays would clear what other work has reported, and memory of the graph's allocator may also be that of
+    # another graph's intermediate results.
+    place = c_void_p()
+    with torch.cuda.device(device):
+        status = core().tlie_zeros_now(ctypes.byref(place), c_longlong(4))
+    if status != 0:
+        raise KernelError(f"the device's error word could not be made: CUDA error {status}")
+    return torch.as_tensor(_DeviceWord(place.value), device=device)
+
+
+class _DeviceWord:
+    """An int32 in device memory that stays for as long as the process, as torch takes it over."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 3}
 
 
 def raise_for_error_word(word: int, device: torch.device) -> None:
