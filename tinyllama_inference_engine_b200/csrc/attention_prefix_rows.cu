@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) prefix_rows_kernel(PrefixRo
     const float p2 = exp2_approx(fmaf(s[2], to_log2, -base[0])), p3 = exp2_approx(fmaf(s[3], to_log2, -base[1]));
     sum[0] = fmaf(sum[0], shrink[0], p0 + p2);
     sum[1] = fmaf(sum[1], shrink[1], p1 + p3);
-    // a weight keeps 8 bits where it meets its value, as in the other bfloat16 attention kernels
+    // a weight keeps 8 bits where it meets its value, as in the other bfloat16 attention kernels (the product takes bfloat16): an error like that of the output's own rounding
     const unsigned w0 = transpose_8x8(pack_bf16(p0, p1)), w1 = transpose_8x8(pack_bf16(p2, p3));
     if (__any_sync(0xffffffffu, shrink[0] != 1.0f || shrink[1] != 1.0f)) {
 #pragma unroll

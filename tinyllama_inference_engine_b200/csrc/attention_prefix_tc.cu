@@ -516,7 +516,9 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
         unpair(fma2(pair_of(sc[2 * i], sc[2 * i + 1]), scale2, minus_base2), x0, x1);
         const float p0 = exp2_approx(x0), p1 = exp2_approx(x1);
         sums = add2(sums, pair_of(p0, p1));
-        packed[i] = pack_bf16(p0, p1);   // a weight keeps 8 bits where it meets its value, as in the other bfloat16 attention kernels; the sum has all of it
+        // A weight keeps 8 bits where it meets its value, as in the other bfloat16 attention kernels (the product takes bfloat16); the sum has all of it.  Over some thousand keys
+        // that is an error of 1.6e-3 of the output, as much as the output's own rounding.
+        packed[i] = pack_bf16(p0, p1);
       }
       if (lane == 0 && j >= 0) mbar_arrive(&sm.exps_done[u][sub]);
       if (j > 0 && ok) ok = warp_wait(&sm.pv_done[u], (j - 1) & 1, gave_up);   // the weights before have been read
@@ -536,7 +538,8 @@ __global__ void __launch_bounds__(kThreadsTC, 1)
         row_sum = 0.0f;
       }
     };
-    // Tiles that every row sees all of, then the others: what the masks take stays out of the loop that counts (with it inside, every tile took a fifth longer).
+    // Tiles that every row sees all of, then the others: what the masks take stays out of the loop that counts (with it inside, every tile took a fifth longer).  Own keys behind a prefix that
+    // ends inside a tile all go through the other loop, for their first tile's sake.
     const int all_seen = JOINS && p.first_key % kKeys != 0 ? 0 : max(0, min(mine, lowest / kKeys - kt_begin));
     int j = -1;
     for (; mine > 0 && j < all_seen; ++j) take_tile(j, std::false_type{});

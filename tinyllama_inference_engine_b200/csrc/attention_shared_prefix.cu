@@ -13,6 +13,8 @@
 // ten.  (With one thread to a score and one to a channel the four rows below took 104 us.)  All sums are
 // 32-bit.  Bound by reads of shared memory where there are many rows (480 rows, 32 heads of 64 over 4, 900 shared and up to 200 own keys: 218 us for 3.7 GFLOP, shared memory busy 60% of the
 // time), by the chain of a chunk's steps where there are few (so runs are short there): 4 rows of the same heads behind 500 keys take 12 us, 5 of them for joining the parts.
+// bfloat16 heads of other sizes than 64 and 128 come here too and are worked out on 32-bit numbers: 8 rows, 32 heads of 96 over 8, 1,024 shared and 30 own keys: 23 us; 64 rows, 700 and 200: 225, where the
+// kernel for single rows that shares nothing (attention_decode.cu, head sizes up to 128) takes 34; 16 rows, 16 heads of 256, 1,000 and 100: 383, where the general kernel that shares nothing takes 1,120.
 #include "common.cuh"
 #include "mma_utils.cuh"
 #include "shared_memory_limit.cuh"

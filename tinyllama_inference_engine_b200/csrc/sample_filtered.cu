@@ -78,7 +78,8 @@ struct Border {
 //
 // Where the list does not do (top_k beyond it, flat rows), a border is found from a histogram over 2,048 runs of logits, 1/64 wide, below the largest, of numbers or
 // of exact weights, and from the tokens of the run that it falls in, which the first CTA sorts.  Where those are too many (equal logits, or very close ones) the run is
-// cut by the bits of the logits, and equal ones by id.  (One row of 32,000 with top-k 450: 48 us; 160 rows of 128,256 with top-k 400: 433, with 300, on the list: 71; 64 rows at a temperature of 3 with top-p alone: 134.)
+// cut by the bits of the logits, and equal ones by id.  (One row of 32,000 with top-k 450: 33 us, 47 with top-p 0.95 beside it; 160 rows of 128,256 with top-k 400: 313 and 435, with 300, on the list: 76 and 74; 64 rows at a
+// temperature of 3 with top-p alone: 125.)
 struct FilterShared {
   union {                         // (one is done with before the other begins)
     struct {
@@ -847,7 +848,8 @@ TLIE_EXPORT int tlie_sample_filtered(const float* logits, long long row_stride, 
   if (vocab <= 0 || vocab > kFilterMaxVocab || row_stride < 0) return (int)cudaErrorInvalidValue;
   // CTAs of a row's cluster, with at least 8,192 tokens each where there are two and more: one per SM in all, or two if each has 16,384 tokens (clusters of four and eight do not fill every
   // SM: nine tenths of that).  us, by halving the CTAs: 120 rows of 32,000 without options 12.9 -> 9.5 (one per SM), 40 rows of 128,256 under top-p 26.8 -> 29.4 (one per SM; two are taken); 74 rows of 128,256
-  // under top-p in 296 CTAs 43.5, in 148 30.2.
+  // under top-p in 296 CTAs 43.5, in 148 30.2.  The rule knows sizes only (the options lie on the device) and was fitted to rows under top-p.  Its steps show with every option where rows lose a CTA:
+  // 148 -> 149 rows of 128,256 take 47 -> 61 us without options, 51 -> 64 under top-p, 35.2 -> 35.5 with top-k 50.
   const int sms = device_sm_count();
   int ctas = 1;
   while (ctas < 8 && vocab > ctas * 8192) {

@@ -760,7 +760,8 @@ def shared_prefix_attention(qkv, pages, positions, seq_starts, block_table, shar
     keys may lie in the rest of that page or of its copy.  An entry brings any number of rows, none included.  Rows in front of ``seq_starts[0]`` and behind ``seq_starts[-1]`` are left as they
     were; a row that sees no key (a negative position) becomes zero.  Positions that the block table does not reach and pages outside the pool are reported in
     the device's error word.  ``scale``: positive, ``head_dim ** -0.5`` by default.  32-bit or bfloat16, head sizes that are multiples of 16 up to 256.
-    Block-table rows that reach 2^31 - 4,096 keys or more are refused.
+    Block-table rows that reach 2^31 - 4,096 keys or more are refused.  bfloat16 heads of 64 and 128 run on the tensor cores, everything else on 32-bit numbers: single bfloat16 rows of
+    other head sizes up to 128 are faster through ``paged_attention`` (64 rows, 32 heads of 96 over 8, 700 shared and 200 own keys: 225 us here, 34 there).
 
     Called inside the capture of a CUDA graph, the graph keeps ``shared`` and the tensors' addresses; what the tensors hold may change from replay to replay."""
     scale = head_dim ** -0.5 if scale is None else float(scale)
